@@ -177,6 +177,57 @@ NineToothedResult launch_addmm_allgather_multicast(NineToothedStream stream, Nin
                                                    NineToothedTensor output, void *multicast_output, int dtype);
 
 /*
+ * Products whose matrix is chosen by the row (no counterpart in the reference, whose definitions tile
+ * dense tensors; beside matmul and bmm here).  The rows of lhs [T, K] form contiguous runs: run e is the
+ * rows offsets[e] <= t < offsets[e + 1] of a mixture-of-experts layer's expert e, say.  `offsets` is a
+ * DEVICE array of runs + 1 int32 or int64 bounds (offsets_dtype: NINETOOTHED_INT32 or NINETOOTHED_INT64),
+ * read by the kernels only: the call neither waits for it nor copies it, so that it may be captured into
+ * a graph and replayed on other bounds.  Bounds should not decrease; they are clamped to 0 .. T and one
+ * that lies below an earlier one counts as that one, so no offsets reach outside the tensors.  Runs may be
+ * empty, at most 2048 of them.  Rows that no run holds (before offsets[0], from the last bound on) are
+ * neither computed nor written.
+ *
+ * launch_grouped_matmul: output[t] = lhs[t] . rhs[e] for the rows t of run e; rhs [E, K, N], output [T, N].
+ * The gradient towards lhs is the same call on the transposed view of rhs ([E, N, K], unit stride along N).
+ * launch_grouped_matmul_rhs_grad: rhs_grad[e] = sum over the rows t of run e of lhs[t]^T output_grad[t];
+ * lhs [T, M], output_grad [T, N], rhs_grad [E, M, N]; the gradient of an empty run is zero.
+ * fp32 accumulation, one rounding at the store, sums in an order that depends on the sizes only.
+ * dtype: FLOAT16 or BFLOAT16.  Any strides; operands that no TMA descriptor can address run on plain
+ * kernels (ninetoothed_b200_plain_launches).  No device memory is allocated.
+ */
+NineToothedResult launch_grouped_matmul(NineToothedStream stream, NineToothedTensor lhs, NineToothedTensor rhs,
+                                        NineToothedTensor offsets, NineToothedTensor output, int dtype,
+                                        int offsets_dtype);
+
+NineToothedResult launch_grouped_matmul_rhs_grad(NineToothedStream stream, NineToothedTensor lhs,
+                                                 NineToothedTensor output_grad, NineToothedTensor offsets,
+                                                 NineToothedTensor rhs_grad, int dtype, int offsets_dtype);
+
+/*
+ * A projection shared by all rows with low-rank adapters of many requests beside it (no counterpart in the
+ * reference): output[t] = lhs[t] . rhs + scales[a] * (lhs[t] . down[a]) . up[a], where a = adapters[s] is the
+ * adapter of the request s that holds row t (offsets[s] <= t < offsets[s + 1], by the rules above; at most 2048
+ * requests).  lhs [T, K], rhs [K, N], down [L, K, R], up [L, R, N], output [T, N] of `dtype`; scales [L] is
+ * a DEVICE array of float; adapters [S] a DEVICE array of int32 or int64 (adapters_dtype).  Requests may
+ * share an adapter; an index outside 0 .. L - 1 (-1, say) means none: the row gets lhs[t] . rhs alone.  Rows
+ * of no request are not written, and nothing of one request's adapter, infinities and NaN included, reaches
+ * another request's rows.  The gradient towards lhs is the same call on transposed views, with up and down
+ * in each other's place.
+ *
+ * Sums are fp32.  scales[a] * (lhs[t] . down[a]) is kept between the two products as the sum of two numbers
+ * of `dtype` (in fp16 it overflows beyond 65504).  `workspace` is device memory of at least
+ * launch_lora_matmul_workspace_size(lhs, down) bytes, 256-byte aligned, free to reuse once the stream has
+ * passed this call; calls that may overlap need one each.
+ */
+NineToothedResult launch_lora_matmul(NineToothedStream stream, NineToothedTensor lhs, NineToothedTensor rhs,
+                                     NineToothedTensor down, NineToothedTensor up, NineToothedTensor scales,
+                                     NineToothedTensor offsets, NineToothedTensor adapters,
+                                     NineToothedTensor output, int dtype, int offsets_dtype, int adapters_dtype,
+                                     void *workspace, size_t workspace_size);
+
+size_t launch_lora_matmul_workspace_size(NineToothedTensor lhs, NineToothedTensor down);
+
+/*
  * Row softmax over the last dimension of a 2-D tensor, fp32 math, one program
  * per row (tests/test_softmax.py:10-27).  dtype of input and output: FLOAT16,
  * BFLOAT16 or FLOAT32.

@@ -35,6 +35,10 @@ ENTRY_POINTS = (
     "launch_addmm",
     "launch_addmm_allgather",
     "launch_addmm_allgather_multicast",
+    "launch_grouped_matmul",
+    "launch_grouped_matmul_rhs_grad",
+    "launch_lora_matmul",
+    "launch_lora_matmul_workspace_size",
     "launch_softmax",
     "launch_attention",
     "launch_attention_scaled",
@@ -106,6 +110,11 @@ def library() -> ctypes.CDLL:
             lib.launch_addmm.argtypes = [S, T, T, T, T, T, T, I]
             lib.launch_addmm_allgather.argtypes = [S, T, T, T, T, T, T, ctypes.POINTER(ctypes.c_void_p), I, I, I]
             lib.launch_addmm_allgather_multicast.argtypes = [S, T, T, T, T, T, T, ctypes.c_void_p, I]
+            lib.launch_grouped_matmul.argtypes = [S, T, T, T, T, I, I]
+            lib.launch_grouped_matmul_rhs_grad.argtypes = [S, T, T, T, T, I, I]
+            lib.launch_lora_matmul.argtypes = [S, T, T, T, T, T, T, T, T, I, I, I, ctypes.c_void_p, ctypes.c_size_t]
+            lib.launch_lora_matmul_workspace_size.argtypes = [T, T]
+            lib.launch_lora_matmul_workspace_size.restype = ctypes.c_size_t
             lib.launch_softmax.argtypes = [S, T, T, I]
             lib.launch_attention.argtypes = [S, T, T, T, T, T, I]
             lib.launch_attention_scaled.argtypes = [S, T, T, T, T, T, T, I]
@@ -284,6 +293,89 @@ def addmm_allgather_multicast(input, mat1, mat2, beta, alpha, output_slab, multi
     c, kc = tensor_arg(output_slab)
     _call("launch_addmm_allgather_multicast", device, i, a, b, be, al, c, ctypes.c_void_p(int(multicast_slab_ptr)),
           dtype_index(mat1))
+
+
+def _validate_aside(kernel, label, t, dtypes):
+    """A 1-D tensor beside the operands (run bounds, adapter indices, scales), of a type of its own."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{kernel}: {label} must be a torch.Tensor, got {type(t).__name__}")
+    if t.ndim != 1:
+        raise ValueError(f"{kernel}: {label} must have 1 dimension, got shape {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{kernel}: {label} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
+
+
+_INDEX_DTYPES = (torch.int32, torch.int64)
+
+
+def grouped_matmul(lhs, rhs, offsets, output):
+    """``output[t] = lhs[t] @ rhs[e]`` for the rows ``offsets[e] <= t < offsets[e + 1]``; other rows stay as they were.
+
+    lhs [T, K], rhs [E, K, N], offsets [E + 1] (int32 or int64, on the device: never read back), output [T, N].  The
+    gradient towards lhs is ``grouped_matmul(output_grad, rhs.transpose(1, 2), offsets, lhs_grad)``."""
+    _validate("grouped_matmul", lhs=(lhs, 2), rhs=(rhs, 3), output=(output, 2))
+    _validate_aside("grouped_matmul", "offsets", offsets, _INDEX_DTYPES)
+    device = _require_cuda(lhs, rhs, offsets, output)
+    a, ka = tensor_arg(lhs)
+    b, kb = tensor_arg(rhs)
+    o, ko = tensor_arg(offsets)
+    c, kc = tensor_arg(output)
+    _call("launch_grouped_matmul", device, a, b, o, c, dtype_index(lhs), dtype_index(offsets))
+
+
+def grouped_matmul_rhs_grad(lhs, output_grad, offsets, rhs_grad):
+    """``rhs_grad[e] = lhs[a:b].T @ output_grad[a:b]`` with ``a, b = offsets[e], offsets[e + 1]`` (zeros for an empty run).
+
+    lhs [T, M], output_grad [T, N], offsets [E + 1], rhs_grad [E, M, N]: the gradient of ``grouped_matmul`` towards rhs."""
+    _validate("grouped_matmul_rhs_grad", lhs=(lhs, 2), output_grad=(output_grad, 2), rhs_grad=(rhs_grad, 3))
+    _validate_aside("grouped_matmul_rhs_grad", "offsets", offsets, _INDEX_DTYPES)
+    device = _require_cuda(lhs, output_grad, offsets, rhs_grad)
+    a, ka = tensor_arg(lhs)
+    b, kb = tensor_arg(output_grad)
+    o, ko = tensor_arg(offsets)
+    c, kc = tensor_arg(rhs_grad)
+    _call("launch_grouped_matmul_rhs_grad", device, a, b, o, c, dtype_index(lhs), dtype_index(offsets))
+
+
+def lora_matmul_workspace_size(lhs, down) -> int:
+    _validate("lora_matmul", lhs=(lhs, 2), down=(down, 3))
+    a, ka = tensor_arg(lhs)
+    d, kd = tensor_arg(down)
+    return int(library().launch_lora_matmul_workspace_size(a, d))
+
+
+def lora_matmul(lhs, rhs, down, up, scales, offsets, adapters, output, workspace=None):
+    """``output[t] = lhs[t] @ rhs + scales[a] * (lhs[t] @ down[a]) @ up[a]``, a = adapters[s] for the request s whose rows
+    ``offsets[s] <= t < offsets[s + 1]`` hold t; an index outside ``0 .. L - 1`` means no adapter, rows of no request
+    stay as they were.
+
+    lhs [T, K], rhs [K, N], down [L, K, R], up [L, R, N], scales [L] (float32), offsets [S + 1] and adapters [S] (int32 or
+    int64), output [T, N].  The gradient towards lhs is the same call on ``output_grad, rhs.t(), up.transpose(1, 2),
+    down.transpose(1, 2)``."""
+    _validate("lora_matmul", lhs=(lhs, 2), rhs=(rhs, 2), down=(down, 3), up=(up, 3), output=(output, 2))
+    _validate_aside("lora_matmul", "scales", scales, (torch.float32,))
+    _validate_aside("lora_matmul", "offsets", offsets, _INDEX_DTYPES)
+    _validate_aside("lora_matmul", "adapters", adapters, _INDEX_DTYPES)
+    device = _require_cuda(lhs, rhs, down, up, scales, offsets, adapters, output)
+    a, ka = tensor_arg(lhs)
+    b, kb = tensor_arg(rhs)
+    d, kd = tensor_arg(down)
+    u, ku = tensor_arg(up)
+    s, ks = tensor_arg(scales)
+    o, ko = tensor_arg(offsets)
+    i, ki = tensor_arg(adapters)
+    c, kc = tensor_arg(output)
+    size = int(library().launch_lora_matmul_workspace_size(a, d))
+    if workspace is None:
+        workspace = torch.empty(max(size, 1), dtype=torch.uint8, device=device)
+    else:
+        if _require_cuda(workspace) != device:
+            raise RuntimeError(f"lora_matmul workspace lives on {workspace.device}, the tensors on {device}")
+        if not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < size:
+            raise ValueError(f"lora_matmul workspace holds {workspace.numel() * workspace.element_size()} bytes, needs {size}"
+                             " (contiguous)")
+    _call("launch_lora_matmul", device, a, b, d, u, s, o, i, c, dtype_index(lhs), dtype_index(offsets),
+          dtype_index(adapters), ctypes.c_void_p(workspace.data_ptr()), ctypes.c_size_t(size))
 
 
 def softmax(input, output):

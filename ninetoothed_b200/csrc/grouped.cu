@@ -1,0 +1,1300 @@
+// Products whose weight matrix is chosen by the row: the rows of lhs form contiguous runs whose bounds lie on the
+// device, and every run has its own matrix.
+//
+//   grouped_matmul           output[t] = lhs[t] . rhs[e]                       for the rows t of run e
+//   grouped_matmul_rhs_grad  rhs_grad[e] = sum over the rows t of run e of lhs[t]^T output_grad[t]
+//   lora_matmul              output[t] = lhs[t] . rhs + scales[a] (lhs[t] . down[a]) . up[a],  a the adapter of t's run
+//
+// Nothing is read back to the host: every CTA turns the offsets into a table of runs in shared memory (bounds are
+// clamped by a running maximum, so no offsets can lead out of the tensors) and walks the tiles that follow from it.
+//
+// Persistent CTAs of six warps: a TMA producer, an MMA issuer, four epilogue warps; a ring of shared-memory stages;
+// two accumulator buffers in tensor memory, so that a tile's epilogue runs under the next tile's products.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+
+#include "host.h"
+#include "ptx.cuh"
+
+namespace nt {
+namespace {
+
+constexpr int BM = 128;  // accumulator rows per CTA
+constexpr int BK = 64;   // 64 16-bit elements: one 128-byte swizzle row
+constexpr int UMMA_K = 16;
+constexpr int A_STAGE_BYTES = BM * BK * 2;
+constexpr int A_CHUNK_ROWS = 32;  // short tiles load only the 32-row boxes that hold rows of theirs
+constexpr int NUM_THREADS = 192;
+constexpr int TMEM_COLS = 512;
+constexpr int MAX_STAGES = 8;
+constexpr int GROUP_ROWS = 16;  // tile-rows of 128 that share a raster group (L2 reuse of a run's weight panels)
+constexpr int MAX_RUNS = 2048;  // the table of runs is 16 bytes a run of shared memory
+constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product: 32 high parts, 32 low parts
+
+enum Mode {
+    PRODUCT,  // tiles of every run, matrix of the run
+    SHRINK,   // the same over the runs that have an adapter; the result is kept as two 16-bit parts
+    LORA,     // tiles over all rows with one matrix; each run's second product is added into its own rows
+};
+
+template <int CG, int BN>
+struct Shape {
+    static constexpr int BN_CTA = BN / CG;
+    static constexpr int B_STAGE_BYTES = BN_CTA * BK * 2;
+    static constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
+    static constexpr int STAGES = 192 * 1024 / STAGE_BYTES < MAX_STAGES ? 192 * 1024 / STAGE_BYTES : MAX_STAGES;
+    static constexpr int TILE_M = BM * CG;
+};
+
+struct Control {
+    uint64_t full[MAX_STAGES];
+    uint64_t empty[MAX_STAGES];
+    uint64_t tmem_full[2];
+    uint64_t tmem_empty[2];
+    uint32_t tmem_base;
+    uint32_t abort_flag;
+    int runs;        // entries of the table
+    int tiles_m;     // tile-rows of all runs
+    int row_begin;   // rows covered by the offsets
+    int row_end;
+};
+
+// One run of the table: rows [begin, end), the matrix it uses, the tile-rows of the runs before it.
+struct Run {
+    int begin, end, matrix, tiles_before;
+};
+
+constexpr int CONTROL_BYTES = 256;
+static_assert(sizeof(Control) <= CONTROL_BYTES, "control block");
+
+constexpr size_t table_bytes(int runs) { return static_cast<size_t>(runs + 1) * sizeof(Run); }
+
+template <int CG, int BN>
+size_t smem_bytes(int runs) {
+    return 1024 + Shape<CG, BN>::STAGES * Shape<CG, BN>::STAGE_BYTES + CONTROL_BYTES + table_bytes(runs);
+}
+
+struct Offsets {
+    const void *data;
+    int64_t stride;
+    int wide;   // int64 elements, otherwise int32
+    int runs;   // offsets holds runs + 1 bounds
+};
+
+struct Params {
+    Offsets offsets;
+    const void *adapters;  // matrix of every run (nullptr: run e uses matrix e)
+    int64_t adapters_stride;
+    int adapters_wide;
+    int matrices;  // runs whose matrix lies outside 0 .. matrices - 1 have none
+    int rows, n, k;
+    int n_tiles, k_blocks, group_m;
+    int bf16;
+    void *out;
+    int64_t out_stride0, out_stride1, out_batch_stride;
+    int out_vec;  // rows of output are 16-byte addressable
+    uint32_t b_lbo;
+    // adapters
+    const float *scales;
+    int64_t scales_stride;
+    int rank, rank_blocks;
+    int up_mn;  // up has unit stride along its columns, otherwise along its ranks
+    unsigned int *status;
+};
+
+__device__ __forceinline__ int load_index(const void *data, int64_t stride, int wide, int i, int low, int high) {
+    const int64_t at = stride * i;
+    const int64_t v = wide ? static_cast<const int64_t *>(data)[at] : static_cast<const int32_t *>(data)[at];
+    return static_cast<int>(v < low ? low : v > high ? high : v);
+}
+
+// Fills the table with the runs that have rows (and, where adapters are given, an adapter), in row order.  All
+// threads of the CTA call it; the table is complete after the next __syncthreads().  Bounds outside 0 .. rows are
+// clamped and a bound below an earlier one counts as that one, so that runs never overlap or leave the tensor.
+__device__ __forceinline__ void build_table(const Params &p, Run *table, Control *ctl, int tile_m) {
+    const int runs = p.offsets.runs;
+    for (int i = threadIdx.x; i <= runs; i += blockDim.x) {
+        table[i].begin = load_index(p.offsets.data, p.offsets.stride, p.offsets.wide, i, 0, p.rows);
+        int matrix = i;
+        if (p.adapters != nullptr && i < runs)
+            matrix = load_index(p.adapters, p.adapters_stride, p.adapters_wide, i, -1, p.matrices);
+        table[i].matrix = matrix;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    const int lane = threadIdx.x;
+    const int first = table[0].begin;
+    int bound = first, count = 0, tiles = 0;
+    for (int base = 0; base < runs; base += 32) {
+        const int i = base + lane;
+        int end = i < runs ? table[i + 1].begin : 0;
+        const int matrix = i < runs ? table[i].matrix : -1;
+        __syncwarp();  // (entries are written below at places this chunk has read)
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int other = __shfl_up_sync(0xffffffffu, end, d);
+            if (lane >= d) end = max(end, other);
+        }
+        end = max(end, bound);
+        int begin = __shfl_up_sync(0xffffffffu, end, 1);
+        if (lane == 0) begin = bound;
+        const bool kept = i < runs && end > begin && matrix >= 0 && matrix < p.matrices;
+        const unsigned votes = __ballot_sync(0xffffffffu, kept);
+        const int own_tiles = kept ? (end - begin + tile_m - 1) / tile_m : 0;
+        int before = own_tiles;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int other = __shfl_up_sync(0xffffffffu, before, d);
+            if (lane >= d) before += other;
+        }
+        if (kept) {
+            // (at most entry `base + lane`; the bound of entry base + 32, still to be read as a next bound's
+            // predecessor, is carried in `bound`)
+            table[count + __popc(votes & ((1u << lane) - 1))] = Run{begin, end, matrix, tiles + before - own_tiles};
+        }
+        count += __popc(votes);
+        tiles += __shfl_sync(0xffffffffu, before, 31);
+        bound = __shfl_sync(0xffffffffu, end, 31);
+        __syncwarp();
+    }
+    if (lane == 0) {
+        ctl->runs = count;
+        ctl->tiles_m = tiles;
+        ctl->row_begin = first;
+        ctl->row_end = bound;
+    }
+}
+
+// Where a tile lies: its first row, the end of the rows it may write, its first column, its matrix.
+struct Place {
+    int row0, row_end, col0, matrix;
+};
+
+__device__ __forceinline__ void raster(int tile, int m_tiles, int n_tiles, int group_m, int &m, int &n) {
+    const int per_group = group_m * n_tiles;
+    const int group = tile / per_group;
+    const int first = group * group_m;
+    const int height = min(m_tiles - first, group_m);
+    const int inside = tile - group * per_group;
+    m = first + inside % height;
+    n = inside / height;
+    if (group & 1) n = n_tiles - 1 - n;  // odd groups walk back, starting on the panels the previous one ended on
+}
+
+// The tiles of one worker in order; every warp role walks its own copy.
+template <Mode MODE, int TILE_M, int BN>
+struct Walk {
+    const Run *table;
+    int tile, total, stride, runs, run;
+    int range_begin, range_end, range_tiles;
+
+    __device__ Walk(const Params &p, const Run *table_, const Control *ctl, int worker, int workers)
+        : table(table_), tile(worker), stride(workers), runs(ctl->runs), run(0) {
+        range_begin = ctl->row_begin;
+        range_end = ctl->row_end;
+        range_tiles = MODE == LORA ? (range_end - range_begin + TILE_M - 1) / TILE_M : ctl->tiles_m;
+        total = range_tiles * p.n_tiles;
+        if (MODE != LORA && tile < total) {
+            int low = 0, high = runs - 1;  // the last run whose first tile is not behind this one
+            while (low < high) {
+                const int mid = (low + high + 1) >> 1;
+                if (table[mid].tiles_before * p.n_tiles <= tile) low = mid;
+                else high = mid - 1;
+            }
+            run = low;
+        }
+    }
+    __device__ bool more() const { return tile < total; }
+    __device__ void advance() { tile += stride; }
+    __device__ Place place(const Params &p) {
+        int m, n;
+        if constexpr (MODE == LORA) {
+            raster(tile, range_tiles, p.n_tiles, p.group_m, m, n);
+            return {range_begin + m * TILE_M, range_end, n * BN, 0};
+        } else {
+            while (run + 1 < runs && table[run + 1].tiles_before * p.n_tiles <= tile) ++run;
+            const Run r = table[run];
+            const int m_tiles = (r.end - r.begin + TILE_M - 1) / TILE_M;
+            raster(tile - r.tiles_before * p.n_tiles, m_tiles, p.n_tiles, p.group_m, m, n);
+            return {r.begin + m * TILE_M, r.end, n * BN, r.matrix};
+        }
+    }
+};
+
+// First run of the table that ends behind `row`.
+__device__ __forceinline__ int first_run_behind(const Run *table, int runs, int row) {
+    int low = 0, high = runs;
+    while (low < high) {
+        const int mid = (low + high) >> 1;
+        if (table[mid].end > row) high = mid;
+        else low = mid + 1;
+    }
+    return low;
+}
+
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// D[tmem] += A[smem] . B[smem] into some of the accumulator's rows only: the lanes set in `off` keep their values.
+template <int CG>
+__device__ __forceinline__ void umma_ss_lanes(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                              const uint32_t (&off)[8]) {
+    if constexpr (CG == 1) {
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, 1, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t"
+            "}\n"
+            :
+            : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, 1, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t"
+            "}\n"
+            :
+            : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]),
+              "r"(off[4]), "r"(off[5]), "r"(off[6]), "r"(off[7])
+            : "memory");
+    }
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
+    uint32_t packed;
+    if (bf16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        packed = *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(a, b);
+        packed = *reinterpret_cast<const uint32_t *>(&v);
+    }
+    return packed;
+}
+
+__device__ __forceinline__ float round16(float v, bool bf16) {
+    return bf16 ? __bfloat162float(__float2bfloat16_rn(v)) : __half2float(__float2half_rn(v));
+}
+
+__device__ __forceinline__ void store16(void *out, int64_t at, float v, bool bf16) {
+    if (bf16) static_cast<__nv_bfloat16 *>(out)[at] = __float2bfloat16_rn(v);
+    else static_cast<__half *>(out)[at] = __float2half_rn(v);
+}
+
+__device__ __forceinline__ float load16(const void *in, int64_t at, bool bf16) {
+    return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(in)[at])
+                : __half2float(static_cast<const __half *>(in)[at]);
+}
+
+// 32 columns of one output row, rounded once: 16-byte stores where the row allows them.
+__device__ __forceinline__ void store_columns(const uint32_t (&acc)[32], void *out, int64_t row_at, int64_t stride1,
+                                              int col0, int n, bool vec, bool bf16) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        const int col = col0 + v * 8;
+        if (vec && col + 8 <= n) {
+            uint4 packed;
+            packed.x = pack2(__uint_as_float(acc[v * 8 + 0]), __uint_as_float(acc[v * 8 + 1]), bf16);
+            packed.y = pack2(__uint_as_float(acc[v * 8 + 2]), __uint_as_float(acc[v * 8 + 3]), bf16);
+            packed.z = pack2(__uint_as_float(acc[v * 8 + 4]), __uint_as_float(acc[v * 8 + 5]), bf16);
+            packed.w = pack2(__uint_as_float(acc[v * 8 + 6]), __uint_as_float(acc[v * 8 + 7]), bf16);
+            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out) + row_at + col) = packed;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (col + j < n) store16(out, row_at + (col + j) * stride1, __uint_as_float(acc[v * 8 + j]), bf16);
+        }
+    }
+}
+
+// The bytes of A that a CTA loads for a tile whose rows from `row` on number `valid`, and the loads themselves: one
+// 128-row box, or as many 32-row boxes as hold rows of the tile.  Rows that no box brings keep what the stage held;
+// they only reach accumulator rows that are never stored.
+__device__ __forceinline__ int a_boxes(int valid) {
+    return valid <= 0 ? 0 : min(BM / A_CHUNK_ROWS, (valid + A_CHUNK_ROWS - 1) / A_CHUNK_ROWS);
+}
+
+template <int CG>
+__device__ __forceinline__ void load_2d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y) {
+    if constexpr (CG == 1) tma_load_2d(dst, map, bar, x, y);
+    else tma_load_2d_pair(dst, map, bar, x, y);
+}
+
+template <int CG>
+__device__ __forceinline__ void load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
+    if constexpr (CG == 1) tma_load_3d(dst, map, bar, x, y, z);
+    else tma_load_3d_pair(dst, map, bar, x, y, z);
+}
+
+// B_MN: the matrices have unit stride along their columns; otherwise along their rows (a transposed view).
+template <int CG, int BN, bool B_MN, Mode MODE>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+    grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_chunk,
+                   const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_low,
+                   const __grid_constant__ CUtensorMap map_up, const __grid_constant__ Params p) {
+    using S = Shape<CG, BN>;
+    constexpr int STAGES = S::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Control *ctl = reinterpret_cast<Control *>(smem + STAGES * S::STAGE_BYTES);
+    Run *table = reinterpret_cast<Run *>(reinterpret_cast<uint8_t *>(ctl) + CONTROL_BYTES);
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int lane = threadIdx.x & 31;
+    const WaitCtx wait_ctx{&ctl->abort_flag, p.status, KID_GROUPED};
+    const uint32_t cta_rank = CG == 1 ? 0u : cluster_cta_rank();
+    const bool leader = cta_rank == 0;
+    const int worker = blockIdx.x / CG;
+    const int workers = gridDim.x / CG;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&ctl->full[s], 1);
+            mbar_init(&ctl->empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&ctl->tmem_full[b], 1);
+            mbar_init(&ctl->tmem_empty[b], 128 * CG);
+        }
+        ctl->abort_flag = 0;
+        mbar_fence_init();
+        tma_prefetch_desc(&map_a);
+        tma_prefetch_desc(&map_b);
+    }
+    if (warp == 1) {
+        tmem_alloc<CG>(&ctl->tmem_base, TMEM_COLS);
+        tmem_relinquish<CG>();
+    }
+    build_table(p, table, ctl, S::TILE_M);
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
+    tcgen05_fence_after_sync();
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+    using W = Walk<MODE, S::TILE_M, BN>;
+
+    if (warp == 0) {
+        // ------------------------------ TMA producer ------------------------------
+        if (lane == 0) {
+            uint32_t it = 0;
+            for (W walk(p, table, ctl, worker, workers); walk.more(); walk.advance()) {
+                const Place at = walk.place(p);
+                const int m0 = at.row0 + static_cast<int>(cta_rank) * BM;
+                const int n0 = at.col0 + static_cast<int>(cta_rank) * S::BN_CTA;
+                const int boxes = a_boxes(at.row_end - m0);
+                // the even CTA's barrier counts the bytes of both
+                int bytes = boxes * (A_CHUNK_ROWS * BK * 2) + S::B_STAGE_BYTES;
+                if constexpr (CG == 2) bytes += a_boxes(at.row_end - m0 - BM) * (A_CHUNK_ROWS * BK * 2) + S::B_STAGE_BYTES;
+                for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+                    const int s = it % STAGES;
+                    mbar_wait(&ctl->empty[s], ((it / STAGES) & 1) ^ 1, wait_ctx, 0x100 | s);
+                    uint8_t *a_dst = smem + s * S::STAGE_BYTES;
+                    uint8_t *b_dst = a_dst + A_STAGE_BYTES;
+                    if (leader) mbar_expect_tx(&ctl->full[s], bytes);
+                    if (boxes == BM / A_CHUNK_ROWS) {
+                        load_2d<CG>(a_dst, &map_a, &ctl->full[s], kb * BK, m0);
+                    } else {
+                        for (int c = 0; c < boxes; ++c)
+                            load_2d<CG>(a_dst + c * (A_CHUNK_ROWS * BK * 2), &map_a_chunk, &ctl->full[s], kb * BK,
+                                        m0 + c * A_CHUNK_ROWS);
+                    }
+                    if constexpr (B_MN) {
+#pragma unroll
+                        for (int j = 0; j < S::BN_CTA / 64; ++j)
+                            load_3d<CG>(b_dst + j * (BK * 128), &map_b, &ctl->full[s], n0 + j * 64, kb * BK, at.matrix);
+                    } else {
+                        load_3d<CG>(b_dst, &map_b, &ctl->full[s], kb * BK, n0, at.matrix);
+                    }
+                }
+                if constexpr (MODE == LORA) {
+                    // the adapters' second product: for every run of the tile, the tile's rows of (scales lhs . down)
+                    // against the run's up, 32 ranks a stage
+                    const int tile_end = min(at.row_end, at.row0 + S::TILE_M);
+                    const int b_bytes = p.up_mn ? S::BN_CTA * RANK_BLOCK * 2 : S::B_STAGE_BYTES;
+                    for (int r = first_run_behind(table, walk.runs, at.row0); r < walk.runs && table[r].begin < tile_end; ++r) {
+                        const Run run = table[r];
+                        // 32-row boxes of this CTA's rows that hold rows of the run (first, last), and the partner's
+                        const auto box_range = [&](int base, int &first, int &last) {
+                            first = max(run.begin - base, 0) / A_CHUNK_ROWS;
+                            last = min((min(run.end, tile_end) - base + A_CHUNK_ROWS - 1) / A_CHUNK_ROWS, BM / A_CHUNK_ROWS);
+                            if (min(run.end, tile_end) <= base) last = 0;
+                            if (last < first) last = first;
+                        };
+                        int first, last, first_other = 0, last_other = 0;
+                        box_range(m0, first, last);
+                        if constexpr (CG == 2) box_range(at.row0 + BM, first_other, last_other);
+                        int ext_bytes = (last - first) * (A_CHUNK_ROWS * BK * 2) + b_bytes;
+                        if constexpr (CG == 2) ext_bytes += (last_other - first_other) * (A_CHUNK_ROWS * BK * 2) + b_bytes;
+                        for (int rb = 0; rb < p.rank_blocks; ++rb, ++it) {
+                            const int s = it % STAGES;
+                            mbar_wait(&ctl->empty[s], ((it / STAGES) & 1) ^ 1, wait_ctx, 0x110 | s);
+                            uint8_t *a_dst = smem + s * S::STAGE_BYTES;
+                            uint8_t *b_dst = a_dst + A_STAGE_BYTES;
+                            if (leader) mbar_expect_tx(&ctl->full[s], ext_bytes);
+                            for (int c = first; c < last; ++c)
+                                load_2d<CG>(a_dst + c * (A_CHUNK_ROWS * BK * 2), &map_low, &ctl->full[s], rb * BK,
+                                            m0 + c * A_CHUNK_ROWS);
+                            if (p.up_mn) {
+                                for (int j = 0; j < S::BN_CTA / 64; ++j)
+                                    load_3d<CG>(b_dst + j * (RANK_BLOCK * 128), &map_up, &ctl->full[s], n0 + j * 64,
+                                                rb * RANK_BLOCK, run.matrix);
+                            } else {
+                                load_3d<CG>(b_dst, &map_up, &ctl->full[s], rb * RANK_BLOCK, n0, run.matrix);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------- MMA issuer -------------------------------
+        // The warp runs the loop as one (the instruction takes uniform registers); an elected lane issues.
+        if (leader) {
+            const uint32_t idesc = umma_instr_desc(BM * CG, BN, p.bf16 != 0, false, B_MN);
+            const bool issuer = elect_one();
+            const uint32_t smem_base = smem_u32(smem);
+            uint32_t s = 0, phase = 0, acc_it = 0;
+            bool ready = false;
+            for (W walk(p, table, ctl, worker, workers); walk.more(); walk.advance(), ++acc_it) {
+                const uint32_t buf = acc_it & 1;
+                mbar_wait(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+                tcgen05_fence_after_sync();
+                const uint32_t tmem_acc = tmem_base + buf * BN;
+                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                    if (!ready) mbar_wait(&ctl->full[s], phase, wait_ctx, 0x300 | s);
+                    tcgen05_fence_after_sync();
+                    const uint32_t a_addr = smem_base + s * S::STAGE_BYTES;
+                    const uint32_t b_addr = a_addr + A_STAGE_BYTES;
+                    const uint32_t s_next = s + 1 == STAGES ? 0 : s + 1;
+                    const uint32_t phase_next = s_next == 0 ? phase ^ 1 : phase;
+#pragma unroll
+                    for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                        const uint64_t desc_a = umma_smem_desc(a_addr + kk * (UMMA_K * 2), 16, 1024);
+                        const uint64_t desc_b =
+                            umma_smem_desc(b_addr + kk * (B_MN ? UMMA_K * 128 : UMMA_K * 2), p.b_lbo, 1024);
+                        if (issuer) umma_ss<CG>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
+                        if (kk == BK / UMMA_K / 2 - 1)  // (a probe between MMAs costs nothing, a wait after them does)
+                            ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
+                    }
+                    if (issuer) {
+                        if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
+                        else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
+                    }
+                    s = s_next;
+                    phase = phase_next;
+                }
+                if constexpr (MODE == LORA) {
+                    const Place at = walk.place(p);
+                    const int tile_end = min(at.row_end, at.row0 + S::TILE_M);
+                    const uint32_t idesc_up = umma_instr_desc(BM * CG, BN, p.bf16 != 0, false, p.up_mn != 0);
+                    const uint32_t b_step = p.up_mn ? UMMA_K * 128 : UMMA_K * 2;
+                    const uint32_t b_lbo = p.up_mn ? RANK_BLOCK * 128 : 16;
+                    for (int r = first_run_behind(table, walk.runs, at.row0); r < walk.runs && table[r].begin < tile_end; ++r) {
+                        // Only the accumulator rows of this run take part: what another run's adapter holds, infinities
+                        // and NaN included, cannot reach them.
+                        const int low = table[r].begin - at.row0, high = min(table[r].end, tile_end) - at.row0;
+                        uint32_t off[8];
+#pragma unroll
+                        for (int w = 0; w < 8; ++w) off[w] = ~(low_bits(high - 32 * w) & ~low_bits(low - 32 * w));
+                        for (int rb = 0; rb < p.rank_blocks; ++rb) {
+                            if (!ready) mbar_wait(&ctl->full[s], phase, wait_ctx, 0x310 | s);
+                            ready = false;
+                            tcgen05_fence_after_sync();
+                            const uint32_t a_addr = smem_base + s * S::STAGE_BYTES;
+                            const uint32_t b_addr = a_addr + A_STAGE_BYTES;
+                            const int steps = (min(RANK_BLOCK, p.rank - rb * RANK_BLOCK) + UMMA_K - 1) / UMMA_K;
+                            for (int kk = 0; kk < steps; ++kk) {
+                                const uint64_t desc_b = umma_smem_desc(b_addr + kk * b_step, b_lbo, 1024);
+#pragma unroll
+                                for (int part = 0; part < 2; ++part) {
+                                    const uint64_t desc_a =
+                                        umma_smem_desc(a_addr + part * (RANK_BLOCK * 2) + kk * (UMMA_K * 2), 16, 1024);
+                                    if (issuer) umma_ss_lanes<CG>(tmem_acc, desc_a, desc_b, idesc_up, off);
+                                }
+                            }
+                            if (issuer) {
+                                if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
+                                else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
+                            }
+                            s = s + 1 == STAGES ? 0 : s + 1;
+                            if (s == 0) phase ^= 1;
+                        }
+                    }
+                }
+                if (issuer) {
+                    if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
+                    else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // -------------------------------- epilogue --------------------------------
+        const int quadrant = warp & 3;
+        const int row_in_tile = static_cast<int>(cta_rank) * BM + quadrant * 32 + lane;
+        const bool bf16 = p.bf16 != 0, vec = p.out_vec != 0;
+        uint32_t acc_it = 0;
+        for (W walk(p, table, ctl, worker, workers); walk.more(); walk.advance(), ++acc_it) {
+            const Place at = walk.place(p);
+            const int row = at.row0 + row_in_tile;
+            const uint32_t buf = acc_it & 1;
+            float scale = 1.f;
+            if constexpr (MODE == SHRINK) scale = p.scales[at.matrix * p.scales_stride];
+            mbar_wait(&ctl->tmem_full[buf], (acc_it >> 1) & 1, wait_ctx, 0x400 | buf);
+            tcgen05_fence_after_sync();
+            const uint32_t taddr = tmem_base + buf * BN + (static_cast<uint32_t>(quadrant * 32) << 16);
+            const int64_t row_at = row * p.out_stride0;
+#pragma unroll 1
+            for (int col = 0; col < BN && at.col0 + col < p.n; col += 32) {
+                uint32_t acc[32];
+                __syncwarp();
+                tmem_ld_32x32(taddr + col, acc);
+                tmem_wait_ld();
+                if (row >= at.row_end) {
+                    // (nothing: the row belongs to the next run, or to none)
+                } else if constexpr (MODE == SHRINK) {
+                    // 32 ranks of a row: their high parts, then the low parts (value = high + low to twice the
+                    // type's precision, so that the second product runs on the tensor cores without the rounding
+                    // of one 16-bit operand).  Ranks past the last are zero: the operands' bounds filled them.
+                    uint4 high[4], low[4];
+                    uint32_t *h = reinterpret_cast<uint32_t *>(high), *l = reinterpret_cast<uint32_t *>(low);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float a = scale * __uint_as_float(acc[2 * j]), b = scale * __uint_as_float(acc[2 * j + 1]);
+                        const float ha = round16(a, bf16), hb = round16(b, bf16);
+                        h[j] = pack2(a, b, bf16);
+                        // (an infinite or NaN high part says it all; inf - inf must not turn it into NaN)
+                        l[j] = pack2(isfinite(ha) ? a - ha : 0.f, isfinite(hb) ? b - hb : 0.f, bf16);
+                    }
+                    uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + row_at + 2 * (at.col0 + col));
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        dst[v] = high[v];
+                        dst[4 + v] = low[v];
+                    }
+                } else {
+                    store_columns(acc, p.out, row_at, p.out_stride1, at.col0 + col, p.n, vec, bf16);
+                }
+            }
+            tcgen05_fence_before_sync();
+            if (CG == 1 || leader) mbar_arrive(&ctl->tmem_empty[buf]);
+            else mbar_arrive_cluster(&ctl->tmem_empty[buf], 0);
+        }
+    }
+
+    __syncwarp();
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
+    if (warp == 1) {
+        tcgen05_fence_after_sync();
+        tmem_dealloc<CG>(tmem_base, TMEM_COLS);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Gradient of the matrices: rhs_grad[e] = lhs_e^T . output_grad_e, the reduction runs over the rows of run e.
+// Both operands are read where they lie, rows of the reduction first ("MN-major" tiles of 64 rows).  A run's last
+// 64-row block also brings rows of the next run: whole 16-row steps behind the run are not issued, and the rest of the
+// last step is overwritten with zeros in BOTH operands (a zero in one alone would let a NaN or an infinity of the
+// neighbouring run through).
+// ---------------------------------------------------------------------------
+struct GradParams {
+    Offsets offsets;
+    int rows, m, n;  // rows of the reduction (all runs), lhs columns, output_grad columns
+    int m_tiles, n_tiles;
+    int bf16;
+    void *out;
+    int64_t out_stride0, out_stride1, out_batch_stride;
+    int out_vec;
+    unsigned int *status;
+};
+
+// Run e's rows, by the same rule as build_table: bounds clamped by a running maximum.  starts has runs + 1 entries.
+__device__ __forceinline__ void build_starts(const Offsets &offsets, int rows, int *starts) {
+    for (int i = threadIdx.x; i <= offsets.runs; i += blockDim.x)
+        starts[i] = load_index(offsets.data, offsets.stride, offsets.wide, i, 0, rows);
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    const int lane = threadIdx.x;
+    int bound = 0;
+    for (int base = 0; base <= offsets.runs; base += 32) {
+        int v = base + lane <= offsets.runs ? starts[base + lane] : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int other = __shfl_up_sync(0xffffffffu, v, d);
+            if (lane >= d) v = max(v, other);
+        }
+        v = max(v, bound);
+        if (base + lane <= offsets.runs) starts[base + lane] = v;
+        bound = __shfl_sync(0xffffffffu, v, 31);
+    }
+}
+
+template <int BN>
+size_t grad_smem_bytes(int runs) {
+    return 1024 + Shape<1, BN>::STAGES * Shape<1, BN>::STAGE_BYTES + CONTROL_BYTES + static_cast<size_t>(runs + 1) * 4;
+}
+
+template <int BN>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+    grouped_grad_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                        const __grid_constant__ GradParams p) {
+    using S = Shape<1, BN>;
+    constexpr int STAGES = S::STAGES;
+    constexpr int BOX_BYTES = BK * 128;  // 64 rows of 64 columns
+    constexpr int BOXES = (BM + BN) / 64;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Control *ctl = reinterpret_cast<Control *>(smem + STAGES * S::STAGE_BYTES);
+    int *starts = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(ctl) + CONTROL_BYTES);
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int lane = threadIdx.x & 31;
+    const WaitCtx wait_ctx{&ctl->abort_flag, p.status, KID_GROUPED_GRAD};
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&ctl->full[s], 1);
+            mbar_init(&ctl->empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&ctl->tmem_full[b], 1);
+            mbar_init(&ctl->tmem_empty[b], 128);
+        }
+        ctl->abort_flag = 0;
+        mbar_fence_init();
+        tma_prefetch_desc(&map_a);
+        tma_prefetch_desc(&map_b);
+    }
+    if (warp == 1) {
+        tmem_alloc<1>(&ctl->tmem_base, TMEM_COLS);
+        tmem_relinquish<1>();
+    }
+    build_starts(p.offsets, p.rows, starts);
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    tcgen05_fence_after_sync();
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+    const int per_run = p.m_tiles * p.n_tiles;
+    const int total = p.offsets.runs * per_run;
+
+    if (warp == 0) {
+        // ------------------------------ TMA producer ------------------------------
+        if (lane == 0) {
+            uint32_t it = 0;
+            for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
+                const int run = tile / per_run, inside = tile - run * per_run;
+                const int m0 = inside % p.m_tiles * BM, n0 = inside / p.m_tiles * BN;
+                const int begin = starts[run], blocks = (starts[run + 1] - begin + BK - 1) / BK;
+                for (int kb = 0; kb < blocks; ++kb, ++it) {
+                    const int s = it % STAGES;
+                    mbar_wait(&ctl->empty[s], ((it / STAGES) & 1) ^ 1, wait_ctx, 0x100 | s);
+                    uint8_t *dst = smem + s * S::STAGE_BYTES;
+                    mbar_expect_tx(&ctl->full[s], S::STAGE_BYTES);
+#pragma unroll
+                    for (int j = 0; j < BM / 64; ++j)
+                        tma_load_2d(dst + j * BOX_BYTES, &map_a, &ctl->full[s], m0 + j * 64, begin + kb * BK);
+#pragma unroll
+                    for (int j = 0; j < BN / 64; ++j)
+                        tma_load_2d(dst + A_STAGE_BYTES + j * BOX_BYTES, &map_b, &ctl->full[s], n0 + j * 64, begin + kb * BK);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------- MMA issuer -------------------------------
+        const uint32_t idesc = umma_instr_desc(BM, BN, p.bf16 != 0, true, true);
+        const bool issuer = elect_one();
+        const uint32_t smem_base = smem_u32(smem);
+        uint32_t s = 0, phase = 0, acc_it = 0;
+        bool ready = false;
+        for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
+            const int run = tile / per_run;
+            const int length = starts[run + 1] - starts[run];
+            if (length == 0) continue;  // (the epilogue stores zeros by itself)
+            const int blocks = (length + BK - 1) / BK;
+            const uint32_t buf = acc_it & 1;
+            mbar_wait(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+            tcgen05_fence_after_sync();
+            const uint32_t tmem_acc = tmem_base + buf * BN;
+            for (int kb = 0; kb < blocks; ++kb) {
+                if (!ready) mbar_wait(&ctl->full[s], phase, wait_ctx, 0x300 | s);
+                tcgen05_fence_after_sync();
+                const uint32_t a_addr = smem_base + s * S::STAGE_BYTES;
+                const uint32_t b_addr = a_addr + A_STAGE_BYTES;
+                const uint32_t s_next = s + 1 == STAGES ? 0 : s + 1;
+                const uint32_t phase_next = s_next == 0 ? phase ^ 1 : phase;
+                const int left = length - kb * BK;
+                const int steps = left >= BK ? BK / UMMA_K : (left + UMMA_K - 1) / UMMA_K;
+                if (left < BK && left % UMMA_K != 0) {
+                    const int first = left, chunks = (steps * UMMA_K - first) * 8;  // 16-byte chunks of a box
+                    uint8_t *stage = smem + s * S::STAGE_BYTES + first * 128;
+                    for (int i = lane; i < chunks; i += 32)
+#pragma unroll
+                        for (int b = 0; b < BOXES; ++b)
+                            *reinterpret_cast<uint4 *>(stage + b * BOX_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                    const uint64_t desc_a = umma_smem_desc(a_addr + kk * (UMMA_K * 128), BOX_BYTES, 1024);
+                    const uint64_t desc_b = umma_smem_desc(b_addr + kk * (UMMA_K * 128), BOX_BYTES, 1024);
+                    if (issuer && kk < steps) umma_ss<1>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
+                    if (kk == BK / UMMA_K / 2 - 1)
+                        ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
+                }
+                if (issuer) umma_commit<1>(&ctl->empty[s]);
+                s = s_next;
+                phase = phase_next;
+            }
+            if (issuer) umma_commit<1>(&ctl->tmem_full[buf]);
+            __syncwarp();
+            ++acc_it;
+        }
+    } else {
+        // -------------------------------- epilogue --------------------------------
+        const int quadrant = warp & 3;
+        const bool bf16 = p.bf16 != 0, vec = p.out_vec != 0;
+        uint32_t acc_it = 0;
+        for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
+            const int run = tile / per_run, inside = tile - run * per_run;
+            const int row = inside % p.m_tiles * BM + quadrant * 32 + lane, n0 = inside / p.m_tiles * BN;
+            const bool empty = starts[run + 1] == starts[run];
+            const int64_t row_at = run * p.out_batch_stride + row * p.out_stride0;
+            const uint32_t buf = acc_it & 1;
+            const uint32_t taddr = tmem_base + buf * BN + (static_cast<uint32_t>(quadrant * 32) << 16);
+            if (!empty) {
+                mbar_wait(&ctl->tmem_full[buf], (acc_it >> 1) & 1, wait_ctx, 0x400 | buf);
+                tcgen05_fence_after_sync();
+            }
+#pragma unroll 1
+            for (int col = 0; col < BN && n0 + col < p.n; col += 32) {
+                uint32_t acc[32] = {};
+                __syncwarp();
+                if (!empty) {
+                    tmem_ld_32x32(taddr + col, acc);
+                    tmem_wait_ld();
+                }
+                if (row < p.m) store_columns(acc, p.out, row_at, p.out_stride1, n0 + col, p.n, vec, bf16);
+            }
+            if (!empty) {
+                tcgen05_fence_before_sync();
+                mbar_arrive(&ctl->tmem_empty[buf]);
+                ++acc_it;
+            }
+        }
+    }
+
+    __syncwarp();
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tcgen05_fence_after_sync();
+        tmem_dealloc<1>(tmem_base, TMEM_COLS);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Plain kernels for operands that no tensor map can address: one thread per output element, fp32 sums, one rounding.
+// ---------------------------------------------------------------------------
+struct View {  // up to three dimensions; stride[0] is the matrix index's
+    const void *data;
+    int64_t stride[3];
+};
+
+// The run that holds `row` by the rule of build_table, or -1.
+__device__ int run_of(const Offsets &o, int rows, int row) {
+    int bound = load_index(o.data, o.stride, o.wide, 0, 0, rows);
+    if (row < bound) return -1;
+    for (int e = 0; e < o.runs; ++e) {
+        bound = max(bound, load_index(o.data, o.stride, o.wide, e + 1, 0, rows));
+        if (row < bound) return e;
+    }
+    return -1;
+}
+
+constexpr int PLAIN_ROWS = 8;
+
+// low (may be nullptr, as may adapters): fp32 [rows, rank], added as low . up of the run's adapter.
+__global__ void __launch_bounds__(256)
+    grouped_plain_kernel(const Offsets offsets, const void *adapters, int64_t adapters_stride, int adapters_wide,
+                         int matrices, int shared_matrix, View a, View b, const float *low, int rank, View up, int rows,
+                         int n, int k, const float *scales, int64_t scales_stride, float *low_out, void *out,
+                         int64_t os0, int64_t os1, int bf16) {
+    __shared__ int runs[PLAIN_ROWS];
+    const int64_t block_row = static_cast<int64_t>(blockIdx.x) * PLAIN_ROWS;
+    if (threadIdx.x < PLAIN_ROWS)
+        runs[threadIdx.x] = block_row + threadIdx.x < rows ? run_of(offsets, rows, static_cast<int>(block_row + threadIdx.x)) : -1;
+    __syncthreads();
+    const int64_t row = block_row + threadIdx.x / 32;
+    const int run = runs[threadIdx.x / 32];
+    if (run < 0) return;
+    int matrix = run;
+    if (adapters != nullptr) {
+        matrix = load_index(adapters, adapters_stride, adapters_wide, run, -1, matrices);
+        if (matrix >= matrices) matrix = -1;
+    }
+    const bool has_matrix = matrix >= 0;
+    if (!shared_matrix && !has_matrix) return;
+    const int64_t b_at = shared_matrix ? 0 : matrix * b.stride[0];
+    for (int64_t col = static_cast<int64_t>(blockIdx.y) * 32 + (threadIdx.x & 31); col < n; col += static_cast<int64_t>(gridDim.y) * 32) {
+        float acc = 0.f;
+        for (int i = 0; i < k; ++i)
+            acc = fmaf(load16(a.data, row * a.stride[1] + i * a.stride[2], bf16),
+                       load16(b.data, b_at + i * b.stride[1] + col * b.stride[2], bf16), acc);
+        if (low_out != nullptr) {
+            low_out[row * n + col] = acc * scales[matrix * scales_stride];
+            continue;
+        }
+        if (low != nullptr && has_matrix)
+            for (int i = 0; i < rank; ++i)
+                acc = fmaf(low[row * rank + i], load16(up.data, matrix * up.stride[0] + i * up.stride[1] + col * up.stride[2], bf16), acc);
+        store16(out, row * os0 + col * os1, acc, bf16);
+    }
+}
+
+__global__ void __launch_bounds__(256)
+    grouped_grad_plain_kernel(const Offsets offsets, View a, View b, int rows, int m, int n, void *out, int64_t ob,
+                              int64_t os0, int64_t os1, int bf16) {
+    __shared__ int bounds[2];
+    const int run = blockIdx.z;
+    if (threadIdx.x == 0) {
+        int begin = 0, end = 0;
+        for (int e = 0; e <= run + 1; ++e) {
+            begin = end;
+            end = max(end, load_index(offsets.data, offsets.stride, offsets.wide, e, 0, rows));
+        }
+        bounds[0] = begin;
+        bounds[1] = end;
+    }
+    __syncthreads();
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * PLAIN_ROWS + threadIdx.x / 32; row < m; row += static_cast<int64_t>(gridDim.x) * PLAIN_ROWS)
+        for (int64_t col = static_cast<int64_t>(blockIdx.y) * 32 + (threadIdx.x & 31); col < n; col += static_cast<int64_t>(gridDim.y) * 32) {
+            float acc = 0.f;
+            for (int64_t t = bounds[0]; t < bounds[1]; ++t)
+                acc = fmaf(load16(a.data, t * a.stride[1] + row * a.stride[2], bf16),
+                           load16(b.data, t * b.stride[1] + col * b.stride[2], bf16), acc);
+            store16(out, run * ob + row * os0 + col * os1, acc, bf16);
+        }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+// Rows with unit stride and 16-byte aligned starts.  A dimension of one element has no stride of its own.
+bool rows_addressable(const void *data, int64_t rows, int64_t cols, int64_t stride0, int64_t stride1) {
+    return aligned16(data) && cols > 0 && (stride1 == 1 || cols == 1) &&
+           (rows <= 1 || (stride0 % 8 == 0 && stride0 >= cols && stride0 < (1LL << 38)));
+}
+
+int64_t row_pitch(int64_t rows, int64_t cols, int64_t stride0) { return rows <= 1 ? (cols + 7) / 8 * 8 : stride0; }
+
+// Matrices [count, rows, cols]: which of the last two dimensions is the unit-stride one, and whether a three-dimensional
+// tensor map can address them.
+struct Matrices {
+    const void *data;
+    int64_t count, rows, cols, stride0, stride1, stride2;
+    bool mn() const { return rows_addressable(data, rows, cols, stride1, stride2); }
+    bool k_major() const { return rows_addressable(data, cols, rows, stride2, stride1); }
+    bool batch_ok(bool as_mn) const {  // one matrix behind the other
+        const int64_t span = as_mn ? row_pitch(rows, cols, stride1) * (rows - 1) + cols
+                                   : row_pitch(cols, rows, stride2) * (cols - 1) + rows;
+        return count <= 1 || (stride0 % 8 == 0 && stride0 >= span && stride0 < (1LL << 38));
+    }
+    bool addressable() const { return (mn() && batch_ok(true)) || (k_major() && batch_ok(false)); }
+    bool use_mn() const { return mn() && batch_ok(true); }
+};
+
+int map_rows(const DeviceState &dev, CUtensorMap *map, int dtype, const void *data, int64_t rows, int64_t cols,
+             int64_t stride0, uint32_t box_cols, uint32_t box_rows) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(row_pitch(rows, cols, stride0)) * 2};
+    const uint32_t box[2] = {box_cols, box_rows};
+    return make_tensor_map(dev, map, dtype, 2, data, dims, strides, box, true);
+}
+
+// box_inner x box_outer boxes over one matrix at a time
+int map_matrices(const DeviceState &dev, CUtensorMap *map, int dtype, const Matrices &t, bool mn, uint32_t box_inner,
+                 uint32_t box_outer) {
+    const int64_t inner = mn ? t.cols : t.rows, outer = mn ? t.rows : t.cols;
+    const int64_t pitch = row_pitch(outer, inner, mn ? t.stride1 : t.stride2);
+    const int64_t batch = t.count <= 1 ? pitch * outer : t.stride0;
+    const uint64_t dims[3] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(outer), static_cast<uint64_t>(t.count)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(pitch) * 2, static_cast<uint64_t>(batch) * 2};
+    const uint32_t box[3] = {box_inner, box_outer, 1};
+    return make_tensor_map(dev, map, dtype, 3, t.data, dims, strides, box, true);
+}
+
+template <typename Kernel>
+int active_pairs(Kernel kernel, const DeviceState &dev, size_t smem) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(dev.sm_count / 2 * 2));
+    config.blockDim = dim3(NUM_THREADS);
+    config.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {2, 1, 1};
+    config.attrs = attr;
+    config.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess || clusters <= 0) {
+        cudaGetLastError();
+        return 0;
+    }
+    return clusters;
+}
+
+struct Maps {
+    CUtensorMap a, a_chunk, b, low, up;
+};
+
+constexpr size_t MAX_SMEM = 227 * 1024;
+
+template <int CG, int BN, bool B_MN, Mode MODE>
+int launch(cudaStream_t stream, const DeviceState &dev, const Maps &maps, const Params &p, int64_t most_tiles) {
+    auto kernel = grouped_kernel<CG, BN, B_MN, MODE>;
+    static_assert(1024 + Shape<CG, BN>::STAGES * Shape<CG, BN>::STAGE_BYTES + CONTROL_BYTES + table_bytes(MAX_RUNS) <= MAX_SMEM,
+                  "shared memory per CTA");
+    const size_t smem = smem_bytes<CG, BN>(p.offsets.runs);
+    static thread_local int configured_device = -1;
+    static thread_local int pairs = 0;
+    if (configured_device != dev.device) {
+        NT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SMEM)));
+        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, MAX_SMEM);
+        configured_device = dev.device;
+    }
+    const int workers = CG == 2 ? pairs : dev.sm_count;
+    if (workers <= 0) return fail(NINETOOTHED_B200_ERR_DEVICE, "grouped matmul: no CTA pair fits this device");
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(most_tiles, workers) * CG));
+    config.blockDim = dim3(NUM_THREADS);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    if (CG == 2) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim = {2, 1, 1};
+        config.attrs = attr;
+        config.numAttrs = 1;
+    }
+    NT_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, maps.a, maps.a_chunk, maps.b, maps.low, maps.up, p));
+    return 0;
+}
+
+// Tensor maps of the row operand and the matrices, then the launch.
+template <int CG, int BN, Mode MODE>
+int launch_shape(cudaStream_t stream, const DeviceState &dev, int dtype, Maps &maps, Params &p, const void *lhs,
+                 int64_t lhs_stride0, const Matrices &rhs, const Matrices *up) {
+    using S = Shape<CG, BN>;
+    p.n_tiles = static_cast<int>((static_cast<int64_t>(p.n) + BN - 1) / BN);
+    p.group_m = GROUP_ROWS / CG;
+    const bool mn = rhs.use_mn();
+    p.b_lbo = mn ? BK * 128 : 16;
+    if (int rc = map_rows(dev, &maps.a, dtype, lhs, p.rows, p.k, lhs_stride0, BK, BM)) return rc;
+    if (int rc = map_rows(dev, &maps.a_chunk, dtype, lhs, p.rows, p.k, lhs_stride0, BK, A_CHUNK_ROWS)) return rc;
+    if (int rc = map_matrices(dev, &maps.b, dtype, rhs, mn, 64, mn ? BK : S::BN_CTA)) return rc;
+    if (up != nullptr) {
+        p.up_mn = up->use_mn();
+        if (int rc = map_matrices(dev, &maps.up, dtype, *up, p.up_mn, 64, p.up_mn ? RANK_BLOCK : S::BN_CTA)) return rc;
+    } else {
+        maps.up = maps.a;
+    }
+    if (MODE != LORA || up == nullptr) maps.low = maps.a;
+    const int64_t m_tiles = (static_cast<int64_t>(p.rows) + S::TILE_M - 1) / S::TILE_M +
+                            (MODE == LORA ? 0 : std::min(p.offsets.runs, p.rows));
+    if (m_tiles * p.n_tiles > INT_MAX / 2) return fail(NINETOOTHED_B200_ERR_SHAPE, "grouped matmul: too many tiles");
+    return mn ? launch<CG, BN, true, MODE>(stream, dev, maps, p, m_tiles * p.n_tiles)
+              : launch<CG, BN, false, MODE>(stream, dev, maps, p, m_tiles * p.n_tiles);
+}
+
+// Tiles of 256 x 256 on CTA pairs where there are rows for them; narrower ones on single CTAs otherwise.
+template <Mode MODE>
+int launch_product(cudaStream_t stream, const DeviceState &dev, int dtype, Maps &maps, Params &p, const void *lhs,
+                   int64_t lhs_stride0, const Matrices &rhs, const Matrices *up, int64_t live_runs) {
+    const int64_t run_rows = p.rows / std::max<int64_t>(1, live_runs);
+    if (run_rows >= 192) return launch_shape<2, 256, MODE>(stream, dev, dtype, maps, p, lhs, lhs_stride0, rhs, up);
+    const int64_t tiles_128 = live_runs * ((run_rows + BM - 1) / BM) * ((p.n + 127) / 128);
+    if (tiles_128 >= 2 * dev.sm_count)
+        return launch_shape<1, 128, MODE>(stream, dev, dtype, maps, p, lhs, lhs_stride0, rhs, up);
+    return launch_shape<1, 64, MODE>(stream, dev, dtype, maps, p, lhs, lhs_stride0, rhs, up);
+}
+
+bool has_arrays(const NineToothedTensor &t) { return t.shape != nullptr && t.strides != nullptr; }
+
+constexpr int64_t MAX_DIM = INT_MAX - 4096;  // coordinates of a tile that overhangs stay 32-bit
+
+int check_offsets(const char *what, const NineToothedTensor &offsets, int64_t runs, int offsets_dtype, Offsets *out) {
+    if (offsets_dtype != NINETOOTHED_INT32 && offsets_dtype != NINETOOTHED_INT64)
+        return fail(NINETOOTHED_B200_ERR_DTYPE, "%s: offsets must be int32 or int64, got dtype %d", what, offsets_dtype);
+    if (static_cast<int64_t>(offsets.shape[0]) != runs + 1)
+        return fail(NINETOOTHED_B200_ERR_SHAPE, "%s: offsets must hold %lld bounds (runs + 1), got %llu", what,
+                    (long long)(runs + 1), (unsigned long long)offsets.shape[0]);
+    if (runs > MAX_RUNS)
+        return fail(NINETOOTHED_B200_ERR_SHAPE, "%s: %lld runs of rows, at most %d are supported", what, (long long)runs, MAX_RUNS);
+    if (!offsets.data) return fail(NINETOOTHED_B200_ERR_ARGUMENT, "%s: null offsets", what);
+    *out = Offsets{offsets.data, offsets.strides[0], offsets_dtype == NINETOOTHED_INT64 ? 1 : 0, static_cast<int>(runs)};
+    return 0;
+}
+
+dim3 plain_grid(int64_t rows, int64_t cols, int64_t runs = 1) {
+    return dim3(static_cast<unsigned>((rows + PLAIN_ROWS - 1) / PLAIN_ROWS),
+                static_cast<unsigned>(std::min<int64_t>((cols + 31) / 32, 65535)), static_cast<unsigned>(runs));
+}
+
+bool output_vec(const NineToothedTensor &t, int row_dim) {
+    return t.strides[row_dim + 1] == 1 && (t.shape[row_dim] <= 1 || t.strides[row_dim] % 8 == 0) && aligned16(t.data) &&
+           (row_dim == 0 || t.shape[0] <= 1 || t.strides[0] % 8 == 0);
+}
+
+int run_grouped(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothedTensor &rhs,
+                const NineToothedTensor &offsets, const NineToothedTensor &output, int dtype, int offsets_dtype) {
+    const char *what = "grouped_matmul";
+    clear_error();
+    for (auto *t : {&lhs, &rhs, &offsets, &output})
+        if (!has_arrays(*t)) return fail(NINETOOTHED_B200_ERR_ARGUMENT, "%s: null shape/strides", what);
+    if (!is_16bit_float(dtype)) return fail(NINETOOTHED_B200_ERR_DTYPE, "%s: dtype %d is not fp16/bf16", what, dtype);
+    const int64_t rows = lhs.shape[0], k = lhs.shape[1], runs = rhs.shape[0], n = rhs.shape[2];
+    if (static_cast<int64_t>(rhs.shape[1]) != k || static_cast<int64_t>(output.shape[0]) != rows ||
+        static_cast<int64_t>(output.shape[1]) != n)
+        return fail(NINETOOTHED_B200_ERR_SHAPE, "%s: shapes do not agree (lhs [%lld, %lld], rhs [%lld, %llu, %lld], output "
+                    "[%llu, %llu])", what, (long long)rows, (long long)k, (long long)runs, (unsigned long long)rhs.shape[1],
+                    (long long)n, (unsigned long long)output.shape[0], (unsigned long long)output.shape[1]);
+    Params p = {};
+    if (int rc = check_offsets(what, offsets, runs, offsets_dtype, &p.offsets)) return rc;
+    if (rows > MAX_DIM || n > MAX_DIM || k > MAX_DIM) return fail(NINETOOTHED_B200_ERR_SHAPE, "%s: a dimension exceeds 32-bit indexing", what);
+    if (rows == 0 || n == 0 || runs == 0) return 0;
+    if (!output.data || (k > 0 && (!lhs.data || !rhs.data))) return fail(NINETOOTHED_B200_ERR_ARGUMENT, "%s: null data pointer", what);
+    const DeviceState *dev = nullptr;
+    if (int rc = current_device_state(&dev)) return rc;
+    p.matrices = static_cast<int>(runs);
+    p.rows = static_cast<int>(rows);
+    p.n = static_cast<int>(n);
+    p.k = static_cast<int>(k);
+    p.k_blocks = static_cast<int>((k + BK - 1) / BK);
+    p.bf16 = dtype == NINETOOTHED_BFLOAT16;
+    p.out = output.data;
+    p.out_stride0 = output.strides[0];
+    p.out_stride1 = output.strides[1];
+    p.out_vec = output_vec(output, 0);
+    p.status = dev->status;
+    const Matrices matrices{rhs.data, runs, k, n, rhs.strides[0], rhs.strides[1], rhs.strides[2]};
+    if (rows_addressable(lhs.data, rows, k, lhs.strides[0], lhs.strides[1]) && matrices.addressable()) {
+        Maps maps;
+        return launch_product<PRODUCT>(stream, *dev, dtype, maps, p, lhs.data, lhs.strides[0], matrices, nullptr, std::min(runs, rows));
+    }
+    note_plain_launch("grouped_matmul %lld x %lld x %lld runs on the plain CUDA-core kernel: the tensor-core path needs a "
+                      "unit-stride K in lhs, a unit-stride dimension in every matrix of rhs, the other strides multiples "
+                      "of 8 elements and 16-byte aligned bases", (long long)rows, (long long)n, (long long)k);
+    grouped_plain_kernel<<<plain_grid(rows, n), 256, 0, stream>>>(
+        p.offsets, nullptr, 0, 0, p.matrices, 0, View{lhs.data, {0, lhs.strides[0], lhs.strides[1]}},
+        View{rhs.data, {rhs.strides[0], rhs.strides[1], rhs.strides[2]}}, nullptr, 0, View{}, p.rows, p.n, p.k, nullptr, 0,
+        nullptr, output.data, output.strides[0], output.strides[1], p.bf16);
+    NT_CUDA_CHECK(cudaGetLastError());
+    return 0;
+}
+
+template <int BN>
+int launch_grad(cudaStream_t stream, const DeviceState &dev, const CUtensorMap &map_a, const CUtensorMap &map_b, GradParams &p) {
+    auto kernel = grouped_grad_kernel<BN>;
+    const size_t smem = grad_smem_bytes<BN>(p.offsets.runs);
+    static thread_local int configured_device = -1;
+    if (configured_device != dev.device) {
+        NT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SMEM)));
+        configured_device = dev.device;
+    }
+    p.m_tiles = (p.m + BM - 1) / BM;
+    p.n_tiles = (p.n + BN - 1) / BN;
+    const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.offsets.runs;
+    if (tiles > INT_MAX / 2) return fail(NINETOOTHED_B200_ERR_SHAPE, "grouped_matmul_rhs_grad: too many tiles");
+    kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles, dev.sm_count)), NUM_THREADS, smem, stream>>>(map_a, map_b, p);
+    NT_CUDA_CHECK(cudaGetLastError());
+    return 0;
+}
+
+int run_grouped_grad(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothedTensor &grad,
+                     const NineToothedTensor &offsets, const NineToothedTensor &rhs_grad, int dtype, int offsets_dtype) {
+    const char *what = "grouped_matmul_rhs_grad";
+    clear_error();
+    for (auto *t : {&lhs, &grad, &offsets, &rhs_grad})
+        if (!has_arrays(*t)) return fail(NINETOOTHED_B200_ERR_ARGUMENT, "%s: null shape/strides", what);
+    if (!is_16bit_float(dtype)) return fail(NINETOOTHED_B200_ERR_DTYPE, "%s: dtype %d is not fp16/bf16", what, dtype);
+    const int64_t rows = lhs.shape[0], m = lhs.shape[1], n = grad.shape[1], runs = rhs_grad.shape[0];
+    if (static_cast<int64_t>(grad.shape[0]) != rows || static_cast<int64_t>(rhs_grad.shape[1]) != m ||
+        static_cast<int64_t>(rhs_grad.shape[2]) != n)
+        return fail(NINETOOTHED_B200_ERR_SHAPE, "%s: shapes do not agree (lhs [%lld, %lld], output_grad [%llu, %lld], rhs_grad "
+                    "[%lld, %llu, %llu])", what, (long long)rows, (long long)m, (unsigned long long)grad.shape[0], (long long)n,
+                    (long long)runs, (unsigned long long)rhs_grad.shape[1], (unsigned long long)rhs_grad.shape[2]);
+    GradParams p = {};
+    if (int rc = check_offsets(what, offsets, runs, offsets_dtype, &p.offsets)) return rc;
+    if (rows > MAX_DIM || n > MAX_DIM || m > MAX_DIM) return fail(NINETOOTHED_B200_ERR_SHAPE, "%s: a dimension exceeds 32-bit indexing", what);
+    if (m == 0 || n == 0 || runs == 0) return 0;
+    if (!rhs_grad.data || (rows > 0 && (!lhs.data || !grad.data))) return fail(NINETOOTHED_B200_ERR_ARGUMENT, "%s: null data pointer", what);
+    const DeviceState *dev = nullptr;
+    if (int rc = current_device_state(&dev)) return rc;
+    p.rows = static_cast<int>(rows);
+    p.m = static_cast<int>(m);
+    p.n = static_cast<int>(n);
+    p.bf16 = dtype == NINETOOTHED_BFLOAT16;
+    p.out = rhs_grad.data;
+    p.out_batch_stride = rhs_grad.strides[0];
+    p.out_stride0 = rhs_grad.strides[1];
+    p.out_stride1 = rhs_grad.strides[2];
+    p.out_vec = output_vec(rhs_grad, 1);
+    p.status = dev->status;
+    if (rows > 0 && rows_addressable(lhs.data, rows, m, lhs.strides[0], lhs.strides[1]) &&
+        rows_addressable(grad.data, rows, n, grad.strides[0], grad.strides[1])) {
+        CUtensorMap map_a, map_b;
+        if (int rc = map_rows(*dev, &map_a, dtype, lhs.data, rows, m, lhs.strides[0], 64, BK)) return rc;
+        if (int rc = map_rows(*dev, &map_b, dtype, grad.data, rows, n, grad.strides[0], 64, BK)) return rc;
+        return n > 128 ? launch_grad<256>(stream, *dev, map_a, map_b, p) : launch_grad<128>(stream, *dev, map_a, map_b, p);
+    }
+    if (rows > 0)
+        note_plain_launch("grouped_matmul_rhs_grad %lld x %lld x %lld runs on the plain CUDA-core kernel: the tensor-core path "
+                          "needs unit-stride columns, row strides that are multiples of 8 elements and 16-byte aligned bases",
+                          (long long)rows, (long long)m, (long long)n);
+    dim3 grid = plain_grid(m, n, runs);
+    grouped_grad_plain_kernel<<<grid, 256, 0, stream>>>(p.offsets, View{lhs.data, {0, lhs.strides[0], lhs.strides[1]}},
+                                                        View{grad.data, {0, grad.strides[0], grad.strides[1]}}, p.rows, p.m,
+                                                        p.n, rhs_grad.data, rhs_grad.strides[0], rhs_grad.strides[1],
+                                                        rhs_grad.strides[2], p.bf16);
+    NT_CUDA_CHECK(cudaGetLastError());
+    return 0;
+}
+
+// scales (lhs . down) of every row: per 32 ranks, 32 high and 32 low 16-bit parts (or, on the plain path, fp32).
+int64_t rank_blocks(int64_t rank) { return (rank + RANK_BLOCK - 1) / RANK_BLOCK; }
+
+int run_lora(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothedTensor &rhs, const NineToothedTensor &down,
+             const NineToothedTensor &up, const NineToothedTensor &scales, const NineToothedTensor &offsets,
+             const NineToothedTensor &adapters, const NineToothedTensor &output, int dtype, int offsets_dtype,
+             int adapters_dtype, void *workspace, size_t workspace_size) {
+    const char *what = "lora_matmul";
+    clear_error();
+    for (auto *t : {&lhs, &rhs, &down, &up, &scales, &offsets, &adapters, &output})
+        if (!has_arrays(*t)) return fail(NINETOOTHED_B200_ERR_ARGUMENT, "%s: null shape/strides", what);
+    if (!is_16bit_float(dtype)) return fail(NINETOOTHED_B200_ERR_DTYPE, "%s: dtype %d is not fp16/bf16", what, dtype);
+    const int64_t rows = lhs.shape[0], k = lhs.shape[1], n = rhs.shape[1], count = down.shape[0], rank = down.shape[2],
+                  runs = adapters.shape[0];
+    if (static_cast<int64_t>(rhs.shape[0]) != k || static_cast<int64_t>(down.shape[1]) != k ||
+        static_cast<int64_t>(up.shape[0]) != count || static_cast<int64_t>(up.shape[1]) != rank ||
+        static_cast<int64_t>(up.shape[2]) != n || static_cast<int64_t>(scales.shape[0]) != count ||
+        static_cast<int64_t>(output.shape[0]) != rows || static_cast<int64_t>(output.shape[1]) != n)
+        return fail(NINETOOTHED_B200_ERR_SHAPE, "%s: shapes do not agree (lhs [%lld, %lld], rhs [%llu, %lld], down [%lld, %llu, "
+                    "%lld], up [%llu, %llu, %llu], scales [%llu], output [%llu, %llu])", what, (long long)rows, (long long)k,
+                    (unsigned long long)rhs.shape[0], (long long)n, (long long)count, (unsigned long long)down.shape[1],
+                    (long long)rank, (unsigned long long)up.shape[0], (unsigned long long)up.shape[1],
+                    (unsigned long long)up.shape[2], (unsigned long long)scales.shape[0],
+                    (unsigned long long)output.shape[0], (unsigned long long)output.shape[1]);
+    if (adapters_dtype != NINETOOTHED_INT32 && adapters_dtype != NINETOOTHED_INT64)
+        return fail(NINETOOTHED_B200_ERR_DTYPE, "%s: adapters must be int32 or int64, got dtype %d", what, adapters_dtype);
+    Params p = {};
+    if (int rc = check_offsets(what, offsets, runs, offsets_dtype, &p.offsets)) return rc;
+    if (rows > MAX_DIM || n > MAX_DIM || k > MAX_DIM || rank > MAX_DIM / 2 || count > MAX_DIM)
+        return fail(NINETOOTHED_B200_ERR_SHAPE, "%s: a dimension exceeds 32-bit indexing", what);
+    if (rows == 0 || n == 0 || runs == 0) return 0;
+    const bool any = count > 0 && rank > 0;  // there are adapters at all
+    if (!output.data || !adapters.data || (k > 0 && (!lhs.data || !rhs.data)) ||
+        (any && (!down.data || !up.data || !scales.data)))
+        return fail(NINETOOTHED_B200_ERR_ARGUMENT, "%s: null data pointer", what);
+    const size_t needed = static_cast<size_t>(rows) * rank_blocks(rank) * RANK_BLOCK * 4;
+    if (any && (workspace == nullptr || workspace_size < needed || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
+        return fail(NINETOOTHED_B200_ERR_ARGUMENT, "%s: needs a 256-byte aligned workspace of %zu bytes, got %zu at %p", what,
+                    needed, workspace_size, workspace);
+    const DeviceState *dev = nullptr;
+    if (int rc = current_device_state(&dev)) return rc;
+    p.adapters = adapters.data;
+    p.adapters_stride = adapters.strides[0];
+    p.adapters_wide = adapters_dtype == NINETOOTHED_INT64;
+    p.matrices = any ? static_cast<int>(count) : 0;
+    p.rows = static_cast<int>(rows);
+    p.k = static_cast<int>(k);
+    p.k_blocks = static_cast<int>((k + BK - 1) / BK);
+    p.bf16 = dtype == NINETOOTHED_BFLOAT16;
+    p.scales = static_cast<const float *>(scales.data);
+    p.scales_stride = scales.strides[0];
+    p.rank = static_cast<int>(rank);
+    p.rank_blocks = static_cast<int>(rank_blocks(rank));
+    p.status = dev->status;
+    const Matrices shared{rhs.data, 1, k, n, 0, rhs.strides[0], rhs.strides[1]};
+    const Matrices first{down.data, count, k, rank, down.strides[0], down.strides[1], down.strides[2]};
+    const Matrices second{up.data, count, rank, n, up.strides[0], up.strides[1], up.strides[2]};
+    if (rows_addressable(lhs.data, rows, k, lhs.strides[0], lhs.strides[1]) && shared.addressable() &&
+        (!any || (first.addressable() && second.addressable()))) {
+        Maps maps;
+        if (any) {
+            Params shrink = p;
+            shrink.n = p.rank;
+            shrink.out = workspace;
+            shrink.out_stride0 = rank_blocks(rank) * RANK_BLOCK * 2;
+            shrink.out_stride1 = 1;
+            if (int rc = launch_shape<1, 64, SHRINK>(stream, *dev, dtype, maps, shrink, lhs.data, lhs.strides[0], first, nullptr))
+                return rc;
+            if (int rc = map_rows(*dev, &maps.low, dtype, workspace, rows, shrink.out_stride0, shrink.out_stride0, BK, A_CHUNK_ROWS))
+                return rc;
+        }
+        p.n = static_cast<int>(n);
+        p.out = output.data;
+        p.out_stride0 = output.strides[0];
+        p.out_stride1 = output.strides[1];
+        p.out_vec = output_vec(output, 0);
+        return launch_product<LORA>(stream, *dev, dtype, maps, p, lhs.data, lhs.strides[0], shared, any ? &second : nullptr, 1);
+    }
+    note_plain_launch("lora_matmul %lld x %lld x %lld, rank %lld, runs on the plain CUDA-core kernels: the tensor-core path needs "
+                      "a unit-stride K in lhs, a unit-stride dimension in rhs, down and up, the other strides multiples of 8 "
+                      "elements and 16-byte aligned bases", (long long)rows, (long long)n, (long long)k, (long long)rank);
+    const View a{lhs.data, {0, lhs.strides[0], lhs.strides[1]}};
+    const View up_view{up.data, {up.strides[0], up.strides[1], up.strides[2]}};
+    float *low = static_cast<float *>(workspace);
+    if (any) {
+        grouped_plain_kernel<<<plain_grid(rows, rank), 256, 0, stream>>>(
+            p.offsets, p.adapters, p.adapters_stride, p.adapters_wide, p.matrices, 0, a,
+            View{down.data, {down.strides[0], down.strides[1], down.strides[2]}}, nullptr, 0, View{}, p.rows, p.rank, p.k,
+            p.scales, p.scales_stride, low, nullptr, 0, 0, p.bf16);
+        NT_CUDA_CHECK(cudaGetLastError());
+    }
+    grouped_plain_kernel<<<plain_grid(rows, n), 256, 0, stream>>>(
+        p.offsets, p.adapters, p.adapters_stride, p.adapters_wide, p.matrices, 1, a, View{rhs.data, {0, rhs.strides[0], rhs.strides[1]}},
+        any ? low : nullptr, p.rank, up_view, p.rows, static_cast<int>(n), p.k, nullptr, 0, nullptr, output.data,
+        output.strides[0], output.strides[1], p.bf16);
+    NT_CUDA_CHECK(cudaGetLastError());
+    return 0;
+}
+
+}  // namespace
+}  // namespace nt
+
+extern "C" {
+
+NineToothedResult launch_grouped_matmul(NineToothedStream stream, NineToothedTensor lhs, NineToothedTensor rhs,
+                                        NineToothedTensor offsets, NineToothedTensor output, int dtype, int offsets_dtype) {
+    return nt::run_grouped(static_cast<cudaStream_t>(stream), lhs, rhs, offsets, output, dtype, offsets_dtype);
+}
+
+NineToothedResult launch_grouped_matmul_rhs_grad(NineToothedStream stream, NineToothedTensor lhs, NineToothedTensor output_grad,
+                                                 NineToothedTensor offsets, NineToothedTensor rhs_grad, int dtype,
+                                                 int offsets_dtype) {
+    return nt::run_grouped_grad(static_cast<cudaStream_t>(stream), lhs, output_grad, offsets, rhs_grad, dtype, offsets_dtype);
+}
+
+NineToothedResult launch_lora_matmul(NineToothedStream stream, NineToothedTensor lhs, NineToothedTensor rhs, NineToothedTensor down,
+                                     NineToothedTensor up, NineToothedTensor scales, NineToothedTensor offsets,
+                                     NineToothedTensor adapters, NineToothedTensor output, int dtype, int offsets_dtype,
+                                     int adapters_dtype, void *workspace, size_t workspace_size) {
+    return nt::run_lora(static_cast<cudaStream_t>(stream), lhs, rhs, down, up, scales, offsets, adapters, output, dtype,
+                        offsets_dtype, adapters_dtype, workspace, workspace_size);
+}
+
+size_t launch_lora_matmul_workspace_size(NineToothedTensor lhs, NineToothedTensor down) {
+    if (!lhs.shape || !down.shape) return 0;
+    if (lhs.shape[0] > static_cast<uint64_t>(nt::MAX_DIM) || down.shape[2] > static_cast<uint64_t>(nt::MAX_DIM)) return 0;
+    return static_cast<size_t>(lhs.shape[0]) * nt::rank_blocks(static_cast<int64_t>(down.shape[2])) * nt::RANK_BLOCK * 4;
+}
+
+}  // extern "C"

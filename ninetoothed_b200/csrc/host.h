@@ -15,7 +15,7 @@
 namespace nt {
 
 // Kernel ids recorded in the device status word next to a wait that gave up.
-enum KernelId : uint32_t { KID_GEMM = 1, KID_ATTENTION = 2, KID_CONV2D = 3, KID_SELFTEST = 15 };
+enum KernelId : uint32_t { KID_GEMM = 1, KID_ATTENTION = 2, KID_CONV2D = 3, KID_GROUPED = 4, KID_GROUPED_GRAD = 5, KID_SELFTEST = 15 };
 
 // printf-style: stores the text for ninetoothed_b200_last_error() and returns `code`.
 int fail(int code, const char *fmt, ...);

@@ -18,6 +18,10 @@ _LIBRARY = torch.library.Library("ninetoothed_b200", "DEF")
 _LIBRARY.define("matmul(Tensor lhs, Tensor rhs, Tensor(a!) output) -> ()")
 _LIBRARY.define("bmm(Tensor lhs, Tensor rhs, Tensor(a!) output) -> ()")
 _LIBRARY.define("addmm(Tensor input, Tensor mat1, Tensor mat2, float beta, float alpha, Tensor(a!) output) -> ()")
+_LIBRARY.define("grouped_matmul(Tensor lhs, Tensor rhs, Tensor offsets, Tensor(a!) output) -> ()")
+_LIBRARY.define("grouped_matmul_rhs_grad(Tensor lhs, Tensor output_grad, Tensor offsets, Tensor(a!) rhs_grad) -> ()")
+_LIBRARY.define("lora_matmul(Tensor lhs, Tensor rhs, Tensor down, Tensor up, Tensor scales, Tensor offsets, "
+                "Tensor adapters, Tensor(a!) output) -> ()")
 _LIBRARY.define("softmax(Tensor input, Tensor(a!) output) -> ()")
 _LIBRARY.define("attention(Tensor q, Tensor k, Tensor v, bool is_causal, Tensor(a!) o) -> ()")
 _LIBRARY.define("attention_scaled(Tensor q, Tensor k, Tensor v, float scale, bool is_causal, Tensor(a!) o) -> ()")
@@ -35,6 +39,18 @@ def _bmm(lhs, rhs, output):
 
 def _addmm(input, mat1, mat2, beta, alpha, output):
     _capi.addmm(input, mat1, mat2, beta, alpha, output)
+
+
+def _grouped_matmul(lhs, rhs, offsets, output):
+    _capi.grouped_matmul(lhs, rhs, offsets, output)
+
+
+def _grouped_matmul_rhs_grad(lhs, output_grad, offsets, rhs_grad):
+    _capi.grouped_matmul_rhs_grad(lhs, output_grad, offsets, rhs_grad)
+
+
+def _lora_matmul(lhs, rhs, down, up, scales, offsets, adapters, output):
+    _capi.lora_matmul(lhs, rhs, down, up, scales, offsets, adapters, output)
 
 
 def _softmax(input, output):
@@ -60,6 +76,9 @@ def _max_pool2d(input, output, window_height, window_width, ceil_mode):
 _LIBRARY.impl("matmul", _matmul, "CUDA")
 _LIBRARY.impl("bmm", _bmm, "CUDA")
 _LIBRARY.impl("addmm", _addmm, "CUDA")
+_LIBRARY.impl("grouped_matmul", _grouped_matmul, "CUDA")
+_LIBRARY.impl("grouped_matmul_rhs_grad", _grouped_matmul_rhs_grad, "CUDA")
+_LIBRARY.impl("lora_matmul", _lora_matmul, "CUDA")
 _LIBRARY.impl("softmax", _softmax, "CUDA")
 _LIBRARY.impl("attention", _attention, "CUDA")
 _LIBRARY.impl("attention_scaled", _attention_scaled, "CUDA")
