@@ -36,9 +36,8 @@ constexpr int MAX_RUNS = 2048;  // the table of runs is 16 bytes a run of shared
 constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product: 32 high parts, 32 low parts
 
 enum Mode {
-    PRODUCT,  // tiles of every run, matrix of the run
-    SHRINK,   // the same over the runs that have an adapter; the result is kept as two 16-bit parts
-    LORA,     // tiles over all rows with one matrix; each run's second product is added into its own rows
+    SHRINK,  // tiles of every run that has an adapter, its matrix; the result is kept as two 16-bit parts
+    LORA,    // tiles over all rows with one matrix; each run's second product is added into its own rows
 };
 
 template <int CG, int BN>
@@ -55,6 +54,8 @@ struct Control {
     uint64_t empty[MAX_STAGES];
     uint64_t tmem_full[2];
     uint64_t tmem_empty[2];
+    uint64_t partials;
+    int tile_rows[MAX_STAGES];  // rows of the tiles whose stages are in the ring
     uint32_t tmem_base;
     uint32_t abort_flag;
     int runs;        // entries of the table
@@ -103,6 +104,7 @@ struct Params {
     int64_t scales_stride;
     int rank, rank_blocks;
     int up_mn;  // up has unit stride along its columns, otherwise along its ranks
+    int split;  // CTAs that share a tile's reduction
     unsigned int *status;
 };
 
@@ -175,6 +177,11 @@ struct Place {
 };
 
 __device__ __forceinline__ void raster(int tile, int m_tiles, int n_tiles, int group_m, int &m, int &n) {
+    if (m_tiles <= group_m) {  // one group: a division is some 100 cycles between two tiles
+        n = m_tiles == 1 ? tile : tile / m_tiles;
+        m = tile - n * m_tiles;
+        return;
+    }
     const int per_group = group_m * n_tiles;
     const int group = tile / per_group;
     const int first = group * group_m;
@@ -320,6 +327,9 @@ __device__ __forceinline__ int a_boxes(int valid) {
     return valid <= 0 ? 0 : min(BM / A_CHUNK_ROWS, (valid + A_CHUNK_ROWS - 1) / A_CHUNK_ROWS);
 }
 
+// Producers run their loops as whole warps, so that addresses and coordinates stay in uniform registers, which is where
+// the copy instructions read them; an elected lane issues.  (A lone lane took 130 cycles a copy: the moves between the
+// register files made issuing, not memory, the limit.)
 template <int CG>
 __device__ __forceinline__ void load_2d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y) {
     if constexpr (CG == 1) tma_load_2d(dst, map, bar, x, y);
@@ -592,6 +602,400 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     tcgen05_fence_before_sync();
     __syncthreads();
     if constexpr (CG == 2) cluster_sync();
+    if (warp == 1) {
+        tcgen05_fence_after_sync();
+        tmem_dealloc<CG>(tmem_base, TMEM_COLS);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The grouped product with its operands' parts exchanged: 128 columns of a run's matrix (256 on a CTA pair) are the
+// rows of the accumulator and up to NT of the run's rows its columns, so that a tile's width follows the number of
+// rows it has, in steps of 16 (32), and no part of an instruction is spent on rows of nobody.
+//
+// SPLIT: a cluster of CTAs shares a tile, each taking a share of the reduction, for calls with fewer tiles than the
+// device has SMs.  Every CTA adds up and stores the tile's rows of one share, reading the others' partial sums, in
+// the order of the CTAs, from its own shared memory, where they have put them.
+// ---------------------------------------------------------------------------
+template <int CG, int NT>
+struct Turned {
+    static constexpr int ROWS_CTA = NT / CG;  // rows of lhs that a CTA loads at most
+    // Stages are two 64-deep blocks: half the barriers, and one box holds 128 rows of a matrix.  (A 64-deep block cost its
+    // producer and its issuer 440 cycles whatever its width, more than the products of a narrow tile take.)
+    static constexpr int SUB = 2;
+    static constexpr int DEPTH = BK * SUB;
+    static constexpr int W_BYTES = A_STAGE_BYTES * SUB;
+    static constexpr int X_BYTES = ROWS_CTA * BK * 2;  // one 64-deep block of them
+    static constexpr int STAGE_BYTES = W_BYTES + X_BYTES * SUB;
+    static constexpr int STAGES = 192 * 1024 / STAGE_BYTES < MAX_STAGES ? 192 * 1024 / STAGE_BYTES : MAX_STAGES;
+    static constexpr int TILE_N = BM * CG;
+};
+// Warp 0 copies the matrices, warp 1 issues the products, warps 2 to 9 are the epilogue (two a quadrant of the
+// accumulator, every other 32 rows each), warp 10 copies the rows.
+constexpr int EPILOGUE_WARPS = 8;
+constexpr int ROW_WARP = 2 + EPILOGUE_WARPS;
+constexpr int TURNED_THREADS = (ROW_WARP + 1) * 32;
+constexpr int SPLIT_NT = 64;
+constexpr int SPLIT_STAGES = 3;
+constexpr int SPLIT_BYTES = SPLIT_NT * BM * 4;  // partial sums: for every CTA of the cluster, its share of the rows
+
+template <int CG, int NT, bool SPLIT>
+constexpr int turned_stages() {
+    return SPLIT ? SPLIT_STAGES : Turned<CG, NT>::STAGES;
+}
+
+template <int CG, int NT, bool SPLIT>
+constexpr size_t turned_smem(int runs) {
+    return 1024 + turned_stages<CG, NT, SPLIT>() * Turned<CG, NT>::STAGE_BYTES + CONTROL_BYTES + (SPLIT ? SPLIT_BYTES : 0) +
+           table_bytes(runs);
+}
+
+// A tile: rows [row0, row0 + rows) of a run against columns from col0 of its matrix.
+struct TurnedPlace {
+    int row0, rows, col0, matrix;
+};
+
+template <int CG, int NT>
+struct TurnedWalk {
+    const Run *table;
+    int tile, total, stride, runs, run;
+
+    __device__ TurnedWalk(const Params &p, const Run *table_, const Control *ctl, int first, int step)
+        : table(table_), tile(first), total(ctl->tiles_m * p.n_tiles), stride(step), runs(ctl->runs), run(0) {
+        int high = runs - 1;
+        while (run < high) {  // the last run whose first tile is not behind this one
+            const int mid = (run + high + 1) >> 1;
+            if (table[mid].tiles_before * p.n_tiles <= tile) run = mid;
+            else high = mid - 1;
+        }
+    }
+    __device__ bool more() const { return tile < total; }
+    __device__ void advance() { tile += stride; }
+    __device__ TurnedPlace place(const Params &p) {
+        while (run + 1 < runs && table[run + 1].tiles_before * p.n_tiles <= tile) ++run;
+        const Run r = table[run];
+        const int length = r.end - r.begin, tiles = (length + NT - 1) / NT;
+        constexpr int STEP = 16 * CG;
+        const int even = tiles == 1 ? length : (length + tiles - 1) / tiles;
+        const int share = (even + STEP - 1) / STEP * STEP;  // rows of a tile, in whole steps
+        int m, n;
+        raster(tile - r.tiles_before * p.n_tiles, tiles, p.n_tiles, p.group_m, m, n);
+        return {r.begin + m * share, min(share, length - m * share), n * Turned<CG, NT>::TILE_N, r.matrix};
+    }
+};
+
+// The address of this CTA's shared-memory location in another CTA of the cluster, and a store to such an address.
+__device__ __forceinline__ uint32_t remote_address(const void *local, uint32_t cta) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(cta));
+    return remote;
+}
+__device__ __forceinline__ void store_remote(uint32_t address, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(address), "f"(v) : "memory");
+}
+
+// Bounded wait for arrivals that come from other CTAs of the cluster with data they have written here.
+__device__ __forceinline__ void mbar_wait_cluster(uint64_t *bar, uint32_t parity, const WaitCtx &ctx, uint32_t code) {
+    const uint64_t start = global_timer_ns();
+    while (!mbar_test_wait_cluster(bar, parity)) {
+        const bool failed_before = *ctx.abort_flag != 0;
+        if (global_timer_ns() - start > (failed_before ? WAIT_LIMIT_AFTER_FAILURE_NS : WAIT_LIMIT_NS)) {
+            if (!failed_before) {
+                *ctx.abort_flag = 1;
+                atomicCAS(ctx.status, 0u, STATUS_WAIT_TIMEOUT | (ctx.kernel_id << 16) | code);
+            }
+            return;
+        }
+    }
+}
+
+// 32 rows of a turned accumulator: lane l holds column n of all of them and the warp's 32 columns are neighbours.  Three
+// exchanges with the lanes 1, 2 and 4 away leave every lane with eight neighbouring columns of every eighth row, which
+// are 16-byte stores.  (One 2-byte store a row and lane took 80 cycles a row: more than the products of 2048 terms.)
+__device__ __forceinline__ void store_turned(const uint32_t (&acc)[32], void *out, int64_t stride0, int64_t row0, int rows, int n,
+                                             int n_end, bool bf16) {
+    const int lane = threadIdx.x & 31;
+    const bool odd1 = lane & 1, odd2 = lane & 2, odd4 = lane & 4;
+    uint32_t pair[16];  // two columns of row 2i + (lane & 1)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, odd1 ? acc[2 * i] : acc[2 * i + 1], 1);
+        pair[i] = pack2(__uint_as_float(odd1 ? other : acc[2 * i]), __uint_as_float(odd1 ? acc[2 * i + 1] : other), bf16);
+    }
+    uint32_t four[8][2];  // four columns of row 4i + (lane & 3)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, odd2 ? pair[2 * i] : pair[2 * i + 1], 2);
+        four[i][0] = odd2 ? other : pair[2 * i];
+        four[i][1] = odd2 ? pair[2 * i + 1] : other;
+    }
+    const int col = n - (lane & 7);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // eight columns of row 8i + (lane & 7)
+        const uint32_t other0 = __shfl_xor_sync(0xffffffffu, odd4 ? four[2 * i][0] : four[2 * i + 1][0], 4);
+        const uint32_t other1 = __shfl_xor_sync(0xffffffffu, odd4 ? four[2 * i][1] : four[2 * i + 1][1], 4);
+        uint4 v;
+        v.x = odd4 ? other0 : four[2 * i][0];
+        v.y = odd4 ? other1 : four[2 * i][1];
+        v.z = odd4 ? four[2 * i + 1][0] : other0;
+        v.w = odd4 ? four[2 * i + 1][1] : other1;
+        const int row = 8 * i + (lane & 7);
+        if (row < rows && col < n_end) {
+            uint16_t *dst = static_cast<uint16_t *>(out) + (row0 + row) * stride0 + col;
+            if (col + 8 <= n_end) {
+                *reinterpret_cast<uint4 *>(dst) = v;
+            } else {
+                const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 7; ++j)
+                    if (col + j < n_end) dst[j] = static_cast<uint16_t>(words[j / 2] >> (16 * (j & 1)));
+            }
+        }
+    }
+}
+
+template <int CG, int NT, bool W_MN, bool SPLIT>
+__global__ void __launch_bounds__(TURNED_THREADS, 1)
+    turned_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                  const __grid_constant__ CUtensorMap map_x_chunk, const __grid_constant__ Params p) {
+    using S = Turned<CG, NT>;
+    constexpr int STAGES = turned_stages<CG, NT, SPLIT>();
+    static_assert(!SPLIT || (CG == 1 && NT == SPLIT_NT), "a cluster that splits the reduction holds single CTAs");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Control *ctl = reinterpret_cast<Control *>(smem + STAGES * S::STAGE_BYTES);
+    float *partials = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(ctl) + CONTROL_BYTES);
+    Run *table = reinterpret_cast<Run *>(reinterpret_cast<uint8_t *>(partials) + (SPLIT ? SPLIT_BYTES : 0));
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int lane = threadIdx.x & 31;
+    const WaitCtx wait_ctx{&ctl->abort_flag, p.status, KID_GROUPED};
+    const uint32_t cta_rank = CG == 1 && !SPLIT ? 0u : cluster_cta_rank();
+    const bool leader = SPLIT || cta_rank == 0;
+    const int split = SPLIT ? p.split : 1;
+    const int worker = blockIdx.x / (SPLIT ? split : CG), workers = gridDim.x / (SPLIT ? split : CG);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&ctl->full[s], 1);
+            mbar_init(&ctl->empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&ctl->tmem_full[b], 1);
+            mbar_init(&ctl->tmem_empty[b], EPILOGUE_WARPS * 32 * CG);
+        }
+        if constexpr (SPLIT) mbar_init(&ctl->partials, EPILOGUE_WARPS * split);
+        ctl->abort_flag = 0;
+        mbar_fence_init();
+        tma_prefetch_desc(&map_w);
+        tma_prefetch_desc(&map_x);
+        tma_prefetch_desc(&map_x_chunk);
+    }
+    if (warp == 1) {
+        tmem_alloc<CG>(&ctl->tmem_base, TMEM_COLS);
+        tmem_relinquish<CG>();
+    }
+    build_table(p, table, ctl, NT);
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
+    if constexpr (SPLIT) cluster_arrive();  // (awaited before the first access to another CTA's memory)
+    tcgen05_fence_after_sync();
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+    using W = TurnedWalk<CG, NT>;
+    // this CTA's share of the reduction (a share may be empty)
+    const int kb_first = SPLIT ? p.k_blocks * static_cast<int>(cta_rank) / split : 0;
+    const int kb_last = SPLIT ? p.k_blocks * (static_cast<int>(cta_rank) + 1) / split : p.k_blocks;
+
+    if (warp == 0 || warp == ROW_WARP) {
+        // ------------- TMA producers: warp 0 the matrices, the last warp the rows -------------
+        const bool issuer = elect_one();
+        uint32_t s = 0, phase = 1, tile_it = 0;
+        for (W walk(p, table, ctl, worker, workers); walk.more(); walk.advance(), ++tile_it) {
+            const TurnedPlace at = walk.place(p);
+            constexpr int STEP = 16 * CG;
+            const int width_cta = (at.rows + STEP - 1) / STEP * 16;
+            const int row0 = at.row0 + (CG == 1 ? 0 : static_cast<int>(cta_rank) * width_cta);
+            const int n0 = at.col0 + (CG == 1 ? 0 : static_cast<int>(cta_rank) * BM);
+            const int boxes = (width_cta + A_CHUNK_ROWS - 1) / A_CHUNK_ROWS;
+            const int bytes = CG * (S::W_BYTES + S::SUB * boxes * (A_CHUNK_ROWS * BK * 2));
+            for (int kb = kb_first; kb < kb_last; ++kb) {
+                mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x100 | s);
+                uint8_t *w_dst = smem + s * S::STAGE_BYTES;
+                uint8_t *x_dst = w_dst + S::W_BYTES;
+                if (issuer && warp == 0) {
+                    if (leader) {
+                        // (the issuer of the products learns the tile's rows here: placing a tile takes a few hundred
+                        // cycles, which the producer is ahead and the tensor core would idle)
+                        if (kb == kb_first) ctl->tile_rows[tile_it % MAX_STAGES] = at.rows;
+                        mbar_expect_tx(&ctl->full[s], bytes);
+                    }
+                    if constexpr (W_MN) {
+#pragma unroll
+                        for (int j = 0; j < BM / 64; ++j)
+                            load_3d<CG>(w_dst + j * (S::DEPTH * 128), &map_w, &ctl->full[s], n0 + j * 64, kb * S::DEPTH, at.matrix);
+                    } else {
+#pragma unroll
+                        for (int sub = 0; sub < S::SUB; ++sub)
+                            load_3d<CG>(w_dst + sub * A_STAGE_BYTES, &map_w, &ctl->full[s], kb * S::DEPTH + sub * BK, n0, at.matrix);
+                    }
+                } else if (issuer) {
+#pragma unroll
+                    for (int sub = 0; sub < S::SUB; ++sub) {
+                        const int k0 = kb * S::DEPTH + sub * BK;
+                        if (boxes == S::ROWS_CTA / A_CHUNK_ROWS) {
+                            load_2d<CG>(x_dst + sub * S::X_BYTES, &map_x, &ctl->full[s], k0, row0);
+                        } else {
+                            for (int c = 0; c < boxes; ++c)
+                                load_2d<CG>(x_dst + sub * S::X_BYTES + c * (A_CHUNK_ROWS * BK * 2), &map_x_chunk, &ctl->full[s],
+                                            k0, row0 + c * A_CHUNK_ROWS);
+                        }
+                    }
+                }
+                if (++s == STAGES) {
+                    s = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------- MMA issuer -------------------------------
+        if (leader) {
+            const bool issuer = elect_one();
+            const uint32_t smem_base = smem_u32(smem);
+            uint32_t s = 0, phase = 0, acc_it = 0;
+            bool ready = false;
+            const int total = ctl->tiles_m * p.n_tiles;
+            for (int tile = worker; tile < total; tile += workers, ++acc_it) {
+                constexpr int STEP = 16 * CG;
+                uint32_t idesc = 0;
+                const uint32_t buf = acc_it & 1;
+                mbar_wait_warp(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+                tcgen05_fence_after_sync();
+                const uint32_t tmem_acc = tmem_base + buf * NT;
+                for (int kb = kb_first; kb < kb_last; ++kb) {
+                    if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x300 | s);
+                    tcgen05_fence_after_sync();
+                    if (kb == kb_first) {
+                        const int rows = __shfl_sync(0xffffffffu, ctl->tile_rows[acc_it % MAX_STAGES], 0);
+                        idesc = umma_instr_desc(BM * CG, (rows + STEP - 1) / STEP * STEP, p.bf16 != 0, W_MN, false);
+                    }
+                    const uint32_t w_addr = smem_base + s * S::STAGE_BYTES;
+                    const uint32_t x_addr = w_addr + S::W_BYTES;
+                    const uint32_t s_next = s + 1 == STAGES ? 0 : s + 1;
+                    const uint32_t phase_next = s_next == 0 ? phase ^ 1 : phase;
+#pragma unroll
+                    for (int kk = 0; kk < S::DEPTH / UMMA_K; ++kk) {
+                        const int sub = kk / (BK / UMMA_K), step = kk % (BK / UMMA_K);
+                        const uint64_t desc_w =
+                            W_MN ? umma_smem_desc(w_addr + kk * (UMMA_K * 128), S::DEPTH * 128, 1024)
+                                 : umma_smem_desc(w_addr + sub * A_STAGE_BYTES + step * (UMMA_K * 2), 16, 1024);
+                        const uint64_t desc_x = umma_smem_desc(x_addr + sub * S::X_BYTES + step * (UMMA_K * 2), 16, 1024);
+                        if (issuer) umma_ss<CG>(tmem_acc, desc_w, desc_x, idesc, (kb != kb_first || kk != 0) ? 1u : 0u);
+                        if (kk == S::DEPTH / UMMA_K / 2 - 1)
+                            ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
+                    }
+                    if (issuer) {
+                        if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
+                        else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
+                    }
+                    s = s_next;
+                    phase = phase_next;
+                }
+                if (issuer) {
+                    if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
+                    else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // -------------------------------- epilogue --------------------------------
+        const int quadrant = warp & 3;
+        const int half = (warp - 2) / 4;
+        const int n_lane = quadrant * 32 + lane;
+        const bool bf16 = p.bf16 != 0;
+        uint32_t acc_it = 0;
+        [[maybe_unused]] bool arrived = false;  // at the cluster barrier that ends the kernel
+        if constexpr (SPLIT) cluster_wait();
+        for (W walk(p, table, ctl, worker, workers); walk.more(); walk.advance(), ++acc_it) {
+            const TurnedPlace at = walk.place(p);
+            const int n = at.col0 + (CG == 1 ? 0 : static_cast<int>(cta_rank) * BM) + n_lane;
+            const uint32_t buf = acc_it & 1;
+            mbar_wait(&ctl->tmem_full[buf], (acc_it >> 1) & 1, wait_ctx, 0x400 | buf);
+            tcgen05_fence_after_sync();
+            const uint32_t taddr = tmem_base + buf * NT + (static_cast<uint32_t>(quadrant * 32) << 16);
+            const int64_t column_at = n * p.out_stride1;
+            const int share = SPLIT ? (at.rows + split - 1) / split : 0;  // rows that each CTA of the cluster stores
+#pragma unroll 1
+            for (int t0 = 32 * half; t0 < at.rows; t0 += 64) {
+                uint32_t acc[32];
+                __syncwarp();
+                tmem_ld_32x32(taddr + t0, acc);
+                tmem_wait_ld();
+                if constexpr (SPLIT) {
+                    // row t0 + j goes to the CTA whose share it is, to this CTA's part of that CTA's sums
+                    int cta = t0 / share, row = t0 - cta * share;
+                    const float *mine = partials + static_cast<int>(cta_rank) * share * BM + n_lane;
+                    uint32_t remote = remote_address(mine, cta);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        if (t0 + j >= at.rows) break;
+                        store_remote(remote + row * (BM * 4), kb_first < kb_last ? __uint_as_float(acc[j]) : 0.f);
+                        if (++row == share) {
+                            row = 0;
+                            if (++cta < split) remote = remote_address(mine, cta);
+                        }
+                    }
+                } else if (p.out_vec) {
+                    store_turned(acc, p.out, p.out_stride0, at.row0 + t0, at.rows - t0, n, p.n, bf16);
+                } else if (n < p.n) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (t0 + j < at.rows)
+                            store16(p.out, (at.row0 + t0 + j) * p.out_stride0 + column_at, __uint_as_float(acc[j]), bf16);
+                }
+            }
+            if constexpr (SPLIT) {
+                __syncwarp();  // (one arrival a warp and CTA, after the stores of all its lanes)
+                if (lane < split) mbar_arrive_cluster(&ctl->partials, lane);
+                __syncwarp();
+                cluster_arrive();
+                arrived = true;
+                mbar_wait_cluster(&ctl->partials, 0, wait_ctx, 0x500);
+                const int first = static_cast<int>(cta_rank) * share, last = min(at.rows, first + share);
+                if (n < p.n)
+                    for (int t = first + half; t < last; t += 2) {
+                        float sum = 0.f;
+                        for (int cta = 0; cta < split; ++cta) sum += partials[(cta * share + t - first) * BM + n_lane];
+                        store16(p.out, (at.row0 + t) * p.out_stride0 + column_at, sum, bf16);
+                    }
+            }
+            tcgen05_fence_before_sync();
+            if (CG == 1 || leader) mbar_arrive(&ctl->tmem_empty[buf]);
+            else mbar_arrive_cluster(&ctl->tmem_empty[buf], 0);
+        }
+        if constexpr (SPLIT) {
+            if (!arrived) cluster_arrive();
+        }
+    }
+    if constexpr (SPLIT) {
+        if (warp < 2 || warp == ROW_WARP) {
+            __syncwarp();
+            cluster_wait();
+            cluster_arrive();
+        }
+    }
+
+    __syncwarp();
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
+    if constexpr (SPLIT) {
+        // No CTA leaves while another may still write into its memory.  (The epilogue has arrived early: what is left
+        // of its work is its own CTA's.)
+        cluster_wait();
+    }
     if (warp == 1) {
         tcgen05_fence_after_sync();
         tmem_dealloc<CG>(tmem_base, TMEM_COLS);
@@ -933,10 +1337,10 @@ int map_matrices(const DeviceState &dev, CUtensorMap *map, int dtype, const Matr
 }
 
 template <typename Kernel>
-int active_pairs(Kernel kernel, const DeviceState &dev, size_t smem) {
+int active_pairs(Kernel kernel, const DeviceState &dev, size_t smem, int threads = NUM_THREADS) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(dev.sm_count / 2 * 2));
-    config.blockDim = dim3(NUM_THREADS);
+    config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1026,6 +1430,82 @@ int launch_product(cudaStream_t stream, const DeviceState &dev, int dtype, Maps 
     return launch_shape<1, 64, MODE>(stream, dev, dtype, maps, p, lhs, lhs_stride0, rhs, up);
 }
 
+template <int CG, int NT, bool W_MN, bool SPLIT>
+int launch_turned_kernel(cudaStream_t stream, const DeviceState &dev, const CUtensorMap &map_w, const CUtensorMap &map_x,
+                         const CUtensorMap &map_x_chunk, const Params &p, int64_t most_tiles) {
+    auto kernel = turned_kernel<CG, NT, W_MN, SPLIT>;
+    static_assert(turned_smem<CG, NT, SPLIT>(MAX_RUNS) <= MAX_SMEM, "shared memory per CTA");
+    static thread_local int configured_device = -1;
+    static thread_local int pairs = 0;
+    if (configured_device != dev.device) {
+        NT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SMEM)));
+        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, MAX_SMEM, TURNED_THREADS);
+        configured_device = dev.device;
+    }
+    cudaLaunchConfig_t config = {};
+    const int64_t workers = SPLIT ? most_tiles : std::min<int64_t>(most_tiles, CG == 2 ? pairs : dev.sm_count);
+    if (workers <= 0) return fail(NINETOOTHED_B200_ERR_DEVICE, "grouped matmul: no CTA pair fits this device");
+    const int cluster = SPLIT ? p.split : CG;
+    config.gridDim = dim3(static_cast<unsigned>(workers * cluster));
+    config.blockDim = dim3(TURNED_THREADS);
+    config.dynamicSmemBytes = turned_smem<CG, NT, SPLIT>(p.offsets.runs);
+    config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    if (cluster > 1) {
+        config.attrs = attr;
+        config.numAttrs = 1;
+    }
+    NT_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, map_w, map_x, map_x_chunk, p));
+    return 0;
+}
+
+template <int CG, int NT, bool SPLIT>
+int launch_turned(cudaStream_t stream, const DeviceState &dev, int dtype, Params &p, const void *lhs, int64_t lhs_stride0,
+                  const Matrices &rhs, int64_t live_runs) {
+    using S = Turned<CG, NT>;
+    p.n_tiles = static_cast<int>((static_cast<int64_t>(p.n) + S::TILE_N - 1) / S::TILE_N);
+    p.k_blocks = (p.k + S::DEPTH - 1) / S::DEPTH;
+    p.group_m = std::max(1, 2048 / NT);
+    const bool mn = rhs.use_mn();
+    CUtensorMap map_w, map_x, map_x_chunk;
+    if (int rc = map_matrices(dev, &map_w, dtype, rhs, mn, 64, mn ? S::DEPTH : BM)) return rc;
+    if (int rc = map_rows(dev, &map_x, dtype, lhs, p.rows, p.k, lhs_stride0, BK, S::ROWS_CTA)) return rc;
+    if (int rc = map_rows(dev, &map_x_chunk, dtype, lhs, p.rows, p.k, lhs_stride0, BK, A_CHUNK_ROWS)) return rc;
+    const int64_t most = (live_runs + p.rows / NT) * p.n_tiles;
+    if (most > INT_MAX / 16) return fail(NINETOOTHED_B200_ERR_SHAPE, "grouped matmul: too many tiles");
+    return mn ? launch_turned_kernel<CG, NT, true, SPLIT>(stream, dev, map_w, map_x, map_x_chunk, p, most)
+              : launch_turned_kernel<CG, NT, false, SPLIT>(stream, dev, map_w, map_x, map_x_chunk, p, most);
+}
+
+// Which tiles a grouped product gets.  The bounds lie on the device, so the host goes by averages: `live` runs at most
+// hold rows, and a run of r rows makes about r / NT + 1/2 tiles.
+//   - Fewer tiles than half the SMs: clusters of 2 to 8 CTAs share each tile's reduction (one row against two 4096 x 2048
+//     matrices: 16.0 us without, 11.2 with four CTAs a tile).
+//   - Otherwise the width with the least modelled time, waves x blocks x cycles per 128-deep block (measured: 830 for 64
+//     rows, 1080 for 128, 1540 for 256 on a pair).  Runs of 96, 192 and 384 rows against eight 4096 x 1024 matrices take
+//     19.7, 30.5, 42.5 us with 64 rows a tile, 23.3, 24.3, 39.4 with 128, 24.2, 30.3, 31.4 with 256.
+int launch_grouped(cudaStream_t stream, const DeviceState &dev, int dtype, Params &p, const void *lhs, int64_t lhs_stride0,
+                   const Matrices &rhs, int64_t live) {
+    const int64_t n_tiles = (static_cast<int64_t>(p.n) + BM - 1) / BM;
+    const int64_t few = (live + p.rows / SPLIT_NT) * n_tiles, blocks = (static_cast<int64_t>(p.k) + 2 * BK - 1) / (2 * BK);
+    p.split = 1;
+    while (p.split < 8 && few * p.split * 2 <= dev.sm_count && blocks >= p.split * 4) p.split *= 2;
+    if (p.split > 1) return launch_turned<1, SPLIT_NT, true>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
+    const auto cost = [&](int64_t rows, int64_t columns, int64_t workers, int64_t cycles) {
+        const int64_t halves = std::max<int64_t>(2 * live, 2 * p.rows / rows + live);  // half tiles
+        const int64_t tiles = (halves * ((p.n + columns - 1) / columns) + 1) / 2;
+        return (tiles + workers - 1) / workers * cycles;
+    };
+    const int64_t narrow = cost(64, 128, dev.sm_count, 830), middle = cost(128, 128, dev.sm_count, 1080),
+                  wide = cost(256, 256, dev.sm_count / 2, 1540);
+    if (narrow <= middle && narrow <= wide)
+        return launch_turned<1, 64, false>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
+    if (middle <= wide) return launch_turned<1, 128, false>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
+    return launch_turned<2, 256, false>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
+}
+
 bool has_arrays(const NineToothedTensor &t) { return t.shape != nullptr && t.strides != nullptr; }
 
 constexpr int64_t MAX_DIM = INT_MAX - 4096;  // coordinates of a tile that overhangs stay 32-bit
@@ -1086,8 +1566,7 @@ int run_grouped(cudaStream_t stream, const NineToothedTensor &lhs, const NineToo
     p.status = dev->status;
     const Matrices matrices{rhs.data, runs, k, n, rhs.strides[0], rhs.strides[1], rhs.strides[2]};
     if (rows_addressable(lhs.data, rows, k, lhs.strides[0], lhs.strides[1]) && matrices.addressable()) {
-        Maps maps;
-        return launch_product<PRODUCT>(stream, *dev, dtype, maps, p, lhs.data, lhs.strides[0], matrices, nullptr, std::min(runs, rows));
+        return launch_grouped(stream, *dev, dtype, p, lhs.data, lhs.strides[0], matrices, std::min(runs, rows));
     }
     note_plain_launch("grouped_matmul %lld x %lld x %lld runs on the plain CUDA-core kernel: the tensor-core path needs a "
                       "unit-stride K in lhs, a unit-stride dimension in every matrix of rhs, the other strides multiples "
