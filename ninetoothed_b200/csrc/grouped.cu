@@ -33,6 +33,11 @@ constexpr int TMEM_COLS = 512;
 constexpr int MAX_STAGES = 8;
 constexpr int GROUP_ROWS = 16;  // tile-rows of 128 that share a raster group (L2 reuse of a run's weight panels)
 constexpr int MAX_RUNS = 2048;  // the table of runs is 16 bytes a run of shared memory
+constexpr int SPLIT_NT = 64;     // rows of a tile whose reduction a cluster shares
+constexpr int FEW_ROWS = 256;
+constexpr int FEW_RANK = 128;    // largest rank whose second product the epilogue of a few-row call computes
+constexpr int LOW_WARPS = 8;
+constexpr int LOW_CHUNK = LOW_WARPS * 256;  // terms of a partial sum of (lhs . down) there
 constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product: 32 high parts, 32 low parts
 
 enum Mode {
@@ -79,6 +84,11 @@ size_t smem_bytes(int runs) {
     return 1024 + Shape<CG, BN>::STAGES * Shape<CG, BN>::STAGE_BYTES + CONTROL_BYTES + table_bytes(runs);
 }
 
+struct View {  // up to three dimensions; stride[0] is the matrix index's
+    const void *data;
+    int64_t stride[3];
+};
+
 struct Offsets {
     const void *data;
     int64_t stride;
@@ -105,6 +115,11 @@ struct Params {
     int rank, rank_blocks;
     int up_mn;  // up has unit stride along its columns, otherwise along its ranks
     int split;  // CTAs that share a tile's reduction
+    // few rows under adapters: sums of (lhs . down) over chunks of the reduction [chunks, rows, rank], and up
+    const float *low;
+    int low_chunks;
+    const void *up;
+    int64_t up_stride[3];
     unsigned int *status;
 };
 
@@ -168,6 +183,42 @@ __device__ __forceinline__ void build_table(const Params &p, Run *table, Control
         ctl->tiles_m = tiles;
         ctl->row_begin = first;
         ctl->row_end = bound;
+    }
+}
+
+// The run that holds `row`, or -1: the one before the first bound above it (a bound above `row` that comes first ends
+// the run by the running maximum too).  The lanes of a warp look at 32 bounds at a time.
+__device__ __forceinline__ int run_of(const Offsets &o, int rows, int row) {
+    const int lane = threadIdx.x & 31;
+    for (int base = 0; base <= o.runs; base += 32) {
+        const bool above = base + lane <= o.runs && load_index(o.data, o.stride, o.wide, base + lane, 0, rows) > row;
+        const unsigned votes = __ballot_sync(0xffffffffu, above);
+        if (votes != 0) return base + __ffs(votes) - 2;
+    }
+    return -1;
+}
+
+// The adapter of `row`, or -1 (whole warps call it).
+__device__ __forceinline__ int adapter_of(const Params &p, int row) {
+    const int run = run_of(p.offsets, p.rows, row);
+    if (run < 0) return -1;
+    const int adapter = load_index(p.adapters, p.adapters_stride, p.adapters_wide, run, -1, p.matrices);
+    return adapter < p.matrices ? adapter : -1;
+}
+
+// The rows covered by all runs: from the first bound to the largest.
+__device__ __forceinline__ void build_range(const Params &p, Control *ctl) {
+    if (threadIdx.x >= 32) return;
+    const int lane = threadIdx.x;
+    int largest = 0;
+    for (int i = lane; i <= p.offsets.runs; i += 32)
+        largest = max(largest, load_index(p.offsets.data, p.offsets.stride, p.offsets.wide, i, 0, p.rows));
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    if (lane == 0) {
+        ctl->row_begin = load_index(p.offsets.data, p.offsets.stride, p.offsets.wide, 0, 0, p.rows);
+        ctl->row_end = largest;
+        ctl->tiles_m = (largest - ctl->row_begin + SPLIT_NT - 1) / SPLIT_NT;
+        ctl->runs = 0;
     }
 }
 
@@ -635,7 +686,6 @@ struct Turned {
 constexpr int EPILOGUE_WARPS = 8;
 constexpr int ROW_WARP = 2 + EPILOGUE_WARPS;
 constexpr int TURNED_THREADS = (ROW_WARP + 1) * 32;
-constexpr int SPLIT_NT = 64;
 constexpr int SPLIT_STAGES = 3;
 constexpr int SPLIT_BYTES = SPLIT_NT * BM * 4;  // partial sums: for every CTA of the cluster, its share of the rows
 
@@ -644,10 +694,12 @@ constexpr int turned_stages() {
     return SPLIT ? SPLIT_STAGES : Turned<CG, NT>::STAGES;
 }
 
-template <int CG, int NT, bool SPLIT>
+constexpr int FEW_BYTES = SPLIT_NT * FEW_RANK * 4 + SPLIT_NT * 4;  // (lhs . down) and the adapter of a CTA's rows
+
+template <int CG, int NT, bool SPLIT, bool FEW>
 constexpr size_t turned_smem(int runs) {
     return 1024 + turned_stages<CG, NT, SPLIT>() * Turned<CG, NT>::STAGE_BYTES + CONTROL_BYTES + (SPLIT ? SPLIT_BYTES : 0) +
-           table_bytes(runs);
+           (FEW ? FEW_BYTES : table_bytes(runs));
 }
 
 // A tile: rows [row0, row0 + rows) of a run against columns from col0 of its matrix.
@@ -655,14 +707,15 @@ struct TurnedPlace {
     int row0, rows, col0, matrix;
 };
 
-template <int CG, int NT>
+template <int CG, int NT, bool FEW>
 struct TurnedWalk {
     const Run *table;
-    int tile, total, stride, runs, run;
+    int tile, total, stride, runs, run, range_begin, range_end;
 
     __device__ TurnedWalk(const Params &p, const Run *table_, const Control *ctl, int first, int step)
-        : table(table_), tile(first), total(ctl->tiles_m * p.n_tiles), stride(step), runs(ctl->runs), run(0) {
-        int high = runs - 1;
+        : table(table_), tile(first), total(ctl->tiles_m * p.n_tiles), stride(step), runs(ctl->runs), run(0),
+          range_begin(ctl->row_begin), range_end(ctl->row_end) {
+        int high = FEW ? 0 : runs - 1;
         while (run < high) {  // the last run whose first tile is not behind this one
             const int mid = (run + high + 1) >> 1;
             if (table[mid].tiles_before * p.n_tiles <= tile) run = mid;
@@ -672,6 +725,10 @@ struct TurnedWalk {
     __device__ bool more() const { return tile < total; }
     __device__ void advance() { tile += stride; }
     __device__ TurnedPlace place(const Params &p) {
+        if constexpr (FEW) {  // all rows against one matrix
+            const int n = tile % p.n_tiles, first = range_begin + tile / p.n_tiles * NT;
+            return {first, min(NT, range_end - first), n * Turned<CG, NT>::TILE_N, 0};
+        }
         while (run + 1 < runs && table[run + 1].tiles_before * p.n_tiles <= tile) ++run;
         const Run r = table[run];
         const int length = r.end - r.begin, tiles = (length + NT - 1) / NT;
@@ -690,9 +747,13 @@ __device__ __forceinline__ uint32_t remote_address(const void *local, uint32_t c
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(cta));
     return remote;
 }
-__device__ __forceinline__ void store_remote(uint32_t address, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(address), "f"(v) : "memory");
+__device__ __forceinline__ void store_remote(uint32_t address, const float4 &v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(address), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
+
+// Partial sums lie four rows together: element (row r, column n) of a CTA's part is float r % 4 of float4 r / 4 * 128 + n.
+// The rows that each CTA of the cluster adds up and stores, a whole number of fours.
+__device__ __forceinline__ int split_share(int rows, int split) { return ((rows + split - 1) / split + 3) / 4 * 4; }
 
 // Bounded wait for arrivals that come from other CTAs of the cluster with data they have written here.
 __device__ __forceinline__ void mbar_wait_cluster(uint64_t *bar, uint32_t parity, const WaitCtx &ctx, uint32_t code) {
@@ -706,6 +767,185 @@ __device__ __forceinline__ void mbar_wait_cluster(uint64_t *bar, uint32_t parity
             }
             return;
         }
+    }
+}
+
+__device__ __forceinline__ void griddepcontrol_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void griddepcontrol_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(EPILOGUE_WARPS * 32) : "memory"); }
+
+__device__ __forceinline__ float half_of(uint32_t pair, int i, bool bf16) {
+    const uint32_t bits = i ? pair >> 16 : pair & 0xffffu;
+    return bf16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+}
+
+// 16 bytes or less of a row of 16-bit values from `at` on, zeros behind `left` elements.  Aligned to `N` elements.
+template <int N>
+__device__ __forceinline__ void load_values(const uint16_t *at, int left, bool bf16, float (&v)[N]) {
+    if (left >= N) {
+        uint32_t words[N / 2];
+        if constexpr (N == 8) *reinterpret_cast<uint4 *>(words) = __ldg(reinterpret_cast<const uint4 *>(at));
+        else *reinterpret_cast<uint2 *>(words) = __ldg(reinterpret_cast<const uint2 *>(at));
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = half_of(words[j / 2], j & 1, bf16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = j < left ? load16(at, j, bf16) : 0.f;
+    }
+}
+
+__device__ __forceinline__ void prefetch_l2(const void *at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at)); }
+
+// scales (lhs . down) . up of the rows that this CTA stores into its own slot of the partial sums.  A warp takes a row, a
+// lane four columns of the tile.  What does not depend on the launch before (which adapter, its matrix on the way to L2)
+// is done before the wait for it.
+__device__ __forceinline__ void adapters_part(const Params &p, const TurnedPlace &at, float *partials, float *low, int *row_adapter,
+                                              int cta_rank, int split) {
+    const int warp = static_cast<int>(threadIdx.x) / 32 - 2, lane = threadIdx.x & 31;
+    const bool bf16 = p.bf16 != 0;
+    const int share = split_share(at.rows, split);
+    const int first = cta_rank * share, mine = min(at.rows, first + share) - first;
+    const int row0 = at.row0 + first, col = at.col0 + lane * 4, left = p.n - col;
+    const uint16_t *up = static_cast<const uint16_t *>(p.up);
+    for (int t = warp; t < mine; t += EPILOGUE_WARPS) {
+        const int adapter = adapter_of(p, row0 + t);
+        if (lane == 0) row_adapter[t] = adapter;
+        if (adapter < 0) continue;
+        const uint16_t *matrix = up + adapter * p.up_stride[0];
+        if (p.up_mn) {
+            for (int i = lane; i < 2 * p.rank; i += 32)
+                if (at.col0 + (i & 1) * 64 < p.n) prefetch_l2(matrix + (i / 2) * p.up_stride[1] + at.col0 + (i & 1) * 64);
+        } else {
+            for (int j = 0; j < 4 && j < left; ++j)
+                for (int r = 0; r < p.rank; r += 64) prefetch_l2(matrix + (col + j) * p.up_stride[2] + r);
+        }
+    }
+    griddepcontrol_wait();  // (the sums of lhs . down come from the launch before)
+    for (int t = warp; t < mine; t += EPILOGUE_WARPS) {
+        __syncwarp();
+        const int adapter = row_adapter[t];
+        float sum[4] = {};
+        if (adapter >= 0) {
+            const float scale = p.scales[adapter * p.scales_stride];
+            float *l = low + t * p.rank;
+            for (int r = lane; r < p.rank; r += 32) {
+                const float *part = p.low + static_cast<int64_t>(row0 + t) * p.rank + r;
+                float total = 0.f;
+#pragma unroll 4
+                for (int c = 0; c < p.low_chunks; ++c) total += __ldcg(part + static_cast<int64_t>(c) * p.rows * p.rank);
+                l[r] = scale * total;
+            }
+            __syncwarp();
+            const uint16_t *matrix = up + adapter * p.up_stride[0];
+            if (left >= 4 && p.up_mn) {
+                for (int r0 = 0; r0 < p.rank; r0 += 16) {  // sixteen loads in flight
+                    uint2 v[16];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        v[r] = r0 + r < p.rank ? __ldg(reinterpret_cast<const uint2 *>(matrix + (r0 + r) * p.up_stride[1] + col)) : make_uint2(0, 0);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float weight = r0 + r < p.rank ? l[r0 + r] : 0.f;
+                        sum[0] = fmaf(weight, half_of(v[r].x, 0, bf16), sum[0]);
+                        sum[1] = fmaf(weight, half_of(v[r].x, 1, bf16), sum[1]);
+                        sum[2] = fmaf(weight, half_of(v[r].y, 0, bf16), sum[2]);
+                        sum[3] = fmaf(weight, half_of(v[r].y, 1, bf16), sum[3]);
+                    }
+                }
+            } else if (left >= 4 && p.rank % 8 == 0) {  // a column's ranks lie side by side
+                for (int r0 = 0; r0 < p.rank; r0 += 32) {
+                    uint4 v[4][4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            v[q][j] = r0 + q * 8 < p.rank
+                                          ? __ldg(reinterpret_cast<const uint4 *>(matrix + (col + j) * p.up_stride[2] + r0 + q * 8))
+                                          : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (r0 + q * 8 >= p.rank) break;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t words[4] = {v[q][j].x, v[q][j].y, v[q][j].z, v[q][j].w};
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) sum[j] = fmaf(l[r0 + q * 8 + i], half_of(words[i / 2], i & 1, bf16), sum[j]);
+                        }
+                    }
+                }
+            } else {
+                for (int r = 0; r < p.rank; ++r)
+                    for (int j = 0; j < 4 && j < left; ++j)
+                        sum[j] = fmaf(l[r], load16(matrix, r * p.up_stride[1] + (col + j) * p.up_stride[2], bf16), sum[j]);
+            }
+        }
+        float *dst = partials + ((cta_rank * share + t) / 4 * BM + lane * 4) * 4 + t % 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dst[j * 4] = sum[j];
+    }
+    epilogue_sync();
+}
+
+// Partial sums of lhs . down over chunks of the reduction, for calls with few rows: a block takes a row, a chunk and eight
+// ranks, a warp 256 terms of them.  All latency: every lane's loads are independent, and its part of the row is asked for
+// before the row's adapter is looked up.
+__global__ void __launch_bounds__(LOW_WARPS * 32) low_kernel(const __grid_constant__ Params p, const void *lhs, int64_t lhs_stride0,
+                                                             View down, int down_mn, float *low) {
+    griddepcontrol_launch_dependents();  // (the projection starts at once and waits for this kernel before it reads `low`)
+    __shared__ float sums[LOW_WARPS][8];
+    const bool bf16 = p.bf16 != 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, groups = (p.rank + 7) / 8;
+    const int task = blockIdx.x, row = task / (p.low_chunks * groups), rest = task - row * (p.low_chunks * groups);
+    const int chunk = rest / groups, r0 = (rest - chunk * groups) * 8;
+    const int k0 = chunk * LOW_CHUNK + warp * 256;
+    const uint16_t *x = static_cast<const uint16_t *>(lhs) + row * lhs_stride0;
+    float xs[8];
+    if (down_mn) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) xs[i] = k0 + i * 32 + lane < p.k ? load16(x, k0 + i * 32 + lane, bf16) : 0.f;
+    } else {
+        load_values<8>(x + k0 + lane * 8, p.k - (k0 + lane * 8), bf16, xs);
+    }
+    const int adapter = adapter_of(p, row);
+    if (adapter < 0) return;
+    const uint16_t *d = static_cast<const uint16_t *>(down.data) + adapter * down.stride[0];
+    float acc[8] = {};
+    if (down_mn) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int k = k0 + i * 32 + lane;
+            if (k >= p.k) continue;
+            float v[8];
+            load_values<8>(d + k * down.stride[1] + r0, p.rank - r0, bf16, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] = fmaf(xs[i], v[j], acc[j]);
+        }
+    } else {
+        const int k = k0 + lane * 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (r0 + j >= p.rank || k >= p.k) continue;
+            float v[8];
+            load_values<8>(d + (r0 + j) * down.stride[2] + k, p.k - k, bf16, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[j] = fmaf(xs[i], v[i], acc[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int d2 = 16; d2 > 0; d2 /= 2) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], d2);
+    float mine = acc[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mine = lane == j ? acc[j] : mine;
+    if (lane < 8) sums[warp][lane] = mine;
+    __syncthreads();
+    if (threadIdx.x < 8 && r0 + static_cast<int>(threadIdx.x) < p.rank) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < LOW_WARPS; ++w) sum += sums[w][threadIdx.x];
+        low[(static_cast<int64_t>(chunk) * p.rows + row) * p.rank + r0 + threadIdx.x] = sum;
     }
 }
 
@@ -754,18 +994,25 @@ __device__ __forceinline__ void store_turned(const uint32_t (&acc)[32], void *ou
     }
 }
 
-template <int CG, int NT, bool W_MN, bool SPLIT>
+// FEW: the shared projection and the adapters of a call with few rows.  The epilogue's warps, idle while the tile's
+// products run, compute the adapters' part of the rows that their CTA will store, (lhs . down) . up in fp32, and put it
+// where the CTA's own partial sums are added to it.
+template <int CG, int NT, bool W_MN, bool SPLIT, bool FEW>
 __global__ void __launch_bounds__(TURNED_THREADS, 1)
     turned_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                   const __grid_constant__ CUtensorMap map_x_chunk, const __grid_constant__ Params p) {
     using S = Turned<CG, NT>;
     constexpr int STAGES = turned_stages<CG, NT, SPLIT>();
     static_assert(!SPLIT || (CG == 1 && NT == SPLIT_NT), "a cluster that splits the reduction holds single CTAs");
+    static_assert(!FEW || SPLIT, "few rows");
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Control *ctl = reinterpret_cast<Control *>(smem + STAGES * S::STAGE_BYTES);
     float *partials = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(ctl) + CONTROL_BYTES);
+    // (one or the other)
     Run *table = reinterpret_cast<Run *>(reinterpret_cast<uint8_t *>(partials) + (SPLIT ? SPLIT_BYTES : 0));
+    float *low = reinterpret_cast<float *>(table);
+    int *row_adapter = reinterpret_cast<int *>(low + SPLIT_NT * FEW_RANK);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
@@ -795,14 +1042,15 @@ __global__ void __launch_bounds__(TURNED_THREADS, 1)
         tmem_alloc<CG>(&ctl->tmem_base, TMEM_COLS);
         tmem_relinquish<CG>();
     }
-    build_table(p, table, ctl, NT);
+    if constexpr (FEW) build_range(p, ctl);
+    else build_table(p, table, ctl, NT);
     tcgen05_fence_before_sync();
     __syncthreads();
     if constexpr (CG == 2) cluster_sync();
     if constexpr (SPLIT) cluster_arrive();  // (awaited before the first access to another CTA's memory)
     tcgen05_fence_after_sync();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
-    using W = TurnedWalk<CG, NT>;
+    using W = TurnedWalk<CG, NT, FEW>;
     // this CTA's share of the reduction (a share may be empty)
     const int kb_first = SPLIT ? p.k_blocks * static_cast<int>(cta_rank) / split : 0;
     const int kb_last = SPLIT ? p.k_blocks * (static_cast<int>(cta_rank) + 1) / split : p.k_blocks;
@@ -922,11 +1170,13 @@ __global__ void __launch_bounds__(TURNED_THREADS, 1)
             const TurnedPlace at = walk.place(p);
             const int n = at.col0 + (CG == 1 ? 0 : static_cast<int>(cta_rank) * BM) + n_lane;
             const uint32_t buf = acc_it & 1;
+            if constexpr (FEW)
+                adapters_part(p, at, partials, low, row_adapter, static_cast<int>(cta_rank), split);
             mbar_wait(&ctl->tmem_full[buf], (acc_it >> 1) & 1, wait_ctx, 0x400 | buf);
             tcgen05_fence_after_sync();
             const uint32_t taddr = tmem_base + buf * NT + (static_cast<uint32_t>(quadrant * 32) << 16);
             const int64_t column_at = n * p.out_stride1;
-            const int share = SPLIT ? (at.rows + split - 1) / split : 0;  // rows that each CTA of the cluster stores
+            const int share = SPLIT ? split_share(at.rows, split) : 0;
 #pragma unroll 1
             for (int t0 = 32 * half; t0 < at.rows; t0 += 64) {
                 uint32_t acc[32];
@@ -934,18 +1184,25 @@ __global__ void __launch_bounds__(TURNED_THREADS, 1)
                 tmem_ld_32x32(taddr + t0, acc);
                 tmem_wait_ld();
                 if constexpr (SPLIT) {
-                    // row t0 + j goes to the CTA whose share it is, to this CTA's part of that CTA's sums
-                    int cta = t0 / share, row = t0 - cta * share;
-                    const float *mine = partials + static_cast<int>(cta_rank) * share * BM + n_lane;
-                    uint32_t remote = remote_address(mine, cta);
+                    // four rows at a time to the CTA whose share they are, into this CTA's part there
+                    float4 *part = reinterpret_cast<float4 *>(partials) + static_cast<int>(cta_rank) * (share / 4) * BM + n_lane;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
+                    for (int j = 0; j < 32; j += 4) {
                         if (t0 + j >= at.rows) break;
-                        store_remote(remote + row * (BM * 4), kb_first < kb_last ? __uint_as_float(acc[j]) : 0.f);
-                        if (++row == share) {
-                            row = 0;
-                            if (++cta < split) remote = remote_address(mine, cta);
+                        const int cta = (t0 + j) / share;
+                        float4 *dst = part + (t0 + j - cta * share) / 4 * BM;
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (kb_first < kb_last)
+                            v = make_float4(__uint_as_float(acc[j]), __uint_as_float(acc[j + 1]), __uint_as_float(acc[j + 2]),
+                                            __uint_as_float(acc[j + 3]));
+                        if (FEW && cta == static_cast<int>(cta_rank)) {
+                            const float4 adapters = *dst;
+                            v.x += adapters.x;
+                            v.y += adapters.y;
+                            v.z += adapters.z;
+                            v.w += adapters.w;
                         }
+                        store_remote(remote_address(dst, cta), v);
                     }
                 } else if (p.out_vec) {
                     store_turned(acc, p.out, p.out_stride0, at.row0 + t0, at.rows - t0, n, p.n, bf16);
@@ -965,16 +1222,27 @@ __global__ void __launch_bounds__(TURNED_THREADS, 1)
                 mbar_wait_cluster(&ctl->partials, 0, wait_ctx, 0x500);
                 const int first = static_cast<int>(cta_rank) * share, last = min(at.rows, first + share);
                 if (n < p.n)
-                    for (int t = first + half; t < last; t += 2) {
-                        float sum = 0.f;
-                        for (int cta = 0; cta < split; ++cta) sum += partials[(cta * share + t - first) * BM + n_lane];
-                        store16(p.out, (at.row0 + t) * p.out_stride0 + column_at, sum, bf16);
+                    for (int t = first + 4 * half; t < last; t += 8) {
+                        const float4 *part = reinterpret_cast<const float4 *>(partials) + (t - first) / 4 * BM + n_lane;
+                        float sum[4] = {};
+#pragma unroll 4
+                        for (int cta = 0; cta < split; ++cta) {
+                            const float4 v = part[cta * (share / 4) * BM];
+                            sum[0] += v.x;
+                            sum[1] += v.y;
+                            sum[2] += v.z;
+                            sum[3] += v.w;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (t + j < last) store16(p.out, (at.row0 + t + j) * p.out_stride0 + column_at, sum[j], bf16);
                     }
             }
             tcgen05_fence_before_sync();
             if (CG == 1 || leader) mbar_arrive(&ctl->tmem_empty[buf]);
             else mbar_arrive_cluster(&ctl->tmem_empty[buf], 0);
         }
+        if constexpr (FEW) griddepcontrol_wait();  // (also where there was no tile: what follows this launch may rely on the one before)
         if constexpr (SPLIT) {
             if (!arrived) cluster_arrive();
         }
@@ -1208,22 +1476,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 // ---------------------------------------------------------------------------
 // Plain kernels for operands that no tensor map can address: one thread per output element, fp32 sums, one rounding.
 // ---------------------------------------------------------------------------
-struct View {  // up to three dimensions; stride[0] is the matrix index's
-    const void *data;
-    int64_t stride[3];
-};
-
-// The run that holds `row` by the rule of build_table, or -1.
-__device__ int run_of(const Offsets &o, int rows, int row) {
-    int bound = load_index(o.data, o.stride, o.wide, 0, 0, rows);
-    if (row < bound) return -1;
-    for (int e = 0; e < o.runs; ++e) {
-        bound = max(bound, load_index(o.data, o.stride, o.wide, e + 1, 0, rows));
-        if (row < bound) return e;
-    }
-    return -1;
-}
-
 constexpr int PLAIN_ROWS = 8;
 
 // low (may be nullptr, as may adapters): fp32 [rows, rank], added as low . up of the run's adapter.
@@ -1232,13 +1484,8 @@ __global__ void __launch_bounds__(256)
                          int matrices, int shared_matrix, View a, View b, const float *low, int rank, View up, int rows,
                          int n, int k, const float *scales, int64_t scales_stride, float *low_out, void *out,
                          int64_t os0, int64_t os1, int bf16) {
-    __shared__ int runs[PLAIN_ROWS];
-    const int64_t block_row = static_cast<int64_t>(blockIdx.x) * PLAIN_ROWS;
-    if (threadIdx.x < PLAIN_ROWS)
-        runs[threadIdx.x] = block_row + threadIdx.x < rows ? run_of(offsets, rows, static_cast<int>(block_row + threadIdx.x)) : -1;
-    __syncthreads();
-    const int64_t row = block_row + threadIdx.x / 32;
-    const int run = runs[threadIdx.x / 32];
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * PLAIN_ROWS + threadIdx.x / 32;  // one warp a row
+    const int run = row < rows ? run_of(offsets, rows, static_cast<int>(row)) : -1;
     if (run < 0) return;
     int matrix = run;
     if (adapters != nullptr) {
@@ -1430,11 +1677,11 @@ int launch_product(cudaStream_t stream, const DeviceState &dev, int dtype, Maps 
     return launch_shape<1, 64, MODE>(stream, dev, dtype, maps, p, lhs, lhs_stride0, rhs, up);
 }
 
-template <int CG, int NT, bool W_MN, bool SPLIT>
+template <int CG, int NT, bool W_MN, bool SPLIT, bool FEW>
 int launch_turned_kernel(cudaStream_t stream, const DeviceState &dev, const CUtensorMap &map_w, const CUtensorMap &map_x,
                          const CUtensorMap &map_x_chunk, const Params &p, int64_t most_tiles) {
-    auto kernel = turned_kernel<CG, NT, W_MN, SPLIT>;
-    static_assert(turned_smem<CG, NT, SPLIT>(MAX_RUNS) <= MAX_SMEM, "shared memory per CTA");
+    auto kernel = turned_kernel<CG, NT, W_MN, SPLIT, FEW>;
+    static_assert(turned_smem<CG, NT, SPLIT, FEW>(MAX_RUNS) <= MAX_SMEM, "shared memory per CTA");
     static thread_local int configured_device = -1;
     static thread_local int pairs = 0;
     if (configured_device != dev.device) {
@@ -1448,20 +1695,24 @@ int launch_turned_kernel(cudaStream_t stream, const DeviceState &dev, const CUte
     const int cluster = SPLIT ? p.split : CG;
     config.gridDim = dim3(static_cast<unsigned>(workers * cluster));
     config.blockDim = dim3(TURNED_THREADS);
-    config.dynamicSmemBytes = turned_smem<CG, NT, SPLIT>(p.offsets.runs);
+    config.dynamicSmemBytes = turned_smem<CG, NT, SPLIT, FEW>(p.offsets.runs);
     config.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    cudaLaunchAttribute attr[2];
+    config.attrs = attr;
+    config.numAttrs = 0;
     if (cluster > 1) {
-        config.attrs = attr;
-        config.numAttrs = 1;
+        attr[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[config.numAttrs++].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    }
+    if (FEW && p.low_chunks > 0) {  // starts under the kernel before it
+        attr[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
     NT_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, map_w, map_x, map_x_chunk, p));
     return 0;
 }
 
-template <int CG, int NT, bool SPLIT>
+template <int CG, int NT, bool SPLIT, bool FEW = false>
 int launch_turned(cudaStream_t stream, const DeviceState &dev, int dtype, Params &p, const void *lhs, int64_t lhs_stride0,
                   const Matrices &rhs, int64_t live_runs) {
     using S = Turned<CG, NT>;
@@ -1473,10 +1724,10 @@ int launch_turned(cudaStream_t stream, const DeviceState &dev, int dtype, Params
     if (int rc = map_matrices(dev, &map_w, dtype, rhs, mn, 64, mn ? S::DEPTH : BM)) return rc;
     if (int rc = map_rows(dev, &map_x, dtype, lhs, p.rows, p.k, lhs_stride0, BK, S::ROWS_CTA)) return rc;
     if (int rc = map_rows(dev, &map_x_chunk, dtype, lhs, p.rows, p.k, lhs_stride0, BK, A_CHUNK_ROWS)) return rc;
-    const int64_t most = (live_runs + p.rows / NT) * p.n_tiles;
+    const int64_t most = (FEW ? (p.rows + NT - 1) / NT : live_runs + p.rows / NT) * p.n_tiles;
     if (most > INT_MAX / 16) return fail(NINETOOTHED_B200_ERR_SHAPE, "grouped matmul: too many tiles");
-    return mn ? launch_turned_kernel<CG, NT, true, SPLIT>(stream, dev, map_w, map_x, map_x_chunk, p, most)
-              : launch_turned_kernel<CG, NT, false, SPLIT>(stream, dev, map_w, map_x, map_x_chunk, p, most);
+    return mn ? launch_turned_kernel<CG, NT, true, SPLIT, FEW>(stream, dev, map_w, map_x, map_x_chunk, p, most)
+              : launch_turned_kernel<CG, NT, false, SPLIT, FEW>(stream, dev, map_w, map_x, map_x_chunk, p, most);
 }
 
 // Which tiles a grouped product gets.  The bounds lie on the device, so the host goes by averages: `live` runs at most
@@ -1504,6 +1755,40 @@ int launch_grouped(cudaStream_t stream, const DeviceState &dev, int dtype, Param
         return launch_turned<1, 64, false>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
     if (middle <= wide) return launch_turned<1, 128, false>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
     return launch_turned<2, 256, false>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
+}
+
+// Few rows under adapters: their share of the output costs no tile of its own, and runs under the streaming of rhs.
+int64_t low_chunks(int64_t k) { return (k + LOW_CHUNK - 1) / LOW_CHUNK; }
+
+bool few_rows(int64_t rows, int64_t rank) { return rows <= FEW_ROWS && rank <= FEW_RANK; }
+
+size_t lora_workspace(int64_t rows, int64_t k, int64_t rank) {
+    const size_t parts = static_cast<size_t>(rows) * ((rank + RANK_BLOCK - 1) / RANK_BLOCK) * RANK_BLOCK * 4;
+    const size_t sums = few_rows(rows, rank) ? static_cast<size_t>(low_chunks(k)) * rows * rank * 4 : 0;
+    return std::max(parts, sums);
+}
+
+int launch_few(cudaStream_t stream, const DeviceState &dev, int dtype, Params &p, const void *lhs, int64_t lhs_stride0,
+               const Matrices &rhs, const Matrices &down, const Matrices &up, float *low) {
+    p.low_chunks = 0;
+    if (p.matrices > 0) {
+        p.low = low;
+        p.low_chunks = static_cast<int>(low_chunks(p.k));
+        p.up = up.data;
+        p.up_mn = up.use_mn();
+        p.up_stride[0] = up.stride0;
+        p.up_stride[1] = up.stride1;
+        p.up_stride[2] = up.stride2;
+        const int64_t tasks = static_cast<int64_t>(p.rows) * p.low_chunks * ((p.rank + 7) / 8);
+        low_kernel<<<static_cast<unsigned>(tasks), LOW_WARPS * 32, 0, stream>>>(
+            p, lhs, lhs_stride0, View{down.data, {down.stride0, down.stride1, down.stride2}}, down.use_mn(), low);
+        NT_CUDA_CHECK(cudaGetLastError());
+    }
+    const int64_t tiles = (static_cast<int64_t>(p.rows) + SPLIT_NT - 1) / SPLIT_NT * ((static_cast<int64_t>(p.n) + BM - 1) / BM);
+    const int64_t blocks = (static_cast<int64_t>(p.k) + 2 * BK - 1) / (2 * BK);
+    p.split = 1;
+    while (p.split < 8 && tiles * p.split * 2 <= dev.sm_count && blocks >= p.split * 2) p.split *= 2;
+    return launch_turned<1, SPLIT_NT, true, true>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, 1);
 }
 
 bool has_arrays(const NineToothedTensor &t) { return t.shape != nullptr && t.strides != nullptr; }
@@ -1682,7 +1967,7 @@ int run_lora(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothe
     if (!output.data || !adapters.data || (k > 0 && (!lhs.data || !rhs.data)) ||
         (any && (!down.data || !up.data || !scales.data)))
         return fail(NINETOOTHED_B200_ERR_ARGUMENT, "%s: null data pointer", what);
-    const size_t needed = static_cast<size_t>(rows) * rank_blocks(rank) * RANK_BLOCK * 4;
+    const size_t needed = lora_workspace(rows, k, rank);
     if (any && (workspace == nullptr || workspace_size < needed || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
         return fail(NINETOOTHED_B200_ERR_ARGUMENT, "%s: needs a 256-byte aligned workspace of %zu bytes, got %zu at %p", what,
                     needed, workspace_size, workspace);
@@ -1706,6 +1991,14 @@ int run_lora(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothe
     const Matrices second{up.data, count, rank, n, up.strides[0], up.strides[1], up.strides[2]};
     if (rows_addressable(lhs.data, rows, k, lhs.strides[0], lhs.strides[1]) && shared.addressable() &&
         (!any || (first.addressable() && second.addressable()))) {
+        if (few_rows(rows, rank)) {
+            p.n = static_cast<int>(n);
+            p.out = output.data;
+            p.out_stride0 = output.strides[0];
+            p.out_stride1 = output.strides[1];
+            p.out_vec = output_vec(output, 0);
+            return launch_few(stream, *dev, dtype, p, lhs.data, lhs.strides[0], shared, first, second, static_cast<float *>(workspace));
+        }
         Maps maps;
         if (any) {
             Params shrink = p;
@@ -1773,7 +2066,7 @@ NineToothedResult launch_lora_matmul(NineToothedStream stream, NineToothedTensor
 size_t launch_lora_matmul_workspace_size(NineToothedTensor lhs, NineToothedTensor down) {
     if (!lhs.shape || !down.shape) return 0;
     if (lhs.shape[0] > static_cast<uint64_t>(nt::MAX_DIM) || down.shape[2] > static_cast<uint64_t>(nt::MAX_DIM)) return 0;
-    return static_cast<size_t>(lhs.shape[0]) * nt::rank_blocks(static_cast<int64_t>(down.shape[2])) * nt::RANK_BLOCK * 4;
+    return nt::lora_workspace(static_cast<int64_t>(lhs.shape[0]), static_cast<int64_t>(lhs.shape[1]), static_cast<int64_t>(down.shape[2]));
 }
 
 }  // extern "C"
