@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <climits>
 #include <cstdint>
+#include <type_traits>
 
 #include "host.h"
 #include "ptx.cuh"
@@ -60,6 +61,8 @@ struct Control {
     uint64_t tmem_full[2];
     uint64_t tmem_empty[2];
     uint64_t partials;
+    uint64_t ragged[MAX_STAGES];
+    uint64_t partner[MAX_STAGES];
     int tile_rows[MAX_STAGES];  // rows of the tiles whose stages are in the ring
     uint32_t tmem_base;
     uint32_t abort_flag;
@@ -74,7 +77,7 @@ struct Run {
     int begin, end, matrix, tiles_before;
 };
 
-constexpr int CONTROL_BYTES = 256;
+constexpr int CONTROL_BYTES = 384;
 static_assert(sizeof(Control) <= CONTROL_BYTES, "control block");
 
 constexpr size_t table_bytes(int runs) { return static_cast<size_t>(runs + 1) * sizeof(Run); }
@@ -686,6 +689,7 @@ struct Turned {
 constexpr int EPILOGUE_WARPS = 8;
 constexpr int ROW_WARP = 2 + EPILOGUE_WARPS;
 constexpr int TURNED_THREADS = (ROW_WARP + 1) * 32;
+constexpr int GRAD_THREADS = TURNED_THREADS + 32;  // and a warp that clears what a run's last block holds of the next run
 constexpr int SPLIT_STAGES = 3;
 constexpr int SPLIT_BYTES = SPLIT_NT * BM * 4;  // partial sums: for every CTA of the cluster, its share of the rows
 
@@ -1309,137 +1313,220 @@ __device__ __forceinline__ void build_starts(const Offsets &offsets, int rows, i
     }
 }
 
-template <int BN>
-size_t grad_smem_bytes(int runs) {
-    return 1024 + Shape<1, BN>::STAGES * Shape<1, BN>::STAGE_BYTES + CONTROL_BYTES + static_cast<size_t>(runs + 1) * 4;
+// Two shapes: 256 x 256 tiles on CTA pairs, whose CTAs each bring 128 columns of either operand, and 128 x 128 tiles on
+// single CTAs for gradients with few tiles.  Warp 0 copies lhs, warp 1 issues the products, warps 2 to 9 are the epilogue,
+// warp 10 copies output_grad.
+//
+// In a pair the even CTA's barriers count both CTAs' copies, but each CTA has to overwrite its own rows: a ragged block is
+// therefore copied against a barrier of its own in each CTA, whose warp 11 overwrites the rows, ahead of the issuer like the
+// copies; the odd CTA's then tells the even CTA's, and that the issuer.
+template <int CG, int BN>
+struct Grad {
+    static constexpr int BN_CTA = BN / CG;
+    static constexpr int STAGE_BYTES = A_STAGE_BYTES + BN_CTA * BK * 2;
+    static constexpr int STAGES = 5;
+    static constexpr int TILE_M = BM * CG;
+    static constexpr int BOX_BYTES = BK * 128;  // 64 rows of 64 columns
+    static constexpr int OUT_BYTES = EPILOGUE_WARPS * 32 * 128;  // a box of 32 rows of 64 columns for every epilogue warp
+};
+
+template <int CG, int BN>
+constexpr size_t grad_smem(int runs) {
+    return 1024 + Grad<CG, BN>::STAGES * Grad<CG, BN>::STAGE_BYTES + Grad<CG, BN>::OUT_BYTES + CONTROL_BYTES +
+           static_cast<size_t>(runs + 1) * 4;
 }
 
-template <int BN>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
-    grouped_grad_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                        const __grid_constant__ GradParams p) {
-    using S = Shape<1, BN>;
+struct GradTile {
+    int run, m0, n0, length, begin;
+};
+
+// Tiles of a run follow one another with the rows of the gradient fastest, so that CTAs at work share panels.
+__device__ __forceinline__ GradTile grad_tile(const GradParams &p, const int *starts, int tile, int tile_m, int tile_n) {
+    const int per_run = p.m_tiles * p.n_tiles;
+    const int run = tile / per_run, inside = tile - run * per_run;
+    const int n = inside / p.m_tiles;
+    return {run, (inside - n * p.m_tiles) * tile_m, n * tile_n, starts[run + 1] - starts[run], starts[run]};
+}
+
+__device__ __forceinline__ void fence_cluster() {
+    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async;" ::: "memory");
+}
+
+template <int CG, int BN>
+__global__ void __launch_bounds__(GRAD_THREADS, 1)
+    grad_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ GradParams p) {
+    using S = Grad<CG, BN>;
     constexpr int STAGES = S::STAGES;
-    constexpr int BOX_BYTES = BK * 128;  // 64 rows of 64 columns
-    constexpr int BOXES = (BM + BN) / 64;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    Control *ctl = reinterpret_cast<Control *>(smem + STAGES * S::STAGE_BYTES);
+    uint8_t *boxes = smem + STAGES * S::STAGE_BYTES;
+    Control *ctl = reinterpret_cast<Control *>(boxes + S::OUT_BYTES);
     int *starts = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(ctl) + CONTROL_BYTES);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
     const WaitCtx wait_ctx{&ctl->abort_flag, p.status, KID_GROUPED_GRAD};
+    const uint32_t cta_rank = CG == 1 ? 0u : cluster_cta_rank();
+    const bool leader = cta_rank == 0;
+    const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&ctl->full[s], 1);
             mbar_init(&ctl->empty[s], 1);
+            mbar_init(&ctl->ragged[s], 1);
+            mbar_init(&ctl->partner[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&ctl->tmem_full[b], 1);
-            mbar_init(&ctl->tmem_empty[b], 128);
+            mbar_init(&ctl->tmem_empty[b], EPILOGUE_WARPS * 32 * CG);
         }
         ctl->abort_flag = 0;
         mbar_fence_init();
         tma_prefetch_desc(&map_a);
         tma_prefetch_desc(&map_b);
+        tma_prefetch_desc(&map_out);
     }
     if (warp == 1) {
-        tmem_alloc<1>(&ctl->tmem_base, TMEM_COLS);
-        tmem_relinquish<1>();
+        tmem_alloc<CG>(&ctl->tmem_base, TMEM_COLS);
+        tmem_relinquish<CG>();
     }
     build_starts(p.offsets, p.rows, starts);
     tcgen05_fence_before_sync();
     __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
     tcgen05_fence_after_sync();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
-    const int per_run = p.m_tiles * p.n_tiles;
-    const int total = p.offsets.runs * per_run;
+    const int total = p.offsets.runs * p.m_tiles * p.n_tiles;
 
-    if (warp == 0) {
-        // ------------------------------ TMA producer ------------------------------
-        if (lane == 0) {
-            uint32_t it = 0;
-            for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
-                const int run = tile / per_run, inside = tile - run * per_run;
-                const int m0 = inside % p.m_tiles * BM, n0 = inside / p.m_tiles * BN;
-                const int begin = starts[run], blocks = (starts[run + 1] - begin + BK - 1) / BK;
-                for (int kb = 0; kb < blocks; ++kb, ++it) {
-                    const int s = it % STAGES;
-                    mbar_wait(&ctl->empty[s], ((it / STAGES) & 1) ^ 1, wait_ctx, 0x100 | s);
-                    uint8_t *dst = smem + s * S::STAGE_BYTES;
-                    mbar_expect_tx(&ctl->full[s], S::STAGE_BYTES);
+    // The copies of one operand, COLS columns of it a CTA.  (The tensor map has to be known here: chosen at run time, its
+    // address is no constant, and a copy costs several times as much to issue.)
+    const auto produce = [&](const CUtensorMap &map, auto cols, auto of_lhs) {
+        constexpr int COLS = decltype(cols)::value;
+        constexpr bool LHS = decltype(of_lhs)::value;
+        const bool issuer = elect_one();
+        uint32_t s = 0, phase = 1;
+        for (int tile = worker; tile < total; tile += workers) {
+            const GradTile at = grad_tile(p, starts, tile, S::TILE_M, BN);
+            const int col0 = (LHS ? at.m0 : at.n0) + static_cast<int>(cta_rank) * COLS;
+            for (int k0 = 0; k0 < at.length; k0 += BK) {
+                mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x100 | s);
+                uint8_t *dst = smem + s * S::STAGE_BYTES + (LHS ? 0 : A_STAGE_BYTES);
+                const bool ragged = at.length - k0 < BK && (at.length & (UMMA_K - 1)) != 0;
+                if (issuer) {
+                    if (ragged) {
+                        if (LHS) mbar_expect_tx(&ctl->ragged[s], S::STAGE_BYTES);
 #pragma unroll
-                    for (int j = 0; j < BM / 64; ++j)
-                        tma_load_2d(dst + j * BOX_BYTES, &map_a, &ctl->full[s], m0 + j * 64, begin + kb * BK);
+                        for (int j = 0; j < COLS / 64; ++j)
+                            tma_load_2d(dst + j * S::BOX_BYTES, &map, &ctl->ragged[s], col0 + j * 64, at.begin + k0);
+                    } else {
+                        if (LHS && leader) mbar_expect_tx(&ctl->full[s], S::STAGE_BYTES * CG);
 #pragma unroll
-                    for (int j = 0; j < BN / 64; ++j)
-                        tma_load_2d(dst + A_STAGE_BYTES + j * BOX_BYTES, &map_b, &ctl->full[s], n0 + j * 64, begin + kb * BK);
+                        for (int j = 0; j < COLS / 64; ++j)
+                            load_2d<CG>(dst + j * S::BOX_BYTES, &map, &ctl->full[s], col0 + j * 64, at.begin + k0);
+                    }
+                }
+                if (++s == STAGES) {
+                    s = 0;
+                    phase ^= 1;
                 }
             }
         }
+    };
+
+    if (warp == 0) {
+        produce(map_a, std::integral_constant<int, BM>(), std::true_type());
+    } else if (warp == ROW_WARP) {
+        produce(map_b, std::integral_constant<int, S::BN_CTA>(), std::false_type());
     } else if (warp == 1) {
         // ------------------------------- MMA issuer -------------------------------
-        const uint32_t idesc = umma_instr_desc(BM, BN, p.bf16 != 0, true, true);
+        const uint32_t idesc = umma_instr_desc(BM * CG, BN, p.bf16 != 0, true, true);
         const bool issuer = elect_one();
         const uint32_t smem_base = smem_u32(smem);
         uint32_t s = 0, phase = 0, acc_it = 0;
         bool ready = false;
-        for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
-            const int run = tile / per_run;
-            const int length = starts[run + 1] - starts[run];
+        for (int tile = leader ? worker : total; tile < total; tile += workers) {
+            const int length = grad_tile(p, starts, tile, S::TILE_M, BN).length;
             if (length == 0) continue;  // (the epilogue stores zeros by itself)
             const int blocks = (length + BK - 1) / BK;
             const uint32_t buf = acc_it & 1;
-            mbar_wait(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+            mbar_wait_warp(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+            ++acc_it;
             tcgen05_fence_after_sync();
             const uint32_t tmem_acc = tmem_base + buf * BN;
             for (int kb = 0; kb < blocks; ++kb) {
-                if (!ready) mbar_wait(&ctl->full[s], phase, wait_ctx, 0x300 | s);
+                if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x300 | s);
                 tcgen05_fence_after_sync();
+                const int left = length - kb * BK;
+                const int steps = left >= BK ? BK / UMMA_K : (left + UMMA_K - 1) / UMMA_K;
                 const uint32_t a_addr = smem_base + s * S::STAGE_BYTES;
                 const uint32_t b_addr = a_addr + A_STAGE_BYTES;
                 const uint32_t s_next = s + 1 == STAGES ? 0 : s + 1;
                 const uint32_t phase_next = s_next == 0 ? phase ^ 1 : phase;
-                const int left = length - kb * BK;
-                const int steps = left >= BK ? BK / UMMA_K : (left + UMMA_K - 1) / UMMA_K;
-                if (left < BK && left % UMMA_K != 0) {
-                    const int first = left, chunks = (steps * UMMA_K - first) * 8;  // 16-byte chunks of a box
-                    uint8_t *stage = smem + s * S::STAGE_BYTES + first * 128;
-                    for (int i = lane; i < chunks; i += 32)
-#pragma unroll
-                        for (int b = 0; b < BOXES; ++b)
-                            *reinterpret_cast<uint4 *>(stage + b * BOX_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                }
 #pragma unroll
                 for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-                    const uint64_t desc_a = umma_smem_desc(a_addr + kk * (UMMA_K * 128), BOX_BYTES, 1024);
-                    const uint64_t desc_b = umma_smem_desc(b_addr + kk * (UMMA_K * 128), BOX_BYTES, 1024);
-                    if (issuer && kk < steps) umma_ss<1>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
+                    const uint64_t desc_a = umma_smem_desc(a_addr + kk * (UMMA_K * 128), S::BOX_BYTES, 1024);
+                    const uint64_t desc_b = umma_smem_desc(b_addr + kk * (UMMA_K * 128), S::BOX_BYTES, 1024);
+                    if (issuer && kk < steps) umma_ss<CG>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
                     if (kk == BK / UMMA_K / 2 - 1)
                         ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
                 }
-                if (issuer) umma_commit<1>(&ctl->empty[s]);
+                if (issuer) {
+                    if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
+                    else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
+                }
                 s = s_next;
                 phase = phase_next;
             }
-            if (issuer) umma_commit<1>(&ctl->tmem_full[buf]);
+            if (issuer) {
+                if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
+                else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
+            }
             __syncwarp();
-            ++acc_it;
+        }
+    } else if (warp == ROW_WARP + 1) {
+        // --------------- the rows behind a run in its last block ---------------
+        uint32_t it = 0, phases = 0;  // blocks so far; a phase bit a stage (not every use of a stage is ragged)
+        for (int tile = worker; tile < total; tile += workers) {
+            const int length = grad_tile(p, starts, tile, S::TILE_M, BN).length;
+            it += (length + BK - 1) / BK;
+            if ((length & (UMMA_K - 1)) == 0) continue;
+            const uint32_t s = (it - 1) % STAGES, phase = (phases >> s) & 1;
+            phases ^= 1u << s;
+            mbar_wait_warp(&ctl->ragged[s], phase, wait_ctx, 0x600 | s);
+            const int first = length & (BK - 1), chunks = (UMMA_K - (length & (UMMA_K - 1))) * 8;  // 16-byte chunks of a box
+            uint8_t *rows = smem + s * S::STAGE_BYTES + first * 128;
+            for (int i = lane; i < chunks; i += 32)
+#pragma unroll
+                for (int b = 0; b < (BM + S::BN_CTA) / 64; ++b)
+                    *reinterpret_cast<uint4 *>(rows + b * S::BOX_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (leader) {
+                    if constexpr (CG == 2) {
+                        mbar_wait_cluster(&ctl->partner[s], phase, wait_ctx, 0x700 | s);
+                        fence_cluster();
+                    }
+                    mbar_arrive(&ctl->full[s]);
+                } else {
+                    mbar_arrive_cluster(&ctl->partner[s], 0);
+                }
+            }
+            __syncwarp();
         }
     } else {
         // -------------------------------- epilogue --------------------------------
-        const int quadrant = warp & 3;
-        const bool bf16 = p.bf16 != 0, vec = p.out_vec != 0;
+        const int quadrant = warp & 3, half = (warp - 2) / 4;
+        const bool bf16 = p.bf16 != 0;
+        uint8_t *const box = boxes + (warp - 2) * (32 * 128);
         uint32_t acc_it = 0;
-        for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
-            const int run = tile / per_run, inside = tile - run * per_run;
-            const int row = inside % p.m_tiles * BM + quadrant * 32 + lane, n0 = inside / p.m_tiles * BN;
-            const bool empty = starts[run + 1] == starts[run];
-            const int64_t row_at = run * p.out_batch_stride + row * p.out_stride0;
+        for (int tile = worker; tile < total; tile += workers) {
+            const GradTile at = grad_tile(p, starts, tile, S::TILE_M, BN);
+            const int row0 = at.m0 + static_cast<int>(cta_rank) * BM + quadrant * 32, row = row0 + lane;
+            const bool empty = at.length == 0;
             const uint32_t buf = acc_it & 1;
             const uint32_t taddr = tmem_base + buf * BN + (static_cast<uint32_t>(quadrant * 32) << 16);
             if (!empty) {
@@ -1447,29 +1534,57 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 tcgen05_fence_after_sync();
             }
 #pragma unroll 1
-            for (int col = 0; col < BN && n0 + col < p.n; col += 32) {
-                uint32_t acc[32] = {};
+            for (int col = 64 * half; col < BN && at.n0 + col < p.n && row0 < p.m; col += 128) {
+                uint32_t acc[2][32] = {};
                 __syncwarp();
                 if (!empty) {
-                    tmem_ld_32x32(taddr + col, acc);
+                    tmem_ld_32x32(taddr + col, acc[0]);
+                    tmem_ld_32x32(taddr + col + 32, acc[1]);
                     tmem_wait_ld();
                 }
-                if (row < p.m) store_columns(acc, p.out, row_at, p.out_stride1, n0 + col, p.n, vec, bf16);
+                if (p.out_vec) {
+                    // a box in the 128-byte swizzle; its store clips rows and columns outside the gradient
+                    if (lane == 0) tma_store_wait_read<0>();
+                    __syncwarp();
+#pragma unroll
+                    for (int v = 0; v < 8; ++v) {
+                        const uint32_t(&c)[32] = acc[v / 4];
+                        uint4 packed;
+                        packed.x = pack2(__uint_as_float(c[v % 4 * 8 + 0]), __uint_as_float(c[v % 4 * 8 + 1]), bf16);
+                        packed.y = pack2(__uint_as_float(c[v % 4 * 8 + 2]), __uint_as_float(c[v % 4 * 8 + 3]), bf16);
+                        packed.z = pack2(__uint_as_float(c[v % 4 * 8 + 4]), __uint_as_float(c[v % 4 * 8 + 5]), bf16);
+                        packed.w = pack2(__uint_as_float(c[v % 4 * 8 + 6]), __uint_as_float(c[v % 4 * 8 + 7]), bf16);
+                        *reinterpret_cast<uint4 *>(box + lane * 128 + ((v ^ (lane & 7)) << 4)) = packed;
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_3d(&map_out, box, at.n0 + col, row0, at.run);
+                        tma_store_commit();
+                    }
+                } else if (row < p.m) {
+                    const int64_t row_at = at.run * p.out_batch_stride + row * p.out_stride0;
+                    store_columns(acc[0], p.out, row_at, p.out_stride1, at.n0 + col, p.n, false, bf16);
+                    store_columns(acc[1], p.out, row_at, p.out_stride1, at.n0 + col + 32, p.n, false, bf16);
+                }
             }
             if (!empty) {
                 tcgen05_fence_before_sync();
-                mbar_arrive(&ctl->tmem_empty[buf]);
+                if (CG == 1 || leader) mbar_arrive(&ctl->tmem_empty[buf]);
+                else mbar_arrive_cluster(&ctl->tmem_empty[buf], 0);
                 ++acc_it;
             }
         }
+        if (lane == 0) tma_store_wait<0>();
     }
 
     __syncwarp();
     tcgen05_fence_before_sync();
     __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
     if (warp == 1) {
         tcgen05_fence_after_sync();
-        tmem_dealloc<1>(tmem_base, TMEM_COLS);
+        tmem_dealloc<CG>(tmem_base, TMEM_COLS);
     }
 }
 
@@ -1813,9 +1928,9 @@ dim3 plain_grid(int64_t rows, int64_t cols, int64_t runs = 1) {
                 static_cast<unsigned>(std::min<int64_t>((cols + 31) / 32, 65535)), static_cast<unsigned>(runs));
 }
 
-bool output_vec(const NineToothedTensor &t, int row_dim) {
-    return t.strides[row_dim + 1] == 1 && (t.shape[row_dim] <= 1 || t.strides[row_dim] % 8 == 0) && aligned16(t.data) &&
-           (row_dim == 0 || t.shape[0] <= 1 || t.strides[0] % 8 == 0);
+// Rows of output take 16-byte stores.
+bool output_vec(const NineToothedTensor &t) {
+    return t.strides[1] == 1 && (t.shape[0] <= 1 || t.strides[0] % 8 == 0) && aligned16(t.data);
 }
 
 int run_grouped(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothedTensor &rhs,
@@ -1847,7 +1962,7 @@ int run_grouped(cudaStream_t stream, const NineToothedTensor &lhs, const NineToo
     p.out = output.data;
     p.out_stride0 = output.strides[0];
     p.out_stride1 = output.strides[1];
-    p.out_vec = output_vec(output, 0);
+    p.out_vec = output_vec(output);
     p.status = dev->status;
     const Matrices matrices{rhs.data, runs, k, n, rhs.strides[0], rhs.strides[1], rhs.strides[2]};
     if (rows_addressable(lhs.data, rows, k, lhs.strides[0], lhs.strides[1]) && matrices.addressable()) {
@@ -1864,21 +1979,46 @@ int run_grouped(cudaStream_t stream, const NineToothedTensor &lhs, const NineToo
     return 0;
 }
 
-template <int BN>
-int launch_grad(cudaStream_t stream, const DeviceState &dev, const CUtensorMap &map_a, const CUtensorMap &map_b, GradParams &p) {
-    auto kernel = grouped_grad_kernel<BN>;
-    const size_t smem = grad_smem_bytes<BN>(p.offsets.runs);
+template <int CG, int BN>
+int launch_grad(cudaStream_t stream, const DeviceState &dev, int dtype, const NineToothedTensor &lhs, const NineToothedTensor &grad,
+                const NineToothedTensor &rhs_grad, GradParams &p) {
+    auto kernel = grad_kernel<CG, BN>;
+    static_assert(grad_smem<CG, BN>(MAX_RUNS) <= MAX_SMEM, "shared memory per CTA");
     static thread_local int configured_device = -1;
+    static thread_local int pairs = 0;
     if (configured_device != dev.device) {
         NT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SMEM)));
+        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, MAX_SMEM, GRAD_THREADS);
         configured_device = dev.device;
     }
-    p.m_tiles = (p.m + BM - 1) / BM;
+    using S = Grad<CG, BN>;
+    p.m_tiles = (p.m + S::TILE_M - 1) / S::TILE_M;
     p.n_tiles = (p.n + BN - 1) / BN;
     const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.offsets.runs;
+    const int64_t workers = std::min<int64_t>(tiles, CG == 2 ? pairs : dev.sm_count);
     if (tiles > INT_MAX / 2) return fail(NINETOOTHED_B200_ERR_SHAPE, "grouped_matmul_rhs_grad: too many tiles");
-    kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles, dev.sm_count)), NUM_THREADS, smem, stream>>>(map_a, map_b, p);
-    NT_CUDA_CHECK(cudaGetLastError());
+    if (workers <= 0) return fail(NINETOOTHED_B200_ERR_DEVICE, "grouped_matmul_rhs_grad: no CTA pair fits this device");
+    CUtensorMap map_a, map_b, map_out;
+    if (int rc = map_rows(dev, &map_a, dtype, lhs.data, p.rows, p.m, lhs.strides[0], 64, BK)) return rc;
+    if (int rc = map_rows(dev, &map_b, dtype, grad.data, p.rows, p.n, grad.strides[0], 64, BK)) return rc;
+    map_out = map_a;
+    const Matrices out{rhs_grad.data, p.offsets.runs, p.m, p.n, rhs_grad.strides[0], rhs_grad.strides[1], rhs_grad.strides[2]};
+    p.out_vec = out.use_mn();
+    if (p.out_vec)
+        if (int rc = map_matrices(dev, &map_out, dtype, out, true, 64, 32)) return rc;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(workers * CG));
+    config.blockDim = dim3(GRAD_THREADS);
+    config.dynamicSmemBytes = grad_smem<CG, BN>(p.offsets.runs);
+    config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    if (CG == 2) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim = {2, 1, 1};
+        config.attrs = attr;
+        config.numAttrs = 1;
+    }
+    NT_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, map_a, map_b, map_out, p));
     return 0;
 }
 
@@ -1910,14 +2050,12 @@ int run_grouped_grad(cudaStream_t stream, const NineToothedTensor &lhs, const Ni
     p.out_batch_stride = rhs_grad.strides[0];
     p.out_stride0 = rhs_grad.strides[1];
     p.out_stride1 = rhs_grad.strides[2];
-    p.out_vec = output_vec(rhs_grad, 1);
     p.status = dev->status;
     if (rows > 0 && rows_addressable(lhs.data, rows, m, lhs.strides[0], lhs.strides[1]) &&
         rows_addressable(grad.data, rows, n, grad.strides[0], grad.strides[1])) {
-        CUtensorMap map_a, map_b;
-        if (int rc = map_rows(*dev, &map_a, dtype, lhs.data, rows, m, lhs.strides[0], 64, BK)) return rc;
-        if (int rc = map_rows(*dev, &map_b, dtype, grad.data, rows, n, grad.strides[0], 64, BK)) return rc;
-        return n > 128 ? launch_grad<256>(stream, *dev, map_a, map_b, p) : launch_grad<128>(stream, *dev, map_a, map_b, p);
+        const int64_t wide = runs * ((m + 255) / 256) * ((n + 255) / 256);
+        return wide * 2 >= dev->sm_count ? launch_grad<2, 256>(stream, *dev, dtype, lhs, grad, rhs_grad, p)
+                                         : launch_grad<1, 128>(stream, *dev, dtype, lhs, grad, rhs_grad, p);
     }
     if (rows > 0)
         note_plain_launch("grouped_matmul_rhs_grad %lld x %lld x %lld runs on the plain CUDA-core kernel: the tensor-core path "
@@ -1996,7 +2134,7 @@ int run_lora(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothe
             p.out = output.data;
             p.out_stride0 = output.strides[0];
             p.out_stride1 = output.strides[1];
-            p.out_vec = output_vec(output, 0);
+            p.out_vec = output_vec(output);
             return launch_few(stream, *dev, dtype, p, lhs.data, lhs.strides[0], shared, first, second, static_cast<float *>(workspace));
         }
         Maps maps;
@@ -2015,7 +2153,7 @@ int run_lora(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothe
         p.out = output.data;
         p.out_stride0 = output.strides[0];
         p.out_stride1 = output.strides[1];
-        p.out_vec = output_vec(output, 0);
+        p.out_vec = output_vec(output);
         return launch_product<LORA>(stream, *dev, dtype, maps, p, lhs.data, lhs.strides[0], shared, any ? &second : nullptr, 1);
     }
     note_plain_launch("lora_matmul %lld x %lld x %lld, rank %lld, runs on the plain CUDA-core kernels: the tensor-core path needs "
