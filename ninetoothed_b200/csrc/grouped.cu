@@ -62,7 +62,7 @@ struct Control {
     uint64_t tmem_empty[2];
     uint64_t partials;
     uint64_t ragged[MAX_STAGES];
-    uint64_t partner[MAX_STAGES];
+    uint64_t clean[MAX_STAGES];
     int tile_rows[MAX_STAGES];  // rows of the tiles whose stages are in the ring
     uint32_t tmem_base;
     uint32_t abort_flag;
@@ -761,6 +761,8 @@ __device__ __forceinline__ int split_share(int rows, int split) { return ((rows 
 
 // Bounded wait for arrivals that come from other CTAs of the cluster with data they have written here.
 __device__ __forceinline__ void mbar_wait_cluster(uint64_t *bar, uint32_t parity, const WaitCtx &ctx, uint32_t code) {
+    for (int i = 0; i < 256; ++i)
+        if (mbar_test_wait_cluster(bar, parity)) return;
     const uint64_t start = global_timer_ns();
     while (!mbar_test_wait_cluster(bar, parity)) {
         const bool failed_before = *ctx.abort_flag != 0;
@@ -1318,8 +1320,10 @@ __device__ __forceinline__ void build_starts(const Offsets &offsets, int rows, i
 // warp 10 copies output_grad.
 //
 // In a pair the even CTA's barriers count both CTAs' copies, but each CTA has to overwrite its own rows: a ragged block is
-// therefore copied against a barrier of its own in each CTA, whose warp 11 overwrites the rows, ahead of the issuer like the
-// copies; the odd CTA's then tells the even CTA's, and that the issuer.
+// therefore copied against a barrier of its own in each CTA (`ragged`), whose warp 11 overwrites the rows, ahead of the
+// issuer like the copies, and arrives at the barrier that the issuer waits for (`clean`, in the even CTA).
+constexpr int OUT_BOX_BYTES = 32 * 64;  // 32 rows of 32 columns; two an epilogue warp, so that filling one hides the other's store
+
 template <int CG, int BN>
 struct Grad {
     static constexpr int BN_CTA = BN / CG;
@@ -1327,7 +1331,7 @@ struct Grad {
     static constexpr int STAGES = 5;
     static constexpr int TILE_M = BM * CG;
     static constexpr int BOX_BYTES = BK * 128;  // 64 rows of 64 columns
-    static constexpr int OUT_BYTES = EPILOGUE_WARPS * 32 * 128;  // a box of 32 rows of 64 columns for every epilogue warp
+    static constexpr int OUT_BYTES = EPILOGUE_WARPS * 2 * OUT_BOX_BYTES;
 };
 
 template <int CG, int BN>
@@ -1346,11 +1350,6 @@ __device__ __forceinline__ GradTile grad_tile(const GradParams &p, const int *st
     const int run = tile / per_run, inside = tile - run * per_run;
     const int n = inside / p.m_tiles;
     return {run, (inside - n * p.m_tiles) * tile_m, n * tile_n, starts[run + 1] - starts[run], starts[run]};
-}
-
-__device__ __forceinline__ void fence_cluster() {
-    asm volatile("fence.acq_rel.cluster;" ::: "memory");
-    asm volatile("fence.proxy.async;" ::: "memory");
 }
 
 template <int CG, int BN>
@@ -1377,7 +1376,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
             mbar_init(&ctl->full[s], 1);
             mbar_init(&ctl->empty[s], 1);
             mbar_init(&ctl->ragged[s], 1);
-            mbar_init(&ctl->partner[s], 1);
+            mbar_init(&ctl->clean[s], CG);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&ctl->tmem_full[b], 1);
@@ -1417,7 +1416,10 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
                 const bool ragged = at.length - k0 < BK && (at.length & (UMMA_K - 1)) != 0;
                 if (issuer) {
                     if (ragged) {
-                        if (LHS) mbar_expect_tx(&ctl->ragged[s], S::STAGE_BYTES);
+                        if (LHS) {
+                            mbar_expect_tx(&ctl->ragged[s], S::STAGE_BYTES);
+                            if (leader) mbar_arrive(&ctl->full[s]);  // (keeps its phases in step; the issuer waits for `clean` too)
+                        }
 #pragma unroll
                         for (int j = 0; j < COLS / 64; ++j)
                             tma_load_2d(dst + j * S::BOX_BYTES, &map, &ctl->ragged[s], col0 + j * 64, at.begin + k0);
@@ -1445,7 +1447,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
         const uint32_t idesc = umma_instr_desc(BM * CG, BN, p.bf16 != 0, true, true);
         const bool issuer = elect_one();
         const uint32_t smem_base = smem_u32(smem);
-        uint32_t s = 0, phase = 0, acc_it = 0;
+        uint32_t s = 0, phase = 0, acc_it = 0, clean_phases = 0;  // (a bit a stage: not every use of a stage is ragged)
         bool ready = false;
         for (int tile = leader ? worker : total; tile < total; tile += workers) {
             const int length = grad_tile(p, starts, tile, S::TILE_M, BN).length;
@@ -1458,8 +1460,13 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
             const uint32_t tmem_acc = tmem_base + buf * BN;
             for (int kb = 0; kb < blocks; ++kb) {
                 if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x300 | s);
-                tcgen05_fence_after_sync();
                 const int left = length - kb * BK;
+                if (left < BK && (left & (UMMA_K - 1)) != 0) {
+                    if (lane == 0) mbar_wait_cluster(&ctl->clean[s], (clean_phases >> s) & 1, wait_ctx, 0x700 | s);
+                    __syncwarp();
+                    clean_phases ^= 1u << s;
+                }
+                tcgen05_fence_after_sync();
                 const int steps = left >= BK ? BK / UMMA_K : (left + UMMA_K - 1) / UMMA_K;
                 const uint32_t a_addr = smem_base + s * S::STAGE_BYTES;
                 const uint32_t b_addr = a_addr + A_STAGE_BYTES;
@@ -1505,15 +1512,8 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-                if (leader) {
-                    if constexpr (CG == 2) {
-                        mbar_wait_cluster(&ctl->partner[s], phase, wait_ctx, 0x700 | s);
-                        fence_cluster();
-                    }
-                    mbar_arrive(&ctl->full[s]);
-                } else {
-                    mbar_arrive_cluster(&ctl->partner[s], 0);
-                }
+                if (leader) mbar_arrive(&ctl->clean[s]);
+                else mbar_arrive_cluster(&ctl->clean[s], 0);
             }
             __syncwarp();
         }
@@ -1521,7 +1521,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
         // -------------------------------- epilogue --------------------------------
         const int quadrant = warp & 3, half = (warp - 2) / 4;
         const bool bf16 = p.bf16 != 0;
-        uint8_t *const box = boxes + (warp - 2) * (32 * 128);
+        uint32_t box_it = 0;
         uint32_t acc_it = 0;
         for (int tile = worker; tile < total; tile += workers) {
             const GradTile at = grad_tile(p, starts, tile, S::TILE_M, BN);
@@ -1534,27 +1534,26 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
                 tcgen05_fence_after_sync();
             }
 #pragma unroll 1
-            for (int col = 64 * half; col < BN && at.n0 + col < p.n && row0 < p.m; col += 128) {
-                uint32_t acc[2][32] = {};
+            for (int col = 32 * half; col < BN && at.n0 + col < p.n && row0 < p.m; col += 64) {
+                uint32_t acc[32] = {};
                 __syncwarp();
                 if (!empty) {
-                    tmem_ld_32x32(taddr + col, acc[0]);
-                    tmem_ld_32x32(taddr + col + 32, acc[1]);
+                    tmem_ld_32x32(taddr + col, acc);
                     tmem_wait_ld();
                 }
                 if (p.out_vec) {
-                    // a box in the 128-byte swizzle; its store clips rows and columns outside the gradient
-                    if (lane == 0) tma_store_wait_read<0>();
+                    // a box in the 64-byte swizzle; its store clips rows and columns outside the gradient
+                    uint8_t *const box = boxes + ((warp - 2) * 2 + (box_it++ & 1)) * OUT_BOX_BYTES;
+                    if (lane == 0) tma_store_wait_read<1>();  // the box of two steps ago has been read
                     __syncwarp();
 #pragma unroll
-                    for (int v = 0; v < 8; ++v) {
-                        const uint32_t(&c)[32] = acc[v / 4];
+                    for (int v = 0; v < 4; ++v) {
                         uint4 packed;
-                        packed.x = pack2(__uint_as_float(c[v % 4 * 8 + 0]), __uint_as_float(c[v % 4 * 8 + 1]), bf16);
-                        packed.y = pack2(__uint_as_float(c[v % 4 * 8 + 2]), __uint_as_float(c[v % 4 * 8 + 3]), bf16);
-                        packed.z = pack2(__uint_as_float(c[v % 4 * 8 + 4]), __uint_as_float(c[v % 4 * 8 + 5]), bf16);
-                        packed.w = pack2(__uint_as_float(c[v % 4 * 8 + 6]), __uint_as_float(c[v % 4 * 8 + 7]), bf16);
-                        *reinterpret_cast<uint4 *>(box + lane * 128 + ((v ^ (lane & 7)) << 4)) = packed;
+                        packed.x = pack2(__uint_as_float(acc[v * 8 + 0]), __uint_as_float(acc[v * 8 + 1]), bf16);
+                        packed.y = pack2(__uint_as_float(acc[v * 8 + 2]), __uint_as_float(acc[v * 8 + 3]), bf16);
+                        packed.z = pack2(__uint_as_float(acc[v * 8 + 4]), __uint_as_float(acc[v * 8 + 5]), bf16);
+                        packed.w = pack2(__uint_as_float(acc[v * 8 + 6]), __uint_as_float(acc[v * 8 + 7]), bf16);
+                        *reinterpret_cast<uint4 *>(box + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4)) = packed;
                     }
                     fence_proxy_async_smem();
                     __syncwarp();
@@ -1563,9 +1562,8 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
                         tma_store_commit();
                     }
                 } else if (row < p.m) {
-                    const int64_t row_at = at.run * p.out_batch_stride + row * p.out_stride0;
-                    store_columns(acc[0], p.out, row_at, p.out_stride1, at.n0 + col, p.n, false, bf16);
-                    store_columns(acc[1], p.out, row_at, p.out_stride1, at.n0 + col + 32, p.n, false, bf16);
+                    store_columns(acc, p.out, at.run * p.out_batch_stride + row * p.out_stride0, p.out_stride1, at.n0 + col, p.n, false,
+                                  bf16);
                 }
             }
             if (!empty) {
@@ -1696,6 +1694,22 @@ int map_matrices(const DeviceState &dev, CUtensorMap *map, int dtype, const Matr
     const uint64_t strides[2] = {static_cast<uint64_t>(pitch) * 2, static_cast<uint64_t>(batch) * 2};
     const uint32_t box[3] = {box_inner, box_outer, 1};
     return make_tensor_map(dev, map, dtype, 3, t.data, dims, strides, box, true);
+}
+
+// 32 x 32 boxes of row-major matrices, in the 64-byte swizzle (for stores).
+int map_boxes(const DeviceState &dev, CUtensorMap *map, int dtype, const Matrices &t) {
+    const int64_t pitch = row_pitch(t.rows, t.cols, t.stride1), batch = t.count <= 1 ? pitch * t.rows : t.stride0;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(t.cols), static_cast<cuuint64_t>(t.rows), static_cast<cuuint64_t>(t.count)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch) * 2, static_cast<cuuint64_t>(batch) * 2};
+    const cuuint32_t box[3] = {32, 32, 1}, ones[3] = {1, 1, 1};
+    const CUresult rc = dev.encode_tiled(
+        map, dtype == NINETOOTHED_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+        const_cast<void *>(t.data), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS)
+        return fail(NINETOOTHED_B200_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the output (CUresult %d): base %p dims [%lld %lld %lld]",
+                    static_cast<int>(rc), t.data, (long long)t.cols, (long long)t.rows, (long long)t.count);
+    return 0;
 }
 
 template <typename Kernel>
@@ -2005,7 +2019,7 @@ int launch_grad(cudaStream_t stream, const DeviceState &dev, int dtype, const Ni
     const Matrices out{rhs_grad.data, p.offsets.runs, p.m, p.n, rhs_grad.strides[0], rhs_grad.strides[1], rhs_grad.strides[2]};
     p.out_vec = out.use_mn();
     if (p.out_vec)
-        if (int rc = map_matrices(dev, &map_out, dtype, out, true, 64, 32)) return rc;
+        if (int rc = map_boxes(dev, &map_out, dtype, out)) return rc;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(workers * CG));
     config.blockDim = dim3(GRAD_THREADS);
