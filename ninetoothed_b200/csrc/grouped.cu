@@ -35,16 +35,13 @@ constexpr int MAX_STAGES = 8;
 constexpr int GROUP_ROWS = 16;  // tile-rows of 128 that share a raster group (L2 reuse of a run's weight panels)
 constexpr int MAX_RUNS = 2048;  // the table of runs is 16 bytes a run of shared memory
 constexpr int SPLIT_NT = 64;     // rows of a tile whose reduction a cluster shares
-constexpr int FEW_ROWS = 256;
+constexpr int FEW_ROWS = 1024;   // rows of a call whose adapters' part may be computed a row at a time (see few_rows)
 constexpr int FEW_RANK = 128;    // largest rank whose second product the epilogue of a few-row call computes
 constexpr int LOW_WARPS = 8;
 constexpr int LOW_CHUNK = LOW_WARPS * 256;  // terms of a partial sum of (lhs . down) there
-constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product: 32 high parts, 32 low parts
+enum Job { JOB_PRODUCT, JOB_PARTS, JOB_FEW };
 
-enum Mode {
-    SHRINK,  // tiles of every run that has an adapter, its matrix; the result is kept as two 16-bit parts
-    LORA,    // tiles over all rows with one matrix; each run's second product is added into its own rows
-};
+constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product: 32 high parts, 32 low parts
 
 template <int CG, int BN>
 struct Shape {
@@ -190,13 +187,21 @@ __device__ __forceinline__ void build_table(const Params &p, Run *table, Control
 }
 
 // The run that holds `row`, or -1: the one before the first bound above it (a bound above `row` that comes first ends
-// the run by the running maximum too).  The lanes of a warp look at 32 bounds at a time.
+// the run by the running maximum too).  A warp looks at 256 bounds at a time, for one memory latency.
 __device__ __forceinline__ int run_of(const Offsets &o, int rows, int row) {
     const int lane = threadIdx.x & 31;
-    for (int base = 0; base <= o.runs; base += 32) {
-        const bool above = base + lane <= o.runs && load_index(o.data, o.stride, o.wide, base + lane, 0, rows) > row;
-        const unsigned votes = __ballot_sync(0xffffffffu, above);
-        if (votes != 0) return base + __ffs(votes) - 2;
+    for (int base = 0; base <= o.runs; base += 256) {
+        bool above[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = base + j * 32 + lane;
+            above[j] = i <= o.runs && load_index(o.data, o.stride, o.wide, i, 0, rows) > row;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const unsigned votes = __ballot_sync(0xffffffffu, above[j]);
+            if (votes != 0) return base + j * 32 + __ffs(votes) - 2;
+        }
     }
     return -1;
 }
@@ -225,11 +230,6 @@ __device__ __forceinline__ void build_range(const Params &p, Control *ctl) {
     }
 }
 
-// Where a tile lies: its first row, the end of the rows it may write, its first column, its matrix.
-struct Place {
-    int row0, row_end, col0, matrix;
-};
-
 __device__ __forceinline__ void raster(int tile, int m_tiles, int n_tiles, int group_m, int &m, int &n) {
     if (m_tiles <= group_m) {  // one group: a division is some 100 cycles between two tiles
         n = m_tiles == 1 ? tile : tile / m_tiles;
@@ -245,46 +245,6 @@ __device__ __forceinline__ void raster(int tile, int m_tiles, int n_tiles, int g
     n = inside / height;
     if (group & 1) n = n_tiles - 1 - n;  // odd groups walk back, starting on the panels the previous one ended on
 }
-
-// The tiles of one worker in order; every warp role walks its own copy.
-template <Mode MODE, int TILE_M, int BN>
-struct Walk {
-    const Run *table;
-    int tile, total, stride, runs, run;
-    int range_begin, range_end, range_tiles;
-
-    __device__ Walk(const Params &p, const Run *table_, const Control *ctl, int worker, int workers)
-        : table(table_), tile(worker), stride(workers), runs(ctl->runs), run(0) {
-        range_begin = ctl->row_begin;
-        range_end = ctl->row_end;
-        range_tiles = MODE == LORA ? (range_end - range_begin + TILE_M - 1) / TILE_M : ctl->tiles_m;
-        total = range_tiles * p.n_tiles;
-        if (MODE != LORA && tile < total) {
-            int low = 0, high = runs - 1;  // the last run whose first tile is not behind this one
-            while (low < high) {
-                const int mid = (low + high + 1) >> 1;
-                if (table[mid].tiles_before * p.n_tiles <= tile) low = mid;
-                else high = mid - 1;
-            }
-            run = low;
-        }
-    }
-    __device__ bool more() const { return tile < total; }
-    __device__ void advance() { tile += stride; }
-    __device__ Place place(const Params &p) {
-        int m, n;
-        if constexpr (MODE == LORA) {
-            raster(tile, range_tiles, p.n_tiles, p.group_m, m, n);
-            return {range_begin + m * TILE_M, range_end, n * BN, 0};
-        } else {
-            while (run + 1 < runs && table[run + 1].tiles_before * p.n_tiles <= tile) ++run;
-            const Run r = table[run];
-            const int m_tiles = (r.end - r.begin + TILE_M - 1) / TILE_M;
-            raster(tile - r.tiles_before * p.n_tiles, m_tiles, p.n_tiles, p.group_m, m, n);
-            return {r.begin + m * TILE_M, r.end, n * BN, r.matrix};
-        }
-    }
-};
 
 // First run of the table that ends behind `row`.
 __device__ __forceinline__ int first_run_behind(const Run *table, int runs, int row) {
@@ -353,23 +313,44 @@ __device__ __forceinline__ float load16(const void *in, int64_t at, bool bf16) {
                 : __half2float(static_cast<const __half *>(in)[at]);
 }
 
-// 32 columns of one output row, rounded once: 16-byte stores where the row allows them.
-__device__ __forceinline__ void store_columns(const uint32_t (&acc)[32], void *out, int64_t row_at, int64_t stride1,
-                                              int col0, int n, bool vec, bool bf16) {
+// 32 columns of 32 rows, a row a lane.  Two exchanges between lanes 1 and 2 away turn four lanes' 64-byte rows so that a
+// store's lanes write 64 neighbouring bytes of eight rows; a lane that stored its own row's 16 bytes 32 times over took
+// twice the time (128 MB of output: 41 against 71 us).
+__device__ __forceinline__ void store_rows(const uint32_t (&acc)[32], void *out, int64_t stride0, int64_t row0, int rows, int col0,
+                                           int n, bool bf16) {
+    const int lane = threadIdx.x & 31;
+    const bool odd1 = lane & 1, odd2 = lane & 2;
+    uint32_t v[4][4];  // v[i]: 16 bytes of the row
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        const int col = col0 + v * 8;
-        if (vec && col + 8 <= n) {
-            uint4 packed;
-            packed.x = pack2(__uint_as_float(acc[v * 8 + 0]), __uint_as_float(acc[v * 8 + 1]), bf16);
-            packed.y = pack2(__uint_as_float(acc[v * 8 + 2]), __uint_as_float(acc[v * 8 + 3]), bf16);
-            packed.z = pack2(__uint_as_float(acc[v * 8 + 4]), __uint_as_float(acc[v * 8 + 5]), bf16);
-            packed.w = pack2(__uint_as_float(acc[v * 8 + 6]), __uint_as_float(acc[v * 8 + 7]), bf16);
-            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out) + row_at + col) = packed;
+    for (int i = 0; i < 16; ++i) v[i / 4][i % 4] = pack2(__uint_as_float(acc[2 * i]), __uint_as_float(acc[2 * i + 1]), bf16);
+#pragma unroll
+    for (int i = 0; i < 4; i += 2)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, odd1 ? v[i][w] : v[i + 1][w], 1);
+            v[i][w] = odd1 ? other : v[i][w];
+            v[i + 1][w] = odd1 ? v[i + 1][w] : other;
+        }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, odd2 ? v[i][w] : v[i + 2][w], 2);
+            v[i][w] = odd2 ? other : v[i][w];
+            v[i + 2][w] = odd2 ? v[i + 2][w] : other;
+        }
+    const int col = col0 + (lane & 3) * 8;  // v[i] is now the lane's quarter of row i of its four lanes'
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = (lane & ~3) + i;
+        if (row >= rows || col >= n) continue;
+        uint16_t *dst = static_cast<uint16_t *>(out) + (row0 + row) * stride0 + col;
+        if (col + 8 <= n) {
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (col + j < n) store16(out, row_at + (col + j) * stride1, __uint_as_float(acc[v * 8 + j]), bf16);
+            for (int j = 0; j < 7; ++j)
+                if (col + j < n) dst[j] = static_cast<uint16_t>(v[i][j / 2] >> (16 * (j & 1)));
         }
     }
 }
@@ -394,272 +375,6 @@ template <int CG>
 __device__ __forceinline__ void load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
     if constexpr (CG == 1) tma_load_3d(dst, map, bar, x, y, z);
     else tma_load_3d_pair(dst, map, bar, x, y, z);
-}
-
-// B_MN: the matrices have unit stride along their columns; otherwise along their rows (a transposed view).
-template <int CG, int BN, bool B_MN, Mode MODE>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
-    grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_chunk,
-                   const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_low,
-                   const __grid_constant__ CUtensorMap map_up, const __grid_constant__ Params p) {
-    using S = Shape<CG, BN>;
-    constexpr int STAGES = S::STAGES;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    Control *ctl = reinterpret_cast<Control *>(smem + STAGES * S::STAGE_BYTES);
-    Run *table = reinterpret_cast<Run *>(reinterpret_cast<uint8_t *>(ctl) + CONTROL_BYTES);
-
-    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
-    const int lane = threadIdx.x & 31;
-    const WaitCtx wait_ctx{&ctl->abort_flag, p.status, KID_GROUPED};
-    const uint32_t cta_rank = CG == 1 ? 0u : cluster_cta_rank();
-    const bool leader = cta_rank == 0;
-    const int worker = blockIdx.x / CG;
-    const int workers = gridDim.x / CG;
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&ctl->full[s], 1);
-            mbar_init(&ctl->empty[s], 1);
-        }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(&ctl->tmem_full[b], 1);
-            mbar_init(&ctl->tmem_empty[b], 128 * CG);
-        }
-        ctl->abort_flag = 0;
-        mbar_fence_init();
-        tma_prefetch_desc(&map_a);
-        tma_prefetch_desc(&map_b);
-    }
-    if (warp == 1) {
-        tmem_alloc<CG>(&ctl->tmem_base, TMEM_COLS);
-        tmem_relinquish<CG>();
-    }
-    build_table(p, table, ctl, S::TILE_M);
-    tcgen05_fence_before_sync();
-    __syncthreads();
-    if constexpr (CG == 2) cluster_sync();
-    tcgen05_fence_after_sync();
-    const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
-    using W = Walk<MODE, S::TILE_M, BN>;
-
-    if (warp == 0) {
-        // ------------------------------ TMA producer ------------------------------
-        if (lane == 0) {
-            uint32_t it = 0;
-            for (W walk(p, table, ctl, worker, workers); walk.more(); walk.advance()) {
-                const Place at = walk.place(p);
-                const int m0 = at.row0 + static_cast<int>(cta_rank) * BM;
-                const int n0 = at.col0 + static_cast<int>(cta_rank) * S::BN_CTA;
-                const int boxes = a_boxes(at.row_end - m0);
-                // the even CTA's barrier counts the bytes of both
-                int bytes = boxes * (A_CHUNK_ROWS * BK * 2) + S::B_STAGE_BYTES;
-                if constexpr (CG == 2) bytes += a_boxes(at.row_end - m0 - BM) * (A_CHUNK_ROWS * BK * 2) + S::B_STAGE_BYTES;
-                for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-                    const int s = it % STAGES;
-                    mbar_wait(&ctl->empty[s], ((it / STAGES) & 1) ^ 1, wait_ctx, 0x100 | s);
-                    uint8_t *a_dst = smem + s * S::STAGE_BYTES;
-                    uint8_t *b_dst = a_dst + A_STAGE_BYTES;
-                    if (leader) mbar_expect_tx(&ctl->full[s], bytes);
-                    if (boxes == BM / A_CHUNK_ROWS) {
-                        load_2d<CG>(a_dst, &map_a, &ctl->full[s], kb * BK, m0);
-                    } else {
-                        for (int c = 0; c < boxes; ++c)
-                            load_2d<CG>(a_dst + c * (A_CHUNK_ROWS * BK * 2), &map_a_chunk, &ctl->full[s], kb * BK,
-                                        m0 + c * A_CHUNK_ROWS);
-                    }
-                    if constexpr (B_MN) {
-#pragma unroll
-                        for (int j = 0; j < S::BN_CTA / 64; ++j)
-                            load_3d<CG>(b_dst + j * (BK * 128), &map_b, &ctl->full[s], n0 + j * 64, kb * BK, at.matrix);
-                    } else {
-                        load_3d<CG>(b_dst, &map_b, &ctl->full[s], kb * BK, n0, at.matrix);
-                    }
-                }
-                if constexpr (MODE == LORA) {
-                    // the adapters' second product: for every run of the tile, the tile's rows of (scales lhs . down)
-                    // against the run's up, 32 ranks a stage
-                    const int tile_end = min(at.row_end, at.row0 + S::TILE_M);
-                    const int b_bytes = p.up_mn ? S::BN_CTA * RANK_BLOCK * 2 : S::B_STAGE_BYTES;
-                    for (int r = first_run_behind(table, walk.runs, at.row0); r < walk.runs && table[r].begin < tile_end; ++r) {
-                        const Run run = table[r];
-                        // 32-row boxes of this CTA's rows that hold rows of the run (first, last), and the partner's
-                        const auto box_range = [&](int base, int &first, int &last) {
-                            first = max(run.begin - base, 0) / A_CHUNK_ROWS;
-                            last = min((min(run.end, tile_end) - base + A_CHUNK_ROWS - 1) / A_CHUNK_ROWS, BM / A_CHUNK_ROWS);
-                            if (min(run.end, tile_end) <= base) last = 0;
-                            if (last < first) last = first;
-                        };
-                        int first, last, first_other = 0, last_other = 0;
-                        box_range(m0, first, last);
-                        if constexpr (CG == 2) box_range(at.row0 + BM, first_other, last_other);
-                        int ext_bytes = (last - first) * (A_CHUNK_ROWS * BK * 2) + b_bytes;
-                        if constexpr (CG == 2) ext_bytes += (last_other - first_other) * (A_CHUNK_ROWS * BK * 2) + b_bytes;
-                        for (int rb = 0; rb < p.rank_blocks; ++rb, ++it) {
-                            const int s = it % STAGES;
-                            mbar_wait(&ctl->empty[s], ((it / STAGES) & 1) ^ 1, wait_ctx, 0x110 | s);
-                            uint8_t *a_dst = smem + s * S::STAGE_BYTES;
-                            uint8_t *b_dst = a_dst + A_STAGE_BYTES;
-                            if (leader) mbar_expect_tx(&ctl->full[s], ext_bytes);
-                            for (int c = first; c < last; ++c)
-                                load_2d<CG>(a_dst + c * (A_CHUNK_ROWS * BK * 2), &map_low, &ctl->full[s], rb * BK,
-                                            m0 + c * A_CHUNK_ROWS);
-                            if (p.up_mn) {
-                                for (int j = 0; j < S::BN_CTA / 64; ++j)
-                                    load_3d<CG>(b_dst + j * (RANK_BLOCK * 128), &map_up, &ctl->full[s], n0 + j * 64,
-                                                rb * RANK_BLOCK, run.matrix);
-                            } else {
-                                load_3d<CG>(b_dst, &map_up, &ctl->full[s], rb * RANK_BLOCK, n0, run.matrix);
-                            }
-                        }
-                    }
-                }
-            }
-        }
-    } else if (warp == 1) {
-        // ------------------------------- MMA issuer -------------------------------
-        // The warp runs the loop as one (the instruction takes uniform registers); an elected lane issues.
-        if (leader) {
-            const uint32_t idesc = umma_instr_desc(BM * CG, BN, p.bf16 != 0, false, B_MN);
-            const bool issuer = elect_one();
-            const uint32_t smem_base = smem_u32(smem);
-            uint32_t s = 0, phase = 0, acc_it = 0;
-            bool ready = false;
-            for (W walk(p, table, ctl, worker, workers); walk.more(); walk.advance(), ++acc_it) {
-                const uint32_t buf = acc_it & 1;
-                mbar_wait(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
-                tcgen05_fence_after_sync();
-                const uint32_t tmem_acc = tmem_base + buf * BN;
-                for (int kb = 0; kb < p.k_blocks; ++kb) {
-                    if (!ready) mbar_wait(&ctl->full[s], phase, wait_ctx, 0x300 | s);
-                    tcgen05_fence_after_sync();
-                    const uint32_t a_addr = smem_base + s * S::STAGE_BYTES;
-                    const uint32_t b_addr = a_addr + A_STAGE_BYTES;
-                    const uint32_t s_next = s + 1 == STAGES ? 0 : s + 1;
-                    const uint32_t phase_next = s_next == 0 ? phase ^ 1 : phase;
-#pragma unroll
-                    for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-                        const uint64_t desc_a = umma_smem_desc(a_addr + kk * (UMMA_K * 2), 16, 1024);
-                        const uint64_t desc_b =
-                            umma_smem_desc(b_addr + kk * (B_MN ? UMMA_K * 128 : UMMA_K * 2), p.b_lbo, 1024);
-                        if (issuer) umma_ss<CG>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
-                        if (kk == BK / UMMA_K / 2 - 1)  // (a probe between MMAs costs nothing, a wait after them does)
-                            ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
-                    }
-                    if (issuer) {
-                        if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
-                        else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
-                    }
-                    s = s_next;
-                    phase = phase_next;
-                }
-                if constexpr (MODE == LORA) {
-                    const Place at = walk.place(p);
-                    const int tile_end = min(at.row_end, at.row0 + S::TILE_M);
-                    const uint32_t idesc_up = umma_instr_desc(BM * CG, BN, p.bf16 != 0, false, p.up_mn != 0);
-                    const uint32_t b_step = p.up_mn ? UMMA_K * 128 : UMMA_K * 2;
-                    const uint32_t b_lbo = p.up_mn ? RANK_BLOCK * 128 : 16;
-                    for (int r = first_run_behind(table, walk.runs, at.row0); r < walk.runs && table[r].begin < tile_end; ++r) {
-                        // Only the accumulator rows of this run take part: what another run's adapter holds, infinities
-                        // and NaN included, cannot reach them.
-                        const int low = table[r].begin - at.row0, high = min(table[r].end, tile_end) - at.row0;
-                        uint32_t off[8];
-#pragma unroll
-                        for (int w = 0; w < 8; ++w) off[w] = ~(low_bits(high - 32 * w) & ~low_bits(low - 32 * w));
-                        for (int rb = 0; rb < p.rank_blocks; ++rb) {
-                            if (!ready) mbar_wait(&ctl->full[s], phase, wait_ctx, 0x310 | s);
-                            ready = false;
-                            tcgen05_fence_after_sync();
-                            const uint32_t a_addr = smem_base + s * S::STAGE_BYTES;
-                            const uint32_t b_addr = a_addr + A_STAGE_BYTES;
-                            const int steps = (min(RANK_BLOCK, p.rank - rb * RANK_BLOCK) + UMMA_K - 1) / UMMA_K;
-                            for (int kk = 0; kk < steps; ++kk) {
-                                const uint64_t desc_b = umma_smem_desc(b_addr + kk * b_step, b_lbo, 1024);
-#pragma unroll
-                                for (int part = 0; part < 2; ++part) {
-                                    const uint64_t desc_a =
-                                        umma_smem_desc(a_addr + part * (RANK_BLOCK * 2) + kk * (UMMA_K * 2), 16, 1024);
-                                    if (issuer) umma_ss_lanes<CG>(tmem_acc, desc_a, desc_b, idesc_up, off);
-                                }
-                            }
-                            if (issuer) {
-                                if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
-                                else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
-                            }
-                            s = s + 1 == STAGES ? 0 : s + 1;
-                            if (s == 0) phase ^= 1;
-                        }
-                    }
-                }
-                if (issuer) {
-                    if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
-                    else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
-                }
-                __syncwarp();
-            }
-        }
-    } else {
-        // -------------------------------- epilogue --------------------------------
-        const int quadrant = warp & 3;
-        const int row_in_tile = static_cast<int>(cta_rank) * BM + quadrant * 32 + lane;
-        const bool bf16 = p.bf16 != 0, vec = p.out_vec != 0;
-        uint32_t acc_it = 0;
-        for (W walk(p, table, ctl, worker, workers); walk.more(); walk.advance(), ++acc_it) {
-            const Place at = walk.place(p);
-            const int row = at.row0 + row_in_tile;
-            const uint32_t buf = acc_it & 1;
-            float scale = 1.f;
-            if constexpr (MODE == SHRINK) scale = p.scales[at.matrix * p.scales_stride];
-            mbar_wait(&ctl->tmem_full[buf], (acc_it >> 1) & 1, wait_ctx, 0x400 | buf);
-            tcgen05_fence_after_sync();
-            const uint32_t taddr = tmem_base + buf * BN + (static_cast<uint32_t>(quadrant * 32) << 16);
-            const int64_t row_at = row * p.out_stride0;
-#pragma unroll 1
-            for (int col = 0; col < BN && at.col0 + col < p.n; col += 32) {
-                uint32_t acc[32];
-                __syncwarp();
-                tmem_ld_32x32(taddr + col, acc);
-                tmem_wait_ld();
-                if (row >= at.row_end) {
-                    // (nothing: the row belongs to the next run, or to none)
-                } else if constexpr (MODE == SHRINK) {
-                    // 32 ranks of a row: their high parts, then the low parts (value = high + low to twice the
-                    // type's precision, so that the second product runs on the tensor cores without the rounding
-                    // of one 16-bit operand).  Ranks past the last are zero: the operands' bounds filled them.
-                    uint4 high[4], low[4];
-                    uint32_t *h = reinterpret_cast<uint32_t *>(high), *l = reinterpret_cast<uint32_t *>(low);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float a = scale * __uint_as_float(acc[2 * j]), b = scale * __uint_as_float(acc[2 * j + 1]);
-                        const float ha = round16(a, bf16), hb = round16(b, bf16);
-                        h[j] = pack2(a, b, bf16);
-                        // (an infinite or NaN high part says it all; inf - inf must not turn it into NaN)
-                        l[j] = pack2(isfinite(ha) ? a - ha : 0.f, isfinite(hb) ? b - hb : 0.f, bf16);
-                    }
-                    uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + row_at + 2 * (at.col0 + col));
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        dst[v] = high[v];
-                        dst[4 + v] = low[v];
-                    }
-                } else {
-                    store_columns(acc, p.out, row_at, p.out_stride1, at.col0 + col, p.n, vec, bf16);
-                }
-            }
-            tcgen05_fence_before_sync();
-            if (CG == 1 || leader) mbar_arrive(&ctl->tmem_empty[buf]);
-            else mbar_arrive_cluster(&ctl->tmem_empty[buf], 0);
-        }
-    }
-
-    __syncwarp();
-    tcgen05_fence_before_sync();
-    __syncthreads();
-    if constexpr (CG == 2) cluster_sync();
-    if (warp == 1) {
-        tcgen05_fence_after_sync();
-        tmem_dealloc<CG>(tmem_base, TMEM_COLS);
-    }
 }
 
 // ---------------------------------------------------------------------------
@@ -698,7 +413,7 @@ constexpr int turned_stages() {
     return SPLIT ? SPLIT_STAGES : Turned<CG, NT>::STAGES;
 }
 
-constexpr int FEW_BYTES = SPLIT_NT * FEW_RANK * 4 + SPLIT_NT * 4;  // (lhs . down) and the adapter of a CTA's rows
+constexpr int FEW_BYTES = SPLIT_NT * FEW_RANK * 4;  // (lhs . down) of a CTA's rows
 
 template <int CG, int NT, bool SPLIT, bool FEW>
 constexpr size_t turned_smem(int runs) {
@@ -803,62 +518,123 @@ __device__ __forceinline__ void load_values(const uint16_t *at, int left, bool b
 
 __device__ __forceinline__ void prefetch_l2(const void *at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at)); }
 
-// scales (lhs . down) . up of the rows that this CTA stores into its own slot of the partial sums.  A warp takes a row, a
-// lane four columns of the tile.  What does not depend on the launch before (which adapter, its matrix on the way to L2)
-// is done before the wait for it.
-__device__ __forceinline__ void adapters_part(const Params &p, const TurnedPlace &at, float *partials, float *low, int *row_adapter,
-                                              int cta_rank, int split) {
+// `count` rows' second products with up (unit stride along its columns), four columns a lane: sixteen ranks of all of them
+// in flight at once.  l: the rows' (scales lhs . down).
+template <int COUNT>
+__device__ __forceinline__ void second_product(const uint16_t *const (&matrix)[COUNT], const float *const (&l)[COUNT], int64_t stride,
+                                               int rank, bool bf16, float (&sum)[COUNT][4]) {
+    for (int r0 = 0; r0 < rank; r0 += 16) {
+        uint2 v[COUNT][16];
+#pragma unroll
+        for (int c = 0; c < COUNT; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                v[c][r] = r0 + r < rank ? __ldg(reinterpret_cast<const uint2 *>(matrix[c] + (r0 + r) * stride)) : make_uint2(0, 0);
+#pragma unroll
+        for (int c = 0; c < COUNT; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float weight = r0 + r < rank ? l[c][r0 + r] : 0.f;
+                sum[c][0] = fmaf(weight, half_of(v[c][r].x, 0, bf16), sum[c][0]);
+                sum[c][1] = fmaf(weight, half_of(v[c][r].x, 1, bf16), sum[c][1]);
+                sum[c][2] = fmaf(weight, half_of(v[c][r].y, 0, bf16), sum[c][2]);
+                sum[c][3] = fmaf(weight, half_of(v[c][r].y, 1, bf16), sum[c][3]);
+            }
+    }
+}
+
+// scales (lhs . down) . up of the rows that this CTA stores into its own slot of the partial sums.  A warp takes every
+// eighth row, a lane four columns of the tile.  What does not depend on the launch before (which adapter, its matrix on the
+// way to L2) is done before the wait for it.  It is all memory latency: a step is done for all of the warp's rows at once.
+__device__ __forceinline__ void adapters_part(const Params &p, const TurnedPlace &at, float *partials, float *low, int cta_rank,
+                                              int split) {
     const int warp = static_cast<int>(threadIdx.x) / 32 - 2, lane = threadIdx.x & 31;
     const bool bf16 = p.bf16 != 0;
     const int share = split_share(at.rows, split);
     const int first = cta_rank * share, mine = min(at.rows, first + share) - first;
     const int row0 = at.row0 + first, col = at.col0 + lane * 4, left = p.n - col;
+    const int rows = mine > warp ? (mine - warp + EPILOGUE_WARPS - 1) / EPILOGUE_WARPS : 0;  // of this warp, at most eight
     const uint16_t *up = static_cast<const uint16_t *>(p.up);
-    for (int t = warp; t < mine; t += EPILOGUE_WARPS) {
-        const int adapter = adapter_of(p, row0 + t);
-        if (lane == 0) row_adapter[t] = adapter;
-        if (adapter < 0) continue;
-        const uint16_t *matrix = up + adapter * p.up_stride[0];
+    // lane i looks after the warp's i-th row, row0 + warp + 8 i
+    int run = -1, open = rows > 0 ? (1 << rows) - 1 : 0;  // rows whose run is not found yet
+    for (int base = 0; base <= p.offsets.runs && open != 0; base += 256) {
+        int bound[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = base + j * 32 + lane;
+            bound[j] = i <= p.offsets.runs ? load_index(p.offsets.data, p.offsets.stride, p.offsets.wide, i, 0, p.rows) : INT_MIN;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (base + j * 32 > p.offsets.runs || open == 0) break;
+            for (int i = 0; i < rows; ++i) {
+                if (!(open >> i & 1)) continue;
+                const unsigned votes = __ballot_sync(0xffffffffu, bound[j] > row0 + warp + EPILOGUE_WARPS * i);
+                if (votes == 0) continue;
+                open &= ~(1 << i);  // (the run before the first bound above the row: see run_of)
+                if (lane == i) run = base + j * 32 + __ffs(votes) - 2;
+            }
+        }
+    }
+    int adapter = -1;
+    float scale = 0.f;
+    if (lane < rows && run >= 0) {
+        adapter = load_index(p.adapters, p.adapters_stride, p.adapters_wide, run, -1, p.matrices);
+        if (adapter >= p.matrices) adapter = -1;
+        if (adapter >= 0) scale = p.scales[adapter * p.scales_stride];
+    }
+    for (int i = 0; i < rows; ++i) {
+        const int which = __shfl_sync(0xffffffffu, adapter, i);
+        if (which < 0) continue;
+        const uint16_t *matrix = up + which * p.up_stride[0];
         if (p.up_mn) {
-            for (int i = lane; i < 2 * p.rank; i += 32)
-                if (at.col0 + (i & 1) * 64 < p.n) prefetch_l2(matrix + (i / 2) * p.up_stride[1] + at.col0 + (i & 1) * 64);
+            for (int q = lane; q < 2 * p.rank; q += 32)
+                if (at.col0 + (q & 1) * 64 < p.n) prefetch_l2(matrix + (q / 2) * p.up_stride[1] + at.col0 + (q & 1) * 64);
         } else {
             for (int j = 0; j < 4 && j < left; ++j)
                 for (int r = 0; r < p.rank; r += 64) prefetch_l2(matrix + (col + j) * p.up_stride[2] + r);
         }
     }
     griddepcontrol_wait();  // (the sums of lhs . down come from the launch before)
-    for (int t = warp; t < mine; t += EPILOGUE_WARPS) {
-        __syncwarp();
-        const int adapter = row_adapter[t];
-        float sum[4] = {};
-        if (adapter >= 0) {
-            const float scale = p.scales[adapter * p.scales_stride];
-            float *l = low + t * p.rank;
-            for (int r = lane; r < p.rank; r += 32) {
-                const float *part = p.low + static_cast<int64_t>(row0 + t) * p.rank + r;
-                float total = 0.f;
 #pragma unroll 4
-                for (int c = 0; c < p.low_chunks; ++c) total += __ldcg(part + static_cast<int64_t>(c) * p.rows * p.rank);
-                l[r] = scale * total;
-            }
-            __syncwarp();
-            const uint16_t *matrix = up + adapter * p.up_stride[0];
+    for (int q = lane; q < rows * p.rank; q += 32) {
+        const int i = q / p.rank, t = warp + EPILOGUE_WARPS * i;
+        const float *part = p.low + static_cast<int64_t>(row0 + t) * p.rank + (q - i * p.rank);
+        float total = 0.f;
+        for (int c = 0; c < p.low_chunks; ++c) total += __ldcg(part + static_cast<int64_t>(c) * p.rows * p.rank);
+        low[t * p.rank + (q - i * p.rank)] = total;
+    }
+    __syncwarp();
+    const auto put = [&](int t, float factor, const float (&sum)[4]) {
+        float *dst = partials + ((cta_rank * share + t) / 4 * BM + lane * 4) * 4 + t % 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dst[j * 4] = factor * sum[j];
+    };
+    int i = 0;
+    for (; p.up_mn && i + 2 <= rows; i += 2) {
+        const int t = warp + EPILOGUE_WARPS * i;
+        const int a0 = __shfl_sync(0xffffffffu, adapter, i), a1 = __shfl_sync(0xffffffffu, adapter, i + 1);
+        const float s0 = __shfl_sync(0xffffffffu, scale, i), s1 = __shfl_sync(0xffffffffu, scale, i + 1);
+        if (a0 < 0 || a1 < 0 || p.n - at.col0 < BM) break;  // (the rest one by one)
+        float sum[2][4] = {};
+        const uint16_t *const matrix[2] = {up + a0 * p.up_stride[0] + col, up + a1 * p.up_stride[0] + col};
+        const float *const l[2] = {low + t * p.rank, low + (t + EPILOGUE_WARPS) * p.rank};
+        second_product<2>(matrix, l, p.up_stride[1], p.rank, bf16, sum);
+        put(t, s0, sum[0]);
+        put(t + EPILOGUE_WARPS, s1, sum[1]);
+    }
+    for (; i < rows; ++i) {
+        const int t = warp + EPILOGUE_WARPS * i;
+        const int which = __shfl_sync(0xffffffffu, adapter, i);
+        const float factor = __shfl_sync(0xffffffffu, scale, i);
+        float sum[1][4] = {};
+        if (which >= 0 && left > 0) {
+            const float *l = low + t * p.rank;
+            const uint16_t *matrix = up + which * p.up_stride[0];
             if (left >= 4 && p.up_mn) {
-                for (int r0 = 0; r0 < p.rank; r0 += 16) {  // sixteen loads in flight
-                    uint2 v[16];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        v[r] = r0 + r < p.rank ? __ldg(reinterpret_cast<const uint2 *>(matrix + (r0 + r) * p.up_stride[1] + col)) : make_uint2(0, 0);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float weight = r0 + r < p.rank ? l[r0 + r] : 0.f;
-                        sum[0] = fmaf(weight, half_of(v[r].x, 0, bf16), sum[0]);
-                        sum[1] = fmaf(weight, half_of(v[r].x, 1, bf16), sum[1]);
-                        sum[2] = fmaf(weight, half_of(v[r].y, 0, bf16), sum[2]);
-                        sum[3] = fmaf(weight, half_of(v[r].y, 1, bf16), sum[3]);
-                    }
-                }
+                const uint16_t *const matrices[1] = {matrix + col};
+                const float *const ls[1] = {l};
+                second_product<1>(matrices, ls, p.up_stride[1], p.rank, bf16, sum);
             } else if (left >= 4 && p.rank % 8 == 0) {  // a column's ranks lie side by side
                 for (int r0 = 0; r0 < p.rank; r0 += 32) {
                     uint4 v[4][4];
@@ -876,19 +652,18 @@ __device__ __forceinline__ void adapters_part(const Params &p, const TurnedPlace
                         for (int j = 0; j < 4; ++j) {
                             const uint32_t words[4] = {v[q][j].x, v[q][j].y, v[q][j].z, v[q][j].w};
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) sum[j] = fmaf(l[r0 + q * 8 + i], half_of(words[i / 2], i & 1, bf16), sum[j]);
+                            for (int e = 0; e < 8; ++e)
+                                sum[0][j] = fmaf(l[r0 + q * 8 + e], half_of(words[e / 2], e & 1, bf16), sum[0][j]);
                         }
                     }
                 }
             } else {
                 for (int r = 0; r < p.rank; ++r)
                     for (int j = 0; j < 4 && j < left; ++j)
-                        sum[j] = fmaf(l[r], load16(matrix, r * p.up_stride[1] + (col + j) * p.up_stride[2], bf16), sum[j]);
+                        sum[0][j] = fmaf(l[r], load16(matrix, r * p.up_stride[1] + (col + j) * p.up_stride[2], bf16), sum[0][j]);
             }
         }
-        float *dst = partials + ((cta_rank * share + t) / 4 * BM + lane * 4) * 4 + t % 4;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dst[j * 4] = sum[j];
+        put(t, factor, sum[0]);
     }
     epilogue_sync();
 }
@@ -1000,14 +775,18 @@ __device__ __forceinline__ void store_turned(const uint32_t (&acc)[32], void *ou
     }
 }
 
-// FEW: the shared projection and the adapters of a call with few rows.  The epilogue's warps, idle while the tile's
+// JOB_PARTS: a run's adapter's down is the matrix, and scales (lhs . down) leaves as two 16-bit parts, in blocks of 32 ranks:
+// 32 high parts, 32 low parts (value = high + low to twice the type's precision, so that the second product runs on the
+// tensor cores without the rounding of one 16-bit operand).  Ranks behind the last are zero, as the bounds filled them.
+// JOB_FEW: the shared projection and the adapters of a call with few rows.  The epilogue's warps, idle while the tile's
 // products run, compute the adapters' part of the rows that their CTA will store, (lhs . down) . up in fp32, and put it
 // where the CTA's own partial sums are added to it.
-template <int CG, int NT, bool W_MN, bool SPLIT, bool FEW>
+template <int CG, int NT, bool W_MN, bool SPLIT, Job JOB>
 __global__ void __launch_bounds__(TURNED_THREADS, 1)
     turned_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                   const __grid_constant__ CUtensorMap map_x_chunk, const __grid_constant__ Params p) {
     using S = Turned<CG, NT>;
+    constexpr bool FEW = JOB == JOB_FEW, PARTS = JOB == JOB_PARTS;
     constexpr int STAGES = turned_stages<CG, NT, SPLIT>();
     static_assert(!SPLIT || (CG == 1 && NT == SPLIT_NT), "a cluster that splits the reduction holds single CTAs");
     static_assert(!FEW || SPLIT, "few rows");
@@ -1018,7 +797,6 @@ __global__ void __launch_bounds__(TURNED_THREADS, 1)
     // (one or the other)
     Run *table = reinterpret_cast<Run *>(reinterpret_cast<uint8_t *>(partials) + (SPLIT ? SPLIT_BYTES : 0));
     float *low = reinterpret_cast<float *>(table);
-    int *row_adapter = reinterpret_cast<int *>(low + SPLIT_NT * FEW_RANK);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
@@ -1177,11 +955,13 @@ __global__ void __launch_bounds__(TURNED_THREADS, 1)
             const int n = at.col0 + (CG == 1 ? 0 : static_cast<int>(cta_rank) * BM) + n_lane;
             const uint32_t buf = acc_it & 1;
             if constexpr (FEW)
-                adapters_part(p, at, partials, low, row_adapter, static_cast<int>(cta_rank), split);
+                adapters_part(p, at, partials, low, static_cast<int>(cta_rank), split);
             mbar_wait(&ctl->tmem_full[buf], (acc_it >> 1) & 1, wait_ctx, 0x400 | buf);
             tcgen05_fence_after_sync();
             const uint32_t taddr = tmem_base + buf * NT + (static_cast<uint32_t>(quadrant * 32) << 16);
             const int64_t column_at = n * p.out_stride1;
+            const int n_end = PARTS ? p.rank_blocks * RANK_BLOCK : p.n;
+            const float scale = PARTS ? p.scales[at.matrix * p.scales_stride] : 1.f;
             const int share = SPLIT ? split_share(at.rows, split) : 0;
 #pragma unroll 1
             for (int t0 = 32 * half; t0 < at.rows; t0 += 64) {
@@ -1210,6 +990,20 @@ __global__ void __launch_bounds__(TURNED_THREADS, 1)
                         }
                         store_remote(remote_address(dst, cta), v);
                     }
+                } else if constexpr (PARTS) {
+                    if (n - lane < n_end) {
+                        uint32_t low_part[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float v = scale * __uint_as_float(acc[j]), high = round16(v, bf16);
+                            acc[j] = __float_as_uint(v);
+                            // (an infinite or NaN high part says it all; inf - inf must not turn it into NaN)
+                            low_part[j] = __float_as_uint(isfinite(high) ? v - high : 0.f);
+                        }
+                        uint16_t *block = static_cast<uint16_t *>(p.out) + n / 32 * 32;
+                        store_turned(acc, block, p.out_stride0, at.row0 + t0, at.rows - t0, n, n_end, bf16);
+                        store_turned(low_part, block + 32, p.out_stride0, at.row0 + t0, at.rows - t0, n, n_end, bf16);
+                    }
                 } else if (p.out_vec) {
                     store_turned(acc, p.out, p.out_stride0, at.row0 + t0, at.rows - t0, n, p.n, bf16);
                 } else if (n < p.n) {
@@ -1227,7 +1021,7 @@ __global__ void __launch_bounds__(TURNED_THREADS, 1)
                 arrived = true;
                 mbar_wait_cluster(&ctl->partials, 0, wait_ctx, 0x500);
                 const int first = static_cast<int>(cta_rank) * share, last = min(at.rows, first + share);
-                if (n < p.n)
+                if (n < n_end)
                     for (int t = first + 4 * half; t < last; t += 8) {
                         const float4 *part = reinterpret_cast<const float4 *>(partials) + (t - first) / 4 * BM + n_lane;
                         float sum[4] = {};
@@ -1240,8 +1034,18 @@ __global__ void __launch_bounds__(TURNED_THREADS, 1)
                             sum[3] += v.w;
                         }
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (t + j < last) store16(p.out, (at.row0 + t + j) * p.out_stride0 + column_at, sum[j], bf16);
+                        for (int j = 0; j < 4; ++j) {
+                            if (t + j >= last) break;
+                            const int64_t row_at = (at.row0 + t + j) * p.out_stride0;
+                            if constexpr (PARTS) {
+                                const float v = scale * sum[j], high = round16(v, bf16);
+                                const int64_t to = row_at + n / RANK_BLOCK * (2 * RANK_BLOCK) + n % RANK_BLOCK;
+                                store16(p.out, to, v, bf16);
+                                store16(p.out, to + RANK_BLOCK, isfinite(high) ? v - high : 0.f, bf16);
+                            } else {
+                                store16(p.out, row_at + column_at, sum[j], bf16);
+                            }
+                        }
                     }
             }
             tcgen05_fence_before_sync();
@@ -1270,6 +1074,289 @@ __global__ void __launch_bounds__(TURNED_THREADS, 1)
         // of its work is its own CTA's.)
         cluster_wait();
     }
+    if (warp == 1) {
+        tcgen05_fence_after_sync();
+        tmem_dealloc<CG>(tmem_base, TMEM_COLS);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The shared projection with adapters beside it, for many rows: tiles of the projection (rows of lhs are the accumulator's
+// rows), then for every request in the tile the second product of its adapter, 32 ranks a stage, into that request's
+// accumulator rows only.  (scales lhs . down comes in two 16-bit parts from the launch before.)
+// B_MN: rhs has unit stride along its columns; otherwise along its rows (a transposed view).
+// ---------------------------------------------------------------------------
+template <int CG, int BN, bool B_MN>
+__global__ void __launch_bounds__(TURNED_THREADS, 1)
+    lora_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_chunk,
+                const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_low,
+                const __grid_constant__ CUtensorMap map_up, const __grid_constant__ Params p) {
+    using S = Shape<CG, BN>;
+    constexpr int STAGES = S::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Control *ctl = reinterpret_cast<Control *>(smem + STAGES * S::STAGE_BYTES);
+    Run *table = reinterpret_cast<Run *>(reinterpret_cast<uint8_t *>(ctl) + CONTROL_BYTES);
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int lane = threadIdx.x & 31;
+    const WaitCtx wait_ctx{&ctl->abort_flag, p.status, KID_GROUPED};
+    const uint32_t cta_rank = CG == 1 ? 0u : cluster_cta_rank();
+    const bool leader = cta_rank == 0;
+    const int worker = blockIdx.x / CG;
+    const int workers = gridDim.x / CG;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&ctl->full[s], 1);
+            mbar_init(&ctl->empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&ctl->tmem_full[b], 1);
+            mbar_init(&ctl->tmem_empty[b], EPILOGUE_WARPS * 32 * CG);
+        }
+        ctl->abort_flag = 0;
+        mbar_fence_init();
+        tma_prefetch_desc(&map_a);
+        tma_prefetch_desc(&map_b);
+    }
+    if (warp == 1) {
+        tmem_alloc<CG>(&ctl->tmem_base, TMEM_COLS);
+        tmem_relinquish<CG>();
+    }
+    build_table(p, table, ctl, S::TILE_M);
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
+    tcgen05_fence_after_sync();
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+    const int begin = ctl->row_begin, end = ctl->row_end, runs = ctl->runs;
+    const int m_tiles = (end - begin + S::TILE_M - 1) / S::TILE_M, total = m_tiles * p.n_tiles;
+
+    if (warp == 0) {
+        // --------------- TMA producer of the rows, of lhs and of (scales lhs . down) ---------------
+        const bool issuer = elect_one();
+        uint32_t s = 0, phase = 1;
+        const auto next = [&] {
+            if (++s == STAGES) {
+                s = 0;
+                phase ^= 1;
+            }
+        };
+        for (int tile = worker; tile < total; tile += workers) {
+            int m, n;
+            raster(tile, m_tiles, p.n_tiles, p.group_m, m, n);
+            const int row0 = begin + m * S::TILE_M, tile_end = min(end, row0 + S::TILE_M);
+            const int m0 = row0 + static_cast<int>(cta_rank) * BM;
+            const int boxes = a_boxes(tile_end - m0);
+            // the even CTA's barrier counts the bytes of both
+            int bytes = boxes * (A_CHUNK_ROWS * BK * 2) + S::B_STAGE_BYTES;
+            if constexpr (CG == 2) bytes += a_boxes(tile_end - m0 - BM) * (A_CHUNK_ROWS * BK * 2) + S::B_STAGE_BYTES;
+            for (int kb = 0; kb < p.k_blocks; ++kb) {
+                mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x100 | s);
+                uint8_t *dst = smem + s * S::STAGE_BYTES;
+                if (issuer) {
+                    if (leader) mbar_expect_tx(&ctl->full[s], bytes);
+                    if (boxes == BM / A_CHUNK_ROWS) {
+                        load_2d<CG>(dst, &map_a, &ctl->full[s], kb * BK, m0);
+                    } else {
+                        for (int c = 0; c < boxes; ++c)
+                            load_2d<CG>(dst + c * (A_CHUNK_ROWS * BK * 2), &map_a_chunk, &ctl->full[s], kb * BK, m0 + c * A_CHUNK_ROWS);
+                    }
+                }
+                next();
+            }
+            const int b_bytes = p.up_mn ? S::BN_CTA * RANK_BLOCK * 2 : S::B_STAGE_BYTES;
+            for (int r = first_run_behind(table, runs, row0); r < runs && table[r].begin < tile_end; ++r) {
+                // 32-row boxes of a CTA's rows that hold rows of the run
+                const int run_begin = table[r].begin, run_end = min(table[r].end, tile_end);
+                const auto box_range = [&](int base, int &first, int &last) {
+                    first = max(run_begin - base, 0) / A_CHUNK_ROWS;
+                    last = run_end <= base ? 0 : min((run_end - base + A_CHUNK_ROWS - 1) / A_CHUNK_ROWS, BM / A_CHUNK_ROWS);
+                    last = max(first, last);
+                };
+                int first, last, first_other = 0, last_other = 0;
+                box_range(m0, first, last);
+                if constexpr (CG == 2) box_range(row0 + BM, first_other, last_other);
+                int ext_bytes = (last - first) * (A_CHUNK_ROWS * BK * 2) + b_bytes;
+                if constexpr (CG == 2) ext_bytes += (last_other - first_other) * (A_CHUNK_ROWS * BK * 2) + b_bytes;
+                for (int rb = 0; rb < p.rank_blocks; ++rb) {
+                    mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x110 | s);
+                    uint8_t *dst = smem + s * S::STAGE_BYTES;
+                    if (issuer) {
+                        if (leader) mbar_expect_tx(&ctl->full[s], ext_bytes);
+                        for (int c = first; c < last; ++c)
+                            load_2d<CG>(dst + c * (A_CHUNK_ROWS * BK * 2), &map_low, &ctl->full[s], rb * BK, m0 + c * A_CHUNK_ROWS);
+                    }
+                    next();
+                }
+            }
+        }
+    } else if (warp == ROW_WARP) {
+        // -------------------- TMA producer of the matrices, rhs and up --------------------
+        const bool issuer = elect_one();
+        uint32_t s = 0, phase = 1;
+        const auto next = [&] {
+            if (++s == STAGES) {
+                s = 0;
+                phase ^= 1;
+            }
+        };
+        for (int tile = worker; tile < total; tile += workers) {
+            int m, n;
+            raster(tile, m_tiles, p.n_tiles, p.group_m, m, n);
+            const int row0 = begin + m * S::TILE_M, tile_end = min(end, row0 + S::TILE_M);
+            const int n0 = n * BN + static_cast<int>(cta_rank) * S::BN_CTA;
+            for (int kb = 0; kb < p.k_blocks; ++kb) {
+                mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x120 | s);
+                uint8_t *dst = smem + s * S::STAGE_BYTES + A_STAGE_BYTES;
+                if (issuer) {
+                    if constexpr (B_MN) {
+#pragma unroll
+                        for (int j = 0; j < S::BN_CTA / 64; ++j)
+                            load_3d<CG>(dst + j * (BK * 128), &map_b, &ctl->full[s], n0 + j * 64, kb * BK, 0);
+                    } else {
+                        load_3d<CG>(dst, &map_b, &ctl->full[s], kb * BK, n0, 0);
+                    }
+                }
+                next();
+            }
+            for (int r = first_run_behind(table, runs, row0); r < runs && table[r].begin < tile_end; ++r) {
+                const int matrix = table[r].matrix;
+                for (int rb = 0; rb < p.rank_blocks; ++rb) {
+                    mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x130 | s);
+                    uint8_t *dst = smem + s * S::STAGE_BYTES + A_STAGE_BYTES;
+                    if (issuer) {
+                        if (p.up_mn) {
+#pragma unroll
+                            for (int j = 0; j < S::BN_CTA / 64; ++j)
+                                load_3d<CG>(dst + j * (RANK_BLOCK * 128), &map_up, &ctl->full[s], n0 + j * 64, rb * RANK_BLOCK, matrix);
+                        } else {
+                            load_3d<CG>(dst, &map_up, &ctl->full[s], rb * RANK_BLOCK, n0, matrix);
+                        }
+                    }
+                    next();
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------- MMA issuer -------------------------------
+        // The warp runs the loop as one (the instruction takes uniform registers); an elected lane issues.
+        if (leader) {
+            const uint32_t idesc = umma_instr_desc(BM * CG, BN, p.bf16 != 0, false, B_MN);
+            const uint32_t idesc_up = umma_instr_desc(BM * CG, BN, p.bf16 != 0, false, p.up_mn != 0);
+            const uint32_t up_step = p.up_mn ? UMMA_K * 128 : UMMA_K * 2, up_lbo = p.up_mn ? RANK_BLOCK * 128 : 16;
+            const bool issuer = elect_one();
+            const uint32_t smem_base = smem_u32(smem);
+            uint32_t s = 0, phase = 0, acc_it = 0;
+            bool ready = false;
+            for (int tile = worker; tile < total; tile += workers, ++acc_it) {
+                int m, n;
+                raster(tile, m_tiles, p.n_tiles, p.group_m, m, n);
+                const int row0 = begin + m * S::TILE_M, tile_end = min(end, row0 + S::TILE_M);
+                const uint32_t buf = acc_it & 1;
+                mbar_wait_warp(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+                tcgen05_fence_after_sync();
+                const uint32_t tmem_acc = tmem_base + buf * BN;
+                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                    if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x300 | s);
+                    tcgen05_fence_after_sync();
+                    const uint32_t a_addr = smem_base + s * S::STAGE_BYTES;
+                    const uint32_t b_addr = a_addr + A_STAGE_BYTES;
+                    const uint32_t s_next = s + 1 == STAGES ? 0 : s + 1;
+                    const uint32_t phase_next = s_next == 0 ? phase ^ 1 : phase;
+#pragma unroll
+                    for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                        const uint64_t desc_a = umma_smem_desc(a_addr + kk * (UMMA_K * 2), 16, 1024);
+                        const uint64_t desc_b =
+                            umma_smem_desc(b_addr + kk * (B_MN ? UMMA_K * 128 : UMMA_K * 2), B_MN ? BK * 128 : 16, 1024);
+                        if (issuer) umma_ss<CG>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
+                        if (kk == BK / UMMA_K / 2 - 1)  // (a probe between MMAs costs nothing, a wait after them does)
+                            ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
+                    }
+                    if (issuer) {
+                        if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
+                        else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
+                    }
+                    s = s_next;
+                    phase = phase_next;
+                }
+                for (int r = first_run_behind(table, runs, row0); r < runs && table[r].begin < tile_end; ++r) {
+                    // Only the accumulator rows of this run take part: what another run's adapter holds, infinities and
+                    // NaN included, cannot reach them.
+                    const int low = table[r].begin - row0, high = min(table[r].end, tile_end) - row0;
+                    uint32_t off[8];
+#pragma unroll
+                    for (int w = 0; w < 8; ++w) off[w] = ~(low_bits(high - 32 * w) & ~low_bits(low - 32 * w));
+                    for (int rb = 0; rb < p.rank_blocks; ++rb) {
+                        if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x310 | s);
+                        ready = false;
+                        tcgen05_fence_after_sync();
+                        const uint32_t a_addr = smem_base + s * S::STAGE_BYTES;
+                        const uint32_t b_addr = a_addr + A_STAGE_BYTES;
+                        const int steps = (min(RANK_BLOCK, p.rank - rb * RANK_BLOCK) + UMMA_K - 1) / UMMA_K;
+                        for (int kk = 0; kk < steps; ++kk) {
+                            const uint64_t desc_b = umma_smem_desc(b_addr + kk * up_step, up_lbo, 1024);
+#pragma unroll
+                            for (int part = 0; part < 2; ++part) {
+                                const uint64_t desc_a =
+                                    umma_smem_desc(a_addr + part * (RANK_BLOCK * 2) + kk * (UMMA_K * 2), 16, 1024);
+                                if (issuer) umma_ss_lanes<CG>(tmem_acc, desc_a, desc_b, idesc_up, off);
+                            }
+                        }
+                        if (issuer) {
+                            if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
+                            else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
+                        }
+                        s = s + 1 == STAGES ? 0 : s + 1;
+                        if (s == 0) phase ^= 1;
+                    }
+                }
+                if (issuer) {
+                    if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
+                    else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // -------------------------------- epilogue --------------------------------
+        const int quadrant = warp & 3, half = (warp - 2) / 4;
+        const bool bf16 = p.bf16 != 0;
+        uint32_t acc_it = 0;
+        for (int tile = worker; tile < total; tile += workers, ++acc_it) {
+            int m, n;
+            raster(tile, m_tiles, p.n_tiles, p.group_m, m, n);
+            const int row0 = begin + m * S::TILE_M + static_cast<int>(cta_rank) * BM + quadrant * 32, n0 = n * BN;
+            const uint32_t buf = acc_it & 1;
+            mbar_wait(&ctl->tmem_full[buf], (acc_it >> 1) & 1, wait_ctx, 0x400 | buf);
+            tcgen05_fence_after_sync();
+            const uint32_t taddr = tmem_base + buf * BN + (static_cast<uint32_t>(quadrant * 32) << 16);
+#pragma unroll 1
+            for (int col = 32 * half; col < BN && n0 + col < p.n && row0 < end; col += 64) {
+                uint32_t acc[32];
+                __syncwarp();
+                tmem_ld_32x32(taddr + col, acc);
+                tmem_wait_ld();
+                if (p.out_vec) {
+                    store_rows(acc, p.out, p.out_stride0, row0, end - row0, n0 + col, p.n, bf16);
+                } else if (row0 + lane < end) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (n0 + col + j < p.n)
+                            store16(p.out, (row0 + lane) * p.out_stride0 + (n0 + col + j) * p.out_stride1, __uint_as_float(acc[j]), bf16);
+                }
+            }
+            tcgen05_fence_before_sync();
+            if (CG == 1 || leader) mbar_arrive(&ctl->tmem_empty[buf]);
+            else mbar_arrive_cluster(&ctl->tmem_empty[buf], 0);
+        }
+    }
+
+    __syncwarp();
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
     if (warp == 1) {
         tcgen05_fence_after_sync();
         tmem_dealloc<CG>(tmem_base, TMEM_COLS);
@@ -1562,8 +1649,12 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
                         tma_store_commit();
                     }
                 } else if (row < p.m) {
-                    store_columns(acc, p.out, at.run * p.out_batch_stride + row * p.out_stride0, p.out_stride1, at.n0 + col, p.n, false,
-                                  bf16);
+                    
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (at.n0 + col + j < p.n)
+                            store16(p.out, at.run * p.out_batch_stride + row * p.out_stride0 + (at.n0 + col + j) * p.out_stride1,
+                                    __uint_as_float(acc[j]), bf16);
                 }
             }
             if (!empty) {
@@ -1737,25 +1828,24 @@ struct Maps {
 
 constexpr size_t MAX_SMEM = 227 * 1024;
 
-template <int CG, int BN, bool B_MN, Mode MODE>
-int launch(cudaStream_t stream, const DeviceState &dev, const Maps &maps, const Params &p, int64_t most_tiles) {
-    auto kernel = grouped_kernel<CG, BN, B_MN, MODE>;
+template <int CG, int BN, bool B_MN>
+int launch_lora_kernel(cudaStream_t stream, const DeviceState &dev, const Maps &maps, const Params &p, int64_t tiles) {
+    auto kernel = lora_kernel<CG, BN, B_MN>;
     static_assert(1024 + Shape<CG, BN>::STAGES * Shape<CG, BN>::STAGE_BYTES + CONTROL_BYTES + table_bytes(MAX_RUNS) <= MAX_SMEM,
                   "shared memory per CTA");
-    const size_t smem = smem_bytes<CG, BN>(p.offsets.runs);
     static thread_local int configured_device = -1;
     static thread_local int pairs = 0;
     if (configured_device != dev.device) {
         NT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SMEM)));
-        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, MAX_SMEM);
+        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, MAX_SMEM, TURNED_THREADS);
         configured_device = dev.device;
     }
     const int workers = CG == 2 ? pairs : dev.sm_count;
-    if (workers <= 0) return fail(NINETOOTHED_B200_ERR_DEVICE, "grouped matmul: no CTA pair fits this device");
+    if (workers <= 0) return fail(NINETOOTHED_B200_ERR_DEVICE, "lora_matmul: no CTA pair fits this device");
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(most_tiles, workers) * CG));
-    config.blockDim = dim3(NUM_THREADS);
-    config.dynamicSmemBytes = smem;
+    config.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, workers) * CG));
+    config.blockDim = dim3(TURNED_THREADS);
+    config.dynamicSmemBytes = smem_bytes<CG, BN>(p.offsets.runs);
     config.stream = stream;
     cudaLaunchAttribute attr[1];
     if (CG == 2) {
@@ -1768,15 +1858,15 @@ int launch(cudaStream_t stream, const DeviceState &dev, const Maps &maps, const 
     return 0;
 }
 
-// Tensor maps of the row operand and the matrices, then the launch.
-template <int CG, int BN, Mode MODE>
-int launch_shape(cudaStream_t stream, const DeviceState &dev, int dtype, Maps &maps, Params &p, const void *lhs,
-                 int64_t lhs_stride0, const Matrices &rhs, const Matrices *up) {
+// Tensor maps, then the launch.  up: null where there are no adapters.
+template <int CG, int BN>
+int launch_lora(cudaStream_t stream, const DeviceState &dev, int dtype, Maps &maps, Params &p, const void *lhs, int64_t lhs_stride0,
+                const Matrices &rhs, const Matrices *up) {
     using S = Shape<CG, BN>;
     p.n_tiles = static_cast<int>((static_cast<int64_t>(p.n) + BN - 1) / BN);
+    p.k_blocks = (p.k + BK - 1) / BK;
     p.group_m = GROUP_ROWS / CG;
     const bool mn = rhs.use_mn();
-    p.b_lbo = mn ? BK * 128 : 16;
     if (int rc = map_rows(dev, &maps.a, dtype, lhs, p.rows, p.k, lhs_stride0, BK, BM)) return rc;
     if (int rc = map_rows(dev, &maps.a_chunk, dtype, lhs, p.rows, p.k, lhs_stride0, BK, A_CHUNK_ROWS)) return rc;
     if (int rc = map_matrices(dev, &maps.b, dtype, rhs, mn, 64, mn ? BK : S::BN_CTA)) return rc;
@@ -1784,33 +1874,18 @@ int launch_shape(cudaStream_t stream, const DeviceState &dev, int dtype, Maps &m
         p.up_mn = up->use_mn();
         if (int rc = map_matrices(dev, &maps.up, dtype, *up, p.up_mn, 64, p.up_mn ? RANK_BLOCK : S::BN_CTA)) return rc;
     } else {
-        maps.up = maps.a;
+        maps.up = maps.low = maps.a;
     }
-    if (MODE != LORA || up == nullptr) maps.low = maps.a;
-    const int64_t m_tiles = (static_cast<int64_t>(p.rows) + S::TILE_M - 1) / S::TILE_M +
-                            (MODE == LORA ? 0 : std::min(p.offsets.runs, p.rows));
-    if (m_tiles * p.n_tiles > INT_MAX / 2) return fail(NINETOOTHED_B200_ERR_SHAPE, "grouped matmul: too many tiles");
-    return mn ? launch<CG, BN, true, MODE>(stream, dev, maps, p, m_tiles * p.n_tiles)
-              : launch<CG, BN, false, MODE>(stream, dev, maps, p, m_tiles * p.n_tiles);
+    const int64_t tiles = (static_cast<int64_t>(p.rows) + S::TILE_M - 1) / S::TILE_M * p.n_tiles;
+    if (tiles > INT_MAX / 2) return fail(NINETOOTHED_B200_ERR_SHAPE, "lora_matmul: too many tiles");
+    return mn ? launch_lora_kernel<CG, BN, true>(stream, dev, maps, p, tiles) : launch_lora_kernel<CG, BN, false>(stream, dev, maps, p, tiles);
 }
 
-// Tiles of 256 x 256 on CTA pairs where there are rows for them; narrower ones on single CTAs otherwise.
-template <Mode MODE>
-int launch_product(cudaStream_t stream, const DeviceState &dev, int dtype, Maps &maps, Params &p, const void *lhs,
-                   int64_t lhs_stride0, const Matrices &rhs, const Matrices *up, int64_t live_runs) {
-    const int64_t run_rows = p.rows / std::max<int64_t>(1, live_runs);
-    if (run_rows >= 192) return launch_shape<2, 256, MODE>(stream, dev, dtype, maps, p, lhs, lhs_stride0, rhs, up);
-    const int64_t tiles_128 = live_runs * ((run_rows + BM - 1) / BM) * ((p.n + 127) / 128);
-    if (tiles_128 >= 2 * dev.sm_count)
-        return launch_shape<1, 128, MODE>(stream, dev, dtype, maps, p, lhs, lhs_stride0, rhs, up);
-    return launch_shape<1, 64, MODE>(stream, dev, dtype, maps, p, lhs, lhs_stride0, rhs, up);
-}
-
-template <int CG, int NT, bool W_MN, bool SPLIT, bool FEW>
+template <int CG, int NT, bool W_MN, bool SPLIT, Job JOB>
 int launch_turned_kernel(cudaStream_t stream, const DeviceState &dev, const CUtensorMap &map_w, const CUtensorMap &map_x,
                          const CUtensorMap &map_x_chunk, const Params &p, int64_t most_tiles) {
-    auto kernel = turned_kernel<CG, NT, W_MN, SPLIT, FEW>;
-    static_assert(turned_smem<CG, NT, SPLIT, FEW>(MAX_RUNS) <= MAX_SMEM, "shared memory per CTA");
+    auto kernel = turned_kernel<CG, NT, W_MN, SPLIT, JOB>;
+    static_assert(turned_smem<CG, NT, SPLIT, JOB == JOB_FEW>(MAX_RUNS) <= MAX_SMEM, "shared memory per CTA");
     static thread_local int configured_device = -1;
     static thread_local int pairs = 0;
     if (configured_device != dev.device) {
@@ -1824,7 +1899,7 @@ int launch_turned_kernel(cudaStream_t stream, const DeviceState &dev, const CUte
     const int cluster = SPLIT ? p.split : CG;
     config.gridDim = dim3(static_cast<unsigned>(workers * cluster));
     config.blockDim = dim3(TURNED_THREADS);
-    config.dynamicSmemBytes = turned_smem<CG, NT, SPLIT, FEW>(p.offsets.runs);
+    config.dynamicSmemBytes = turned_smem<CG, NT, SPLIT, JOB == JOB_FEW>(p.offsets.runs);
     config.stream = stream;
     cudaLaunchAttribute attr[2];
     config.attrs = attr;
@@ -1833,7 +1908,7 @@ int launch_turned_kernel(cudaStream_t stream, const DeviceState &dev, const CUte
         attr[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
         attr[config.numAttrs++].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
     }
-    if (FEW && p.low_chunks > 0) {  // starts under the kernel before it
+    if (JOB == JOB_FEW && p.low_chunks > 0) {  // starts under the kernel before it
         attr[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
@@ -1841,7 +1916,7 @@ int launch_turned_kernel(cudaStream_t stream, const DeviceState &dev, const CUte
     return 0;
 }
 
-template <int CG, int NT, bool SPLIT, bool FEW = false>
+template <int CG, int NT, bool SPLIT, Job JOB>
 int launch_turned(cudaStream_t stream, const DeviceState &dev, int dtype, Params &p, const void *lhs, int64_t lhs_stride0,
                   const Matrices &rhs, int64_t live_runs) {
     using S = Turned<CG, NT>;
@@ -1853,10 +1928,10 @@ int launch_turned(cudaStream_t stream, const DeviceState &dev, int dtype, Params
     if (int rc = map_matrices(dev, &map_w, dtype, rhs, mn, 64, mn ? S::DEPTH : BM)) return rc;
     if (int rc = map_rows(dev, &map_x, dtype, lhs, p.rows, p.k, lhs_stride0, BK, S::ROWS_CTA)) return rc;
     if (int rc = map_rows(dev, &map_x_chunk, dtype, lhs, p.rows, p.k, lhs_stride0, BK, A_CHUNK_ROWS)) return rc;
-    const int64_t most = (FEW ? (p.rows + NT - 1) / NT : live_runs + p.rows / NT) * p.n_tiles;
+    const int64_t most = (JOB == JOB_FEW ? (p.rows + NT - 1) / NT : live_runs + p.rows / NT) * p.n_tiles;
     if (most > INT_MAX / 16) return fail(NINETOOTHED_B200_ERR_SHAPE, "grouped matmul: too many tiles");
-    return mn ? launch_turned_kernel<CG, NT, true, SPLIT, FEW>(stream, dev, map_w, map_x, map_x_chunk, p, most)
-              : launch_turned_kernel<CG, NT, false, SPLIT, FEW>(stream, dev, map_w, map_x, map_x_chunk, p, most);
+    return mn ? launch_turned_kernel<CG, NT, true, SPLIT, JOB>(stream, dev, map_w, map_x, map_x_chunk, p, most)
+              : launch_turned_kernel<CG, NT, false, SPLIT, JOB>(stream, dev, map_w, map_x, map_x_chunk, p, most);
 }
 
 // Which tiles a grouped product gets.  The bounds lie on the device, so the host goes by averages: `live` runs at most
@@ -1872,7 +1947,7 @@ int launch_grouped(cudaStream_t stream, const DeviceState &dev, int dtype, Param
     const int64_t few = (live + p.rows / SPLIT_NT) * n_tiles, blocks = (static_cast<int64_t>(p.k) + 2 * BK - 1) / (2 * BK);
     p.split = 1;
     while (p.split < 8 && few * p.split * 2 <= dev.sm_count && blocks >= p.split * 4) p.split *= 2;
-    if (p.split > 1) return launch_turned<1, SPLIT_NT, true>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
+    if (p.split > 1) return launch_turned<1, SPLIT_NT, true, JOB_PRODUCT>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
     const auto cost = [&](int64_t rows, int64_t columns, int64_t workers, int64_t cycles) {
         const int64_t halves = std::max<int64_t>(2 * live, 2 * p.rows / rows + live);  // half tiles
         const int64_t tiles = (halves * ((p.n + columns - 1) / columns) + 1) / 2;
@@ -1881,19 +1956,24 @@ int launch_grouped(cudaStream_t stream, const DeviceState &dev, int dtype, Param
     const int64_t narrow = cost(64, 128, dev.sm_count, 830), middle = cost(128, 128, dev.sm_count, 1080),
                   wide = cost(256, 256, dev.sm_count / 2, 1540);
     if (narrow <= middle && narrow <= wide)
-        return launch_turned<1, 64, false>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
-    if (middle <= wide) return launch_turned<1, 128, false>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
-    return launch_turned<2, 256, false>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
+        return launch_turned<1, 64, false, JOB_PRODUCT>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
+    if (middle <= wide) return launch_turned<1, 128, false, JOB_PRODUCT>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
+    return launch_turned<2, 256, false, JOB_PRODUCT>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
 }
 
-// Few rows under adapters: their share of the output costs no tile of its own, and runs under the streaming of rhs.
 int64_t low_chunks(int64_t k) { return (k + LOW_CHUNK - 1) / LOW_CHUNK; }
 
-bool few_rows(int64_t rows, int64_t rank) { return rows <= FEW_ROWS && rank <= FEW_RANK; }
+// Few rows, or requests of few rows each: the adapters' part costs no tile of its own and runs under the streaming of rhs, a
+// row at a time.  Otherwise every request of a tile costs the tensor cores' issuer half a microsecond, whatever its length.
+// 4096 x 4096, rank 16, this way against the other: 64 rows in 64 requests 19 against 46 us, in 4 requests 19 / 29; 256 rows
+// in 256 requests 48 / 95, in 16 requests 45 / 33; 512 rows in 512 requests 97 / 125, in 128 requests 91 / 62.
+bool few_rows(int64_t rows, int64_t rank, int64_t requests) {
+    return rank <= FEW_RANK && (rows <= 64 || (rows <= FEW_ROWS && rows < 4 * requests));
+}
 
 size_t lora_workspace(int64_t rows, int64_t k, int64_t rank) {
     const size_t parts = static_cast<size_t>(rows) * ((rank + RANK_BLOCK - 1) / RANK_BLOCK) * RANK_BLOCK * 4;
-    const size_t sums = few_rows(rows, rank) ? static_cast<size_t>(low_chunks(k)) * rows * rank * 4 : 0;
+    const size_t sums = few_rows(rows, rank, rows) ? static_cast<size_t>(low_chunks(k)) * rows * rank * 4 : 0;
     return std::max(parts, sums);
 }
 
@@ -1917,7 +1997,7 @@ int launch_few(cudaStream_t stream, const DeviceState &dev, int dtype, Params &p
     const int64_t blocks = (static_cast<int64_t>(p.k) + 2 * BK - 1) / (2 * BK);
     p.split = 1;
     while (p.split < 8 && tiles * p.split * 2 <= dev.sm_count && blocks >= p.split * 2) p.split *= 2;
-    return launch_turned<1, SPLIT_NT, true, true>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, 1);
+    return launch_turned<1, SPLIT_NT, true, JOB_FEW>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, 1);
 }
 
 bool has_arrays(const NineToothedTensor &t) { return t.shape != nullptr && t.strides != nullptr; }
@@ -2084,8 +2164,37 @@ int run_grouped_grad(cudaStream_t stream, const NineToothedTensor &lhs, const Ni
     return 0;
 }
 
-// scales (lhs . down) of every row: per 32 ranks, 32 high and 32 low 16-bit parts (or, on the plain path, fp32).
-int64_t rank_blocks(int64_t rank) { return (rank + RANK_BLOCK - 1) / RANK_BLOCK; }
+// Many rows under adapters: first scales (lhs . down), then the projection with the second products.
+int launch_many(cudaStream_t stream, const DeviceState &dev, int dtype, Params &p, const void *lhs, int64_t lhs_stride0,
+                const Matrices &rhs, const Matrices &down, const Matrices &up, void *workspace) {
+    Maps maps;
+    const bool any = p.matrices > 0;
+    if (any) {
+        Params parts = p;
+        parts.n = p.rank;
+        parts.out = workspace;
+        parts.out_stride0 = p.rank_blocks * (2 * RANK_BLOCK);
+        parts.out_stride1 = 1;
+        const int64_t live = std::min(p.offsets.runs, p.rows), n_tiles = (p.rank + BM - 1) / BM;
+        const int64_t blocks = (static_cast<int64_t>(p.k) + 2 * BK - 1) / (2 * BK), narrow = (live + p.rows / 64) * n_tiles;
+        parts.split = 1;
+        while (parts.split < 8 && narrow * parts.split * 2 <= dev.sm_count && blocks >= parts.split * 2) parts.split *= 2;
+        int rc;
+        if (parts.split > 1) rc = launch_turned<1, SPLIT_NT, true, JOB_PARTS>(stream, dev, dtype, parts, lhs, lhs_stride0, down, live);
+        else if (narrow <= 2 * dev.sm_count) rc = launch_turned<1, 64, false, JOB_PARTS>(stream, dev, dtype, parts, lhs, lhs_stride0, down, live);
+        else rc = launch_turned<1, 128, false, JOB_PARTS>(stream, dev, dtype, parts, lhs, lhs_stride0, down, live);
+        if (rc != 0) return rc;
+        if ((rc = map_rows(dev, &maps.low, dtype, workspace, p.rows, parts.out_stride0, parts.out_stride0, BK, A_CHUNK_ROWS)) != 0) return rc;
+    }
+    // Tiles of 256 x 256 on CTA pairs, or 128 x 128 on single CTAs where that takes fewer waves' time (a 128 x 128 tile takes
+    // about half the pair's time for its 64-deep block: it is bound by L2).
+    const auto waves = [&](int64_t rows, int64_t columns, int64_t workers) {
+        return ((p.rows + rows - 1) / rows * ((p.n + columns - 1) / columns) + workers - 1) / workers;
+    };
+    if (7 * waves(256, 256, dev.sm_count / 2) <= 5 * waves(128, 128, dev.sm_count))
+        return launch_lora<2, 256>(stream, dev, dtype, maps, p, lhs, lhs_stride0, rhs, any ? &up : nullptr);
+    return launch_lora<1, 128>(stream, dev, dtype, maps, p, lhs, lhs_stride0, rhs, any ? &up : nullptr);
+}
 
 int run_lora(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothedTensor &rhs, const NineToothedTensor &down,
              const NineToothedTensor &up, const NineToothedTensor &scales, const NineToothedTensor &offsets,
@@ -2136,39 +2245,21 @@ int run_lora(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothe
     p.scales = static_cast<const float *>(scales.data);
     p.scales_stride = scales.strides[0];
     p.rank = static_cast<int>(rank);
-    p.rank_blocks = static_cast<int>(rank_blocks(rank));
+    p.rank_blocks = static_cast<int>((rank + RANK_BLOCK - 1) / RANK_BLOCK);
     p.status = dev->status;
     const Matrices shared{rhs.data, 1, k, n, 0, rhs.strides[0], rhs.strides[1]};
     const Matrices first{down.data, count, k, rank, down.strides[0], down.strides[1], down.strides[2]};
     const Matrices second{up.data, count, rank, n, up.strides[0], up.strides[1], up.strides[2]};
     if (rows_addressable(lhs.data, rows, k, lhs.strides[0], lhs.strides[1]) && shared.addressable() &&
         (!any || (first.addressable() && second.addressable()))) {
-        if (few_rows(rows, rank)) {
-            p.n = static_cast<int>(n);
-            p.out = output.data;
-            p.out_stride0 = output.strides[0];
-            p.out_stride1 = output.strides[1];
-            p.out_vec = output_vec(output);
-            return launch_few(stream, *dev, dtype, p, lhs.data, lhs.strides[0], shared, first, second, static_cast<float *>(workspace));
-        }
-        Maps maps;
-        if (any) {
-            Params shrink = p;
-            shrink.n = p.rank;
-            shrink.out = workspace;
-            shrink.out_stride0 = rank_blocks(rank) * RANK_BLOCK * 2;
-            shrink.out_stride1 = 1;
-            if (int rc = launch_shape<1, 64, SHRINK>(stream, *dev, dtype, maps, shrink, lhs.data, lhs.strides[0], first, nullptr))
-                return rc;
-            if (int rc = map_rows(*dev, &maps.low, dtype, workspace, rows, shrink.out_stride0, shrink.out_stride0, BK, A_CHUNK_ROWS))
-                return rc;
-        }
         p.n = static_cast<int>(n);
         p.out = output.data;
         p.out_stride0 = output.strides[0];
         p.out_stride1 = output.strides[1];
         p.out_vec = output_vec(output);
-        return launch_product<LORA>(stream, *dev, dtype, maps, p, lhs.data, lhs.strides[0], shared, any ? &second : nullptr, 1);
+        if (few_rows(rows, rank, runs))
+            return launch_few(stream, *dev, dtype, p, lhs.data, lhs.strides[0], shared, first, second, static_cast<float *>(workspace));
+        return launch_many(stream, *dev, dtype, p, lhs.data, lhs.strides[0], shared, first, second, workspace);
     }
     note_plain_launch("lora_matmul %lld x %lld x %lld, rank %lld, runs on the plain CUDA-core kernels: the tensor-core path needs "
                       "a unit-stride K in lhs, a unit-stride dimension in rhs, down and up, the other strides multiples of 8 "
