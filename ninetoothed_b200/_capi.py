@@ -19,6 +19,7 @@ import warnings
 import torch
 
 LIBRARY_PATH = pathlib.Path(__file__).resolve().parent / "lib" / "libninetoothed_b200.so"
+TORCH_LIBRARY_PATH = LIBRARY_PATH.with_name("libninetoothed_b200_torch.so")
 
 # enum NineToothedDataType (same order as the reference, src/ninetoothed/aot.py:524-537)
 DTYPE_INDEX = {
@@ -218,17 +219,23 @@ _plain_launches_seen = 0
 
 
 def _call(name, device, *args):
-    global _plain_launches_seen
     lib = library()
     if torch.cuda.current_device() == device.index:  # (switching the device and back costs more than a small launch)
         check(name, getattr(lib, name)(current_stream(device), *args))
     else:
         with torch.cuda.device(device):
             check(name, getattr(lib, name)(current_stream(device), *args))
+    warn_of_plain_launches()
+
+
+def warn_of_plain_launches():
+    """A launch that left the tensor-core path says so (Python shows it once per site)."""
+    global _plain_launches_seen
+    lib = library()
     count = lib.ninetoothed_b200_plain_launches(0)
-    if count != _plain_launches_seen:  # this launch left the tensor-core path: say so (Python shows it once per site)
+    if count != _plain_launches_seen:
         _plain_launches_seen = count
-        warnings.warn(lib.ninetoothed_b200_last_note().decode("utf-8", "replace"), SlowPathWarning, stacklevel=3)
+        warnings.warn(lib.ninetoothed_b200_last_note().decode("utf-8", "replace"), SlowPathWarning, stacklevel=4)
 
 
 def matmul(lhs, rhs, output):

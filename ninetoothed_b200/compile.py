@@ -6,6 +6,9 @@ Each ``csrc/*.cu`` is compiled to an object file (in parallel), then linked with
 the static CUDA runtime into ``ninetoothed_b200/lib/libninetoothed_b200.so``.
 The library has no link-time dependency on the driver (it looks the one driver
 entry point it needs up at run time), so it loads on a GPU-less host.
+
+``csrc/torch_binding.cpp``, the C++ half of the PyTorch operators, becomes
+``libninetoothed_b200_torch.so`` beside it (the only part that knows PyTorch).
 """
 
 from __future__ import annotations
@@ -23,6 +26,8 @@ INCLUDE_DIR = PACKAGE_DIR.parent / "include"
 LIB_DIR = PACKAGE_DIR / "lib"
 OBJ_DIR = LIB_DIR / "obj"
 LIBRARY = LIB_DIR / "libninetoothed_b200.so"
+TORCH_SOURCE = CSRC_DIR / "torch_binding.cpp"
+TORCH_LIBRARY = LIB_DIR / "libninetoothed_b200_torch.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -82,7 +87,29 @@ def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
+    header = INCLUDE_DIR / "ninetoothed_b200.h"
+    if force or not TORCH_LIBRARY.exists() or TORCH_LIBRARY.stat().st_mtime < max(TORCH_SOURCE.stat().st_mtime,
+                                                                                 header.stat().st_mtime):
+        _build_torch_binding()
     return LIBRARY
+
+
+def _build_torch_binding() -> None:
+    import sysconfig
+
+    import torch
+
+    torch_dir = pathlib.Path(torch.__file__).resolve().parent
+    cuda_include = pathlib.Path(find_nvcc()).resolve().parent.parent / "include"
+    includes = [INCLUDE_DIR, torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include", cuda_include,
+                sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared", *(f"-I{path}" for path in includes),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", str(TORCH_SOURCE), "-o", str(TORCH_LIBRARY),
+           f"-L{LIB_DIR}", f"-L{torch_dir / 'lib'}", "-lninetoothed_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {TORCH_SOURCE.name}:\n{proc.stdout}\n{proc.stderr}")
 
 
 if __name__ == "__main__":

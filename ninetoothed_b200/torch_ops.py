@@ -76,9 +76,14 @@ def _max_pool2d(input, output, window_height, window_width, ceil_mode):
 _LIBRARY.impl("matmul", _matmul, "CUDA")
 _LIBRARY.impl("bmm", _bmm, "CUDA")
 _LIBRARY.impl("addmm", _addmm, "CUDA")
-_LIBRARY.impl("grouped_matmul", _grouped_matmul, "CUDA")
-_LIBRARY.impl("grouped_matmul_rhs_grad", _grouped_matmul_rhs_grad, "CUDA")
-_LIBRARY.impl("lora_matmul", _lora_matmul, "CUDA")
+if _capi.TORCH_LIBRARY_PATH.exists():
+    # The products by runs of rows are small calls as often as not: their ordinary calls are marshalled in C++, which
+    # hands everything else to the functions above.
+    torch.ops.load_library(str(_capi.TORCH_LIBRARY_PATH))
+else:  # (not built: these raise)
+    _LIBRARY.impl("grouped_matmul", _grouped_matmul, "CUDA")
+    _LIBRARY.impl("grouped_matmul_rhs_grad", _grouped_matmul_rhs_grad, "CUDA")
+    _LIBRARY.impl("lora_matmul", _lora_matmul, "CUDA")
 _LIBRARY.impl("softmax", _softmax, "CUDA")
 _LIBRARY.impl("attention", _attention, "CUDA")
 _LIBRARY.impl("attention_scaled", _attention_scaled, "CUDA")

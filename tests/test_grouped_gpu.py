@@ -478,3 +478,31 @@ def test_far_rows_pass_32_bit_offsets():
     for e, (a, b) in enumerate(((-300, -100), (-100, None))):
         x, y = lhs[a:b].double(), output[a:b, :64].double()
         assert_within(grad[e], x.t() @ y, x.abs().t() @ y.abs() * (200 * 2.0 ** -23))
+
+
+def test_the_operators_raise_what_the_bindings_raise():
+    """Refusals come through the custom operators as the bindings' own exceptions, and nothing is written."""
+    from ninetoothed_b200 import _capi
+    from ninetoothed_b200.torch_ops import ops
+
+    lhs, rhs, offsets = normal(95, 40, 64), normal(96, 2, 64, 72), bounds_of([10, 30])
+    output = torch.full((40, 72), 7.0, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(TypeError, match="must have the same dtype"):
+        ops.grouped_matmul(lhs, rhs.half(), offsets, output)
+    with pytest.raises(ValueError, match="must have 3 dimensions"):
+        ops.grouped_matmul(lhs, rhs[0], offsets, output)
+    with pytest.raises(TypeError, match="int32 or torch.int64"):
+        ops.grouped_matmul(lhs, rhs, offsets.short(), output)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        ops.grouped_matmul(lhs, rhs, offsets.cpu(), output)
+    with pytest.raises(_capi.KernelLaunchError, match="shapes do not agree"):
+        ops.grouped_matmul(lhs, rhs, offsets, output[:, :64])
+    with pytest.raises(_capi.KernelLaunchError, match="must hold 3 bounds"):
+        ops.grouped_matmul_rhs_grad(lhs, output, offsets[:2], torch.empty_like(rhs))
+    down, up, scales = normal(97, 3, 64, 8), normal(98, 3, 8, 72), torch.ones(3, device="cuda")
+    adapters = torch.zeros(2, dtype=torch.int64, device="cuda")
+    with pytest.raises(TypeError, match="scales must be torch.float32"):
+        ops.lora_matmul(lhs, rhs[0], down, up, scales.half(), offsets, adapters, output)
+    with pytest.raises(_capi.KernelLaunchError, match="shapes do not agree"):
+        ops.lora_matmul(lhs, rhs[0], down, up[:, :, :64], scales, offsets, adapters, output)
+    assert (output == 7.0).all()
