@@ -518,34 +518,52 @@ __device__ __forceinline__ void load_values(const uint16_t *at, int left, bool b
 
 __device__ __forceinline__ void prefetch_l2(const void *at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at)); }
 
-// `count` rows' second products with up (unit stride along its columns), four columns a lane: sixteen ranks of all of them
-// in flight at once.  l: the rows' (scales lhs . down).
-template <int COUNT>
-__device__ __forceinline__ void second_product(const uint16_t *const (&matrix)[COUNT], const float *const (&l)[COUNT], int64_t stride,
-                                               int rank, bool bf16, float (&sum)[COUNT][4]) {
-    for (int r0 = 0; r0 < rank; r0 += 16) {
-        uint2 v[COUNT][16];
+// Sixteen ranks of four columns of up, from rank r0 on: eight bytes a rank where a rank's columns lie side by side, two times
+// sixteen bytes a column where a column's ranks do (their number is a multiple of eight then).  Ranks behind the last are 0.
+__device__ __forceinline__ void load_ranks(const Params &p, const uint16_t *matrix, int col, int r0, uint32_t (&v)[32]) {
+    if (p.up_mn) {
 #pragma unroll
-        for (int c = 0; c < COUNT; ++c)
+        for (int r = 0; r < 16; ++r) {
+            const uint2 w = r0 + r < p.rank ? __ldg(reinterpret_cast<const uint2 *>(matrix + (r0 + r) * p.up_stride[1] + col)) : make_uint2(0, 0);
+            v[2 * r] = w.x;
+            v[2 * r + 1] = w.y;
+        }
+    } else {
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                v[c][r] = r0 + r < rank ? __ldg(reinterpret_cast<const uint2 *>(matrix[c] + (r0 + r) * stride)) : make_uint2(0, 0);
+        for (int i = 0; i < 8; ++i) {
+            const int r = r0 + i % 2 * 8;
+            const uint4 w = r < p.rank ? __ldg(reinterpret_cast<const uint4 *>(matrix + (col + i / 2) * p.up_stride[2] + r)) : make_uint4(0, 0, 0, 0);
+            v[4 * i] = w.x;
+            v[4 * i + 1] = w.y;
+            v[4 * i + 2] = w.z;
+            v[4 * i + 3] = w.w;
+        }
+    }
+}
+
+// ... times the row's (lhs . down).
+__device__ __forceinline__ void add_ranks(const Params &p, const uint32_t (&v)[32], const float *l, int r0, bool bf16, float (&sum)[4]) {
+    if (p.up_mn) {
 #pragma unroll
-        for (int c = 0; c < COUNT; ++c)
+        for (int r = 0; r < 16; ++r) {
+            const float weight = r0 + r < p.rank ? l[r0 + r] : 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float weight = r0 + r < rank ? l[c][r0 + r] : 0.f;
-                sum[c][0] = fmaf(weight, half_of(v[c][r].x, 0, bf16), sum[c][0]);
-                sum[c][1] = fmaf(weight, half_of(v[c][r].x, 1, bf16), sum[c][1]);
-                sum[c][2] = fmaf(weight, half_of(v[c][r].y, 0, bf16), sum[c][2]);
-                sum[c][3] = fmaf(weight, half_of(v[c][r].y, 1, bf16), sum[c][3]);
-            }
+            for (int j = 0; j < 4; ++j) sum[j] = fmaf(weight, half_of(v[2 * r + j / 2], j & 1, bf16), sum[j]);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float weight = r0 + r < p.rank ? l[r0 + r] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] = fmaf(weight, half_of(v[8 * j + r / 2], r & 1, bf16), sum[j]);
+        }
     }
 }
 
 // scales (lhs . down) . up of the rows that this CTA stores into its own slot of the partial sums.  A warp takes every
-// eighth row, a lane four columns of the tile.  What does not depend on the launch before (which adapter, its matrix on the
-// way to L2) is done before the wait for it.  It is all memory latency: a step is done for all of the warp's rows at once.
+// eighth row, a lane four columns of the tile.  It is all memory latency, and a load waits behind the copies that stream the
+// tile's operands: a step is done for all of the warp's rows at once, and what does not depend on the launch before (which
+// adapter, its matrix on the way to L2, its first ranks for the first two rows in registers) before the wait for it.
 __device__ __forceinline__ void adapters_part(const Params &p, const TurnedPlace &at, float *partials, float *low, int cta_rank,
                                               int split) {
     const int warp = static_cast<int>(threadIdx.x) / 32 - 2, lane = threadIdx.x & 31;
@@ -595,6 +613,15 @@ __device__ __forceinline__ void adapters_part(const Params &p, const TurnedPlace
                 for (int r = 0; r < p.rank; r += 64) prefetch_l2(matrix + (col + j) * p.up_stride[2] + r);
         }
     }
+    const bool wide = left >= 4 && (p.up_mn || p.rank % 8 == 0);  // this lane's columns come in whole loads
+    const auto matrix_of = [&](int i) {
+        const int which = __shfl_sync(0xffffffffu, adapter, i);
+        return which < 0 || i >= rows ? nullptr : up + which * p.up_stride[0];
+    };
+    const uint16_t *m0 = matrix_of(0), *m1 = matrix_of(1);
+    uint32_t v0[32], v1[32];
+    if (wide && m0 != nullptr) load_ranks(p, m0, col, 0, v0);
+    if (wide && m1 != nullptr) load_ranks(p, m1, col, 0, v1);
     griddepcontrol_wait();  // (the sums of lhs . down come from the launch before)
 #pragma unroll 4
     for (int q = lane; q < rows * p.rank; q += 32) {
@@ -605,65 +632,38 @@ __device__ __forceinline__ void adapters_part(const Params &p, const TurnedPlace
         low[t * p.rank + (q - i * p.rank)] = total;
     }
     __syncwarp();
-    const auto put = [&](int t, float factor, const float (&sum)[4]) {
-        float *dst = partials + ((cta_rank * share + t) / 4 * BM + lane * 4) * 4 + t % 4;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dst[j * 4] = factor * sum[j];
-    };
-    int i = 0;
-    for (; p.up_mn && i + 2 <= rows; i += 2) {
-        const int t = warp + EPILOGUE_WARPS * i;
-        const int a0 = __shfl_sync(0xffffffffu, adapter, i), a1 = __shfl_sync(0xffffffffu, adapter, i + 1);
-        const float s0 = __shfl_sync(0xffffffffu, scale, i), s1 = __shfl_sync(0xffffffffu, scale, i + 1);
-        if (a0 < 0 || a1 < 0 || p.n - at.col0 < BM) break;  // (the rest one by one)
-        float sum[2][4] = {};
-        const uint16_t *const matrix[2] = {up + a0 * p.up_stride[0] + col, up + a1 * p.up_stride[0] + col};
-        const float *const l[2] = {low + t * p.rank, low + (t + EPILOGUE_WARPS) * p.rank};
-        second_product<2>(matrix, l, p.up_stride[1], p.rank, bf16, sum);
-        put(t, s0, sum[0]);
-        put(t + EPILOGUE_WARPS, s1, sum[1]);
-    }
-    for (; i < rows; ++i) {
-        const int t = warp + EPILOGUE_WARPS * i;
-        const int which = __shfl_sync(0xffffffffu, adapter, i);
-        const float factor = __shfl_sync(0xffffffffu, scale, i);
-        float sum[1][4] = {};
-        if (which >= 0 && left > 0) {
-            const float *l = low + t * p.rank;
-            const uint16_t *matrix = up + which * p.up_stride[0];
-            if (left >= 4 && p.up_mn) {
-                const uint16_t *const matrices[1] = {matrix + col};
-                const float *const ls[1] = {l};
-                second_product<1>(matrices, ls, p.up_stride[1], p.rank, bf16, sum);
-            } else if (left >= 4 && p.rank % 8 == 0) {  // a column's ranks lie side by side
-                for (int r0 = 0; r0 < p.rank; r0 += 32) {
-                    uint4 v[4][4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            v[q][j] = r0 + q * 8 < p.rank
-                                          ? __ldg(reinterpret_cast<const uint4 *>(matrix + (col + j) * p.up_stride[2] + r0 + q * 8))
-                                          : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        if (r0 + q * 8 >= p.rank) break;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t words[4] = {v[q][j].x, v[q][j].y, v[q][j].z, v[q][j].w};
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                sum[0][j] = fmaf(l[r0 + q * 8 + e], half_of(words[e / 2], e & 1, bf16), sum[0][j]);
-                        }
-                    }
-                }
-            } else {
-                for (int r = 0; r < p.rank; ++r)
-                    for (int j = 0; j < 4 && j < left; ++j)
-                        sum[0][j] = fmaf(l[r], load16(matrix, r * p.up_stride[1] + (col + j) * p.up_stride[2], bf16), sum[0][j]);
-            }
+    for (int i = 0; i < rows; i += 2) {
+        const int t0 = warp + EPILOGUE_WARPS * i, t1 = t0 + EPILOGUE_WARPS;
+        const float *l0 = low + t0 * p.rank, *l1 = low + t1 * p.rank;
+        if (i > 0) {
+            m0 = matrix_of(i);
+            m1 = matrix_of(min(i + 1, 31));
         }
-        put(t, factor, sum[0]);
+        float sum0[4] = {}, sum1[4] = {};
+        if (wide) {
+            for (int r0 = 0; r0 < p.rank; r0 += 16) {
+                if (i > 0 || r0 > 0) {
+                    if (m0 != nullptr) load_ranks(p, m0, col, r0, v0);
+                    if (m1 != nullptr) load_ranks(p, m1, col, r0, v1);
+                }
+                if (m0 != nullptr) add_ranks(p, v0, l0, r0, bf16, sum0);
+                if (m1 != nullptr) add_ranks(p, v1, l1, r0, bf16, sum1);
+            }
+        } else {
+            for (int r = 0; r < p.rank; ++r)
+                for (int j = 0; j < 4 && j < left; ++j) {
+                    const int64_t at_up = r * p.up_stride[1] + (col + j) * p.up_stride[2];
+                    if (m0 != nullptr) sum0[j] = fmaf(l0[r], load16(m0, at_up, bf16), sum0[j]);
+                    if (m1 != nullptr) sum1[j] = fmaf(l1[r], load16(m1, at_up, bf16), sum1[j]);
+                }
+        }
+        const float s0 = __shfl_sync(0xffffffffu, scale, i), s1 = __shfl_sync(0xffffffffu, scale, i + 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            partials[((cta_rank * share + t0) / 4 * BM + lane * 4 + j) * 4 + t0 % 4] = m0 != nullptr ? s0 * sum0[j] : 0.f;
+            if (i + 1 < rows)
+                partials[((cta_rank * share + t1) / 4 * BM + lane * 4 + j) * 4 + t1 % 4] = m1 != nullptr ? s1 * sum1[j] : 0.f;
+        }
     }
     epilogue_sync();
 }
@@ -1964,11 +1964,13 @@ int launch_grouped(cudaStream_t stream, const DeviceState &dev, int dtype, Param
 int64_t low_chunks(int64_t k) { return (k + LOW_CHUNK - 1) / LOW_CHUNK; }
 
 // Few rows, or requests of few rows each: the adapters' part costs no tile of its own and runs under the streaming of rhs, a
-// row at a time.  Otherwise every request of a tile costs the tensor cores' issuer half a microsecond, whatever its length.
-// 4096 x 4096, rank 16, this way against the other: 64 rows in 64 requests 19 against 46 us, in 4 requests 19 / 29; 256 rows
-// in 256 requests 48 / 95, in 16 requests 45 / 33; 512 rows in 512 requests 97 / 125, in 128 requests 91 / 62.
+// row at a time (0.05 to 0.15 us a row).  Otherwise every request of a tile costs the tensor cores' issuer about half a
+// microsecond, whatever its length, and every 32 ranks more of it as much again or less.  4096 x 4096, rank 16, this way
+// against the other: 64 rows in 64 requests 19 against 46 us, in 4 requests 19 / 29; 256 rows in 256 requests 48 / 95, in 16
+// requests 45 / 33; 512 rows in 512 requests 97 / 125, in 128 requests 91 / 62.
 bool few_rows(int64_t rows, int64_t rank, int64_t requests) {
-    return rank <= FEW_RANK && (rows <= 64 || (rows <= FEW_ROWS && rows < 4 * requests));
+    const int64_t blocks = (rank + RANK_BLOCK - 1) / RANK_BLOCK;
+    return rank <= FEW_RANK && (rows <= 64 || (rows <= FEW_ROWS && rows - 64 < requests * (1 + blocks)));
 }
 
 size_t lora_workspace(int64_t rows, int64_t k, int64_t rank) {
