@@ -8,8 +8,14 @@
 // Nothing is read back to the host: every CTA turns the offsets into a table of runs in shared memory (bounds are
 // clamped by a running maximum, so no offsets can lead out of the tensors) and walks the tiles that follow from it.
 //
-// Persistent CTAs of six warps: a TMA producer, an MMA issuer, four epilogue warps; a ring of shared-memory stages;
-// two accumulator buffers in tensor memory, so that a tile's epilogue runs under the next tile's products.
+// The kernels share a skeleton: persistent CTAs (or CTA pairs) of eleven warps, two that copy an operand each with TMA, one
+// that issues tcgen05.mma, eight that drain the accumulator; a ring of shared-memory stages; two accumulator buffers in
+// tensor memory, so that a tile's epilogue runs under the next tile's products.
+//   turned_kernel   the grouped product (matrix columns are the accumulator's rows), the adapters' first product, and the
+//                   whole of lora_matmul for few rows (with low_kernel before it)
+//   lora_kernel     lora_matmul for many rows
+//   grad_kernel     the gradient of the matrices
+//   *_plain_kernel  operands that no tensor map can address
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -29,19 +35,26 @@ constexpr int BK = 64;   // 64 16-bit elements: one 128-byte swizzle row
 constexpr int UMMA_K = 16;
 constexpr int A_STAGE_BYTES = BM * BK * 2;
 constexpr int A_CHUNK_ROWS = 32;  // short tiles load only the 32-row boxes that hold rows of theirs
-constexpr int NUM_THREADS = 192;
 constexpr int TMEM_COLS = 512;
 constexpr int MAX_STAGES = 8;
-constexpr int GROUP_ROWS = 16;  // tile-rows of 128 that share a raster group (L2 reuse of a run's weight panels)
+constexpr int GROUP_ROWS = 16;  // tile-rows of 128 that share a raster group (L2 reuse of a matrix's panels)
 constexpr int MAX_RUNS = 2048;  // the table of runs is 16 bytes a run of shared memory
-constexpr int SPLIT_NT = 64;     // rows of a tile whose reduction a cluster shares
-constexpr int FEW_ROWS = 1024;   // rows of a call whose adapters' part may be computed a row at a time (see few_rows)
-constexpr int FEW_RANK = 128;    // largest rank whose second product the epilogue of a few-row call computes
+constexpr size_t MAX_SMEM = 227 * 1024;
+
+// Warp 0 and the last copy, warp 1 issues the products, warps 2 to 9 are the epilogue (two a quadrant of the accumulator).
+constexpr int EPILOGUE_WARPS = 8;
+constexpr int ROW_WARP = 2 + EPILOGUE_WARPS;
+constexpr int NUM_THREADS = (ROW_WARP + 1) * 32;
+constexpr int GRAD_THREADS = NUM_THREADS + 32;  // and a warp that clears what a run's last block holds of the next run
+
+enum Job { JOB_PRODUCT, JOB_PARTS, JOB_FEW };  // of turned_kernel
+
+constexpr int SPLIT_NT = 64;   // rows of a tile whose reduction a cluster shares
+constexpr int FEW_ROWS = 1024;  // rows of a call whose adapters' part may be computed a row at a time (see few_rows)
+constexpr int FEW_RANK = 128;  // largest rank there
 constexpr int LOW_WARPS = 8;
 constexpr int LOW_CHUNK = LOW_WARPS * 256;  // terms of a partial sum of (lhs . down) there
-enum Job { JOB_PRODUCT, JOB_PARTS, JOB_FEW };
-
-constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product: 32 high parts, 32 low parts
+constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product elsewhere: 32 high parts, 32 low parts
 
 template <int CG, int BN>
 struct Shape {
@@ -106,9 +119,8 @@ struct Params {
     int n_tiles, k_blocks, group_m;
     int bf16;
     void *out;
-    int64_t out_stride0, out_stride1, out_batch_stride;
+    int64_t out_stride0, out_stride1;
     int out_vec;  // rows of output are 16-byte addressable
-    uint32_t b_lbo;
     // adapters
     const float *scales;
     int64_t scales_stride;
@@ -355,9 +367,8 @@ __device__ __forceinline__ void store_rows(const uint32_t (&acc)[32], void *out,
     }
 }
 
-// The bytes of A that a CTA loads for a tile whose rows from `row` on number `valid`, and the loads themselves: one
-// 128-row box, or as many 32-row boxes as hold rows of the tile.  Rows that no box brings keep what the stage held;
-// they only reach accumulator rows that are never stored.
+// How many 32-row boxes hold the `valid` rows that a CTA has of a tile.  Rows that no box brings keep what the stage held;
+// they only reach parts of the accumulator that are never stored.
 __device__ __forceinline__ int a_boxes(int valid) {
     return valid <= 0 ? 0 : min(BM / A_CHUNK_ROWS, (valid + A_CHUNK_ROWS - 1) / A_CHUNK_ROWS);
 }
@@ -399,12 +410,6 @@ struct Turned {
     static constexpr int STAGES = 192 * 1024 / STAGE_BYTES < MAX_STAGES ? 192 * 1024 / STAGE_BYTES : MAX_STAGES;
     static constexpr int TILE_N = BM * CG;
 };
-// Warp 0 copies the matrices, warp 1 issues the products, warps 2 to 9 are the epilogue (two a quadrant of the
-// accumulator, every other 32 rows each), warp 10 copies the rows.
-constexpr int EPILOGUE_WARPS = 8;
-constexpr int ROW_WARP = 2 + EPILOGUE_WARPS;
-constexpr int TURNED_THREADS = (ROW_WARP + 1) * 32;
-constexpr int GRAD_THREADS = TURNED_THREADS + 32;  // and a warp that clears what a run's last block holds of the next run
 constexpr int SPLIT_STAGES = 3;
 constexpr int SPLIT_BYTES = SPLIT_NT * BM * 4;  // partial sums: for every CTA of the cluster, its share of the rows
 
@@ -782,7 +787,7 @@ __device__ __forceinline__ void store_turned(const uint32_t (&acc)[32], void *ou
 // products run, compute the adapters' part of the rows that their CTA will store, (lhs . down) . up in fp32, and put it
 // where the CTA's own partial sums are added to it.
 template <int CG, int NT, bool W_MN, bool SPLIT, Job JOB>
-__global__ void __launch_bounds__(TURNED_THREADS, 1)
+__global__ void __launch_bounds__(NUM_THREADS, 1)
     turned_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                   const __grid_constant__ CUtensorMap map_x_chunk, const __grid_constant__ Params p) {
     using S = Turned<CG, NT>;
@@ -1087,7 +1092,7 @@ __global__ void __launch_bounds__(TURNED_THREADS, 1)
 // B_MN: rhs has unit stride along its columns; otherwise along its rows (a transposed view).
 // ---------------------------------------------------------------------------
 template <int CG, int BN, bool B_MN>
-__global__ void __launch_bounds__(TURNED_THREADS, 1)
+__global__ void __launch_bounds__(NUM_THREADS, 1)
     lora_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_chunk,
                 const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_low,
                 const __grid_constant__ CUtensorMap map_up, const __grid_constant__ Params p) {
@@ -1804,11 +1809,11 @@ int map_boxes(const DeviceState &dev, CUtensorMap *map, int dtype, const Matrice
 }
 
 template <typename Kernel>
-int active_pairs(Kernel kernel, const DeviceState &dev, size_t smem, int threads = NUM_THREADS) {
+int active_pairs(Kernel kernel, const DeviceState &dev, int threads) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(dev.sm_count / 2 * 2));
     config.blockDim = dim3(threads);
-    config.dynamicSmemBytes = smem;
+    config.dynamicSmemBytes = MAX_SMEM;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim = {2, 1, 1};
@@ -1826,8 +1831,6 @@ struct Maps {
     CUtensorMap a, a_chunk, b, low, up;
 };
 
-constexpr size_t MAX_SMEM = 227 * 1024;
-
 template <int CG, int BN, bool B_MN>
 int launch_lora_kernel(cudaStream_t stream, const DeviceState &dev, const Maps &maps, const Params &p, int64_t tiles) {
     auto kernel = lora_kernel<CG, BN, B_MN>;
@@ -1837,14 +1840,14 @@ int launch_lora_kernel(cudaStream_t stream, const DeviceState &dev, const Maps &
     static thread_local int pairs = 0;
     if (configured_device != dev.device) {
         NT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SMEM)));
-        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, MAX_SMEM, TURNED_THREADS);
+        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, NUM_THREADS);
         configured_device = dev.device;
     }
     const int workers = CG == 2 ? pairs : dev.sm_count;
     if (workers <= 0) return fail(NINETOOTHED_B200_ERR_DEVICE, "lora_matmul: no CTA pair fits this device");
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, workers) * CG));
-    config.blockDim = dim3(TURNED_THREADS);
+    config.blockDim = dim3(NUM_THREADS);
     config.dynamicSmemBytes = smem_bytes<CG, BN>(p.offsets.runs);
     config.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -1890,7 +1893,7 @@ int launch_turned_kernel(cudaStream_t stream, const DeviceState &dev, const CUte
     static thread_local int pairs = 0;
     if (configured_device != dev.device) {
         NT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SMEM)));
-        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, MAX_SMEM, TURNED_THREADS);
+        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, NUM_THREADS);
         configured_device = dev.device;
     }
     cudaLaunchConfig_t config = {};
@@ -1898,7 +1901,7 @@ int launch_turned_kernel(cudaStream_t stream, const DeviceState &dev, const CUte
     if (workers <= 0) return fail(NINETOOTHED_B200_ERR_DEVICE, "grouped matmul: no CTA pair fits this device");
     const int cluster = SPLIT ? p.split : CG;
     config.gridDim = dim3(static_cast<unsigned>(workers * cluster));
-    config.blockDim = dim3(TURNED_THREADS);
+    config.blockDim = dim3(NUM_THREADS);
     config.dynamicSmemBytes = turned_smem<CG, NT, SPLIT, JOB == JOB_FEW>(p.offsets.runs);
     config.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -2084,7 +2087,7 @@ int launch_grad(cudaStream_t stream, const DeviceState &dev, int dtype, const Ni
     static thread_local int pairs = 0;
     if (configured_device != dev.device) {
         NT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SMEM)));
-        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, MAX_SMEM, GRAD_THREADS);
+        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, GRAD_THREADS);
         configured_device = dev.device;
     }
     using S = Grad<CG, BN>;

@@ -295,8 +295,29 @@ def test_lora_matmul_transposed_views(turned):
         run_lora(lhs, rhs, down, up, scales, offsets, which)
 
 
+@pytest.mark.parametrize("turned", [(False, False), (False, True), (True, False), (True, True)])
+@pytest.mark.parametrize("k, n, rank", [(2056, 136, 24), (4104, 130, 20), (72, 264, 128), (264, 8, 8)])
+def test_lora_matmul_few_rows(k, n, rank, turned):
+    """Single rows under adapters, whose matrices lie either way round, in wider tensors, ragged in every size."""
+    lengths, adapters = [1] * 30 + [0, 5, 3], [i % 6 - 1 for i in range(33)]
+    lhs, rhs, down, up, scales, offsets, which = lora_inputs(lengths, adapters, k, n, rank, 4, torch.bfloat16, first=1)
+
+    def wider(t):  # the same values, rows eight-element aligned inside a wider tensor
+        box = torch.full((*t.shape[:-1], t.shape[-1] // 8 * 8 + 24), float("nan"), dtype=t.dtype, device="cuda")
+        box[..., 8:8 + t.shape[-1]] = t
+        return box[..., 8:8 + t.shape[-1]]
+
+    down = wider(down.transpose(1, 2)).transpose(1, 2) if turned[0] else wider(down)
+    up = wider(up.transpose(1, 2)).transpose(1, 2) if turned[1] else wider(up)
+    from ninetoothed_b200 import _capi
+
+    before = _capi.plain_launches()
+    run_lora(wider(lhs), wider(rhs), down, up, scales, offsets, which)
+    assert _capi.plain_launches() == before
+
+
 def test_lora_matmul_many_requests_and_wide_indices():
-    lengths = [i % 4 for i in range(2048)]
+    lengths = [i % 3 for i in range(2048)]
     args = lora_inputs(lengths, [(i * 7) % 40 - 2 for i in range(2048)], 128, 136, 16, 36, torch.float16)
     run_lora(*args[:5], args[5].long(), args[6].long())
 
@@ -309,6 +330,8 @@ def test_lora_matmul_on_sizes_no_tensor_map_addresses_and_without_adapters():
     args = lora_inputs([20, 3, 9], [1, -1, 0], 64, 72, 16, 2, torch.bfloat16)
     run_lora(args[0], args[1], args[2][:0], args[3][:0], args[4][:0], *args[5:])           # no adapters at all
     run_lora(args[0], args[1], args[2][..., :0], args[3][:, :0], *args[4:])                 # adapters of rank 0
+    args = lora_inputs([300, 100], [1, -1], 64, 72, 16, 2, torch.bfloat16)
+    run_lora(args[0], args[1], args[2][:0], args[3][:0], args[4][:0], *args[5:])
 
 
 def test_a_broken_adapter_stays_with_its_requests():
@@ -457,6 +480,34 @@ def test_two_streams_at_once():
                 ops.lora_matmul(*a, o)
     torch.cuda.synchronize()
     for got, expected in zip(outputs, alone):
+        assert torch.equal(got, expected)
+
+
+def test_different_products_on_two_streams_at_once():
+    """Products of CTA pairs and of single CTAs in flight together give what each gives alone."""
+    from ninetoothed_b200.torch_ops import ops
+
+    lhs, rhs, grad = normal(81, 2000, 264), normal(82, 4, 264, 1032), normal(83, 2000, 1032)
+    offsets, few = bounds_of([700, 300, 990, 5]), bounds_of([1, 0, 2, 3])
+    calls = [lambda o: ops.grouped_matmul(lhs, rhs, offsets, o[0]), lambda o: ops.grouped_matmul_rhs_grad(lhs, grad, offsets, o[1]),
+             lambda o: ops.grouped_matmul(lhs, rhs, few, o[2]), lambda o: ops.grouped_matmul_rhs_grad(lhs, grad, few, o[3])]
+
+    def outputs():
+        return [torch.zeros(2000, 1032, dtype=torch.bfloat16, device="cuda"), torch.zeros_like(rhs),
+                torch.zeros(2000, 1032, dtype=torch.bfloat16, device="cuda"), torch.zeros_like(rhs)]
+
+    alone, together = outputs(), outputs()
+    for call in calls:
+        call(alone)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for turn in range(8):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                for call in (calls[:2], calls[2:])[i]:
+                    call(together)
+    torch.cuda.synchronize()
+    for got, expected in zip(together, alone):
         assert torch.equal(got, expected)
 
 
