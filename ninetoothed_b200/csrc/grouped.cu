@@ -37,7 +37,6 @@ constexpr int A_STAGE_BYTES = BM * BK * 2;
 constexpr int A_CHUNK_ROWS = 32;  // short tiles load only the 32-row boxes that hold rows of theirs
 constexpr int TMEM_COLS = 512;
 constexpr int MAX_STAGES = 8;
-constexpr int GROUP_ROWS = 16;  // tile-rows of 128 that share a raster group (L2 reuse of a matrix's panels)
 constexpr int MAX_RUNS = 2048;  // the table of runs is 16 bytes a run of shared memory
 constexpr size_t MAX_SMEM = 227 * 1024;
 
@@ -55,15 +54,6 @@ constexpr int FEW_RANK = 128;  // largest rank there
 constexpr int LOW_WARPS = 8;
 constexpr int LOW_CHUNK = LOW_WARPS * 256;  // terms of a partial sum of (lhs . down) there
 constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product elsewhere: 32 high parts, 32 low parts
-
-template <int CG, int BN>
-struct Shape {
-    static constexpr int BN_CTA = BN / CG;
-    static constexpr int B_STAGE_BYTES = BN_CTA * BK * 2;
-    static constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
-    static constexpr int STAGES = 192 * 1024 / STAGE_BYTES < MAX_STAGES ? 192 * 1024 / STAGE_BYTES : MAX_STAGES;
-    static constexpr int TILE_M = BM * CG;
-};
 
 struct Control {
     uint64_t full[MAX_STAGES];
@@ -91,11 +81,6 @@ constexpr int CONTROL_BYTES = 384;
 static_assert(sizeof(Control) <= CONTROL_BYTES, "control block");
 
 constexpr size_t table_bytes(int runs) { return static_cast<size_t>(runs + 1) * sizeof(Run); }
-
-template <int CG, int BN>
-size_t smem_bytes(int runs) {
-    return 1024 + Shape<CG, BN>::STAGES * Shape<CG, BN>::STAGE_BYTES + CONTROL_BYTES + table_bytes(runs);
-}
 
 struct View {  // up to three dimensions; stride[0] is the matrix index's
     const void *data;
@@ -141,9 +126,11 @@ __device__ __forceinline__ int load_index(const void *data, int64_t stride, int 
     return static_cast<int>(v < low ? low : v > high ? high : v);
 }
 
-// Fills the table with the runs that have rows (and, where adapters are given, an adapter), in row order.  All
-// threads of the CTA call it; the table is complete after the next __syncthreads().  Bounds outside 0 .. rows are
-// clamped and a bound below an earlier one counts as that one, so that runs never overlap or leave the tensor.
+// Fills the table with the runs that have rows (and, where adapters are given, an adapter, unless ALL: then runs without one
+// have matrix -1), in row order.  All threads of the CTA call it; the table is complete after the next __syncthreads().
+// Bounds outside 0 .. rows are clamped and a bound below an earlier one counts as that one, so that runs never overlap or
+// leave the tensor.  tiles_before is in units of tiles, or with ALL in rows, of whole tiles all the same.
+template <bool ALL>
 __device__ __forceinline__ void build_table(const Params &p, Run *table, Control *ctl, int tile_m) {
     const int runs = p.offsets.runs;
     for (int i = threadIdx.x; i <= runs; i += blockDim.x) {
@@ -171,7 +158,8 @@ __device__ __forceinline__ void build_table(const Params &p, Run *table, Control
         end = max(end, bound);
         int begin = __shfl_up_sync(0xffffffffu, end, 1);
         if (lane == 0) begin = bound;
-        const bool kept = i < runs && end > begin && matrix >= 0 && matrix < p.matrices;
+        const bool valid = matrix >= 0 && matrix < p.matrices;
+        const bool kept = i < runs && end > begin && (ALL || valid);
         const unsigned votes = __ballot_sync(0xffffffffu, kept);
         const int own_tiles = kept ? (end - begin + tile_m - 1) / tile_m : 0;
         int before = own_tiles;
@@ -183,7 +171,8 @@ __device__ __forceinline__ void build_table(const Params &p, Run *table, Control
         if (kept) {
             // (at most entry `base + lane`; the bound of entry base + 32, still to be read as a next bound's
             // predecessor, is carried in `bound`)
-            table[count + __popc(votes & ((1u << lane) - 1))] = Run{begin, end, matrix, tiles + before - own_tiles};
+            table[count + __popc(votes & ((1u << lane) - 1))] =
+                Run{begin, end, valid ? matrix : -1, (tiles + before - own_tiles) * (ALL ? tile_m : 1)};
         }
         count += __popc(votes);
         tiles += __shfl_sync(0xffffffffu, before, 31);
@@ -258,47 +247,6 @@ __device__ __forceinline__ void raster(int tile, int m_tiles, int n_tiles, int g
     if (group & 1) n = n_tiles - 1 - n;  // odd groups walk back, starting on the panels the previous one ended on
 }
 
-// First run of the table that ends behind `row`.
-__device__ __forceinline__ int first_run_behind(const Run *table, int runs, int row) {
-    int low = 0, high = runs;
-    while (low < high) {
-        const int mid = (low + high) >> 1;
-        if (table[mid].end > row) high = mid;
-        else low = mid + 1;
-    }
-    return low;
-}
-
-__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
-
-// D[tmem] += A[smem] . B[smem] into some of the accumulator's rows only: the lanes set in `off` keep their values.
-template <int CG>
-__device__ __forceinline__ void umma_ss_lanes(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
-                                              const uint32_t (&off)[8]) {
-    if constexpr (CG == 1) {
-        asm volatile(
-            "{\n\t"
-            ".reg .pred p;\n\t"
-            "setp.ne.b32 p, 1, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t"
-            "}\n"
-            :
-            : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
-            : "memory");
-    } else {
-        asm volatile(
-            "{\n\t"
-            ".reg .pred p;\n\t"
-            "setp.ne.b32 p, 1, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t"
-            "}\n"
-            :
-            : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]),
-              "r"(off[4]), "r"(off[5]), "r"(off[6]), "r"(off[7])
-            : "memory");
-    }
-}
-
 __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
     uint32_t packed;
     if (bf16) {
@@ -323,54 +271,6 @@ __device__ __forceinline__ void store16(void *out, int64_t at, float v, bool bf1
 __device__ __forceinline__ float load16(const void *in, int64_t at, bool bf16) {
     return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(in)[at])
                 : __half2float(static_cast<const __half *>(in)[at]);
-}
-
-// 32 columns of 32 rows, a row a lane.  Two exchanges between lanes 1 and 2 away turn four lanes' 64-byte rows so that a
-// store's lanes write 64 neighbouring bytes of eight rows; a lane that stored its own row's 16 bytes 32 times over took
-// twice the time (128 MB of output: 41 against 71 us).
-__device__ __forceinline__ void store_rows(const uint32_t (&acc)[32], void *out, int64_t stride0, int64_t row0, int rows, int col0,
-                                           int n, bool bf16) {
-    const int lane = threadIdx.x & 31;
-    const bool odd1 = lane & 1, odd2 = lane & 2;
-    uint32_t v[4][4];  // v[i]: 16 bytes of the row
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i / 4][i % 4] = pack2(__uint_as_float(acc[2 * i]), __uint_as_float(acc[2 * i + 1]), bf16);
-#pragma unroll
-    for (int i = 0; i < 4; i += 2)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t other = __shfl_xor_sync(0xffffffffu, odd1 ? v[i][w] : v[i + 1][w], 1);
-            v[i][w] = odd1 ? other : v[i][w];
-            v[i + 1][w] = odd1 ? v[i + 1][w] : other;
-        }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t other = __shfl_xor_sync(0xffffffffu, odd2 ? v[i][w] : v[i + 2][w], 2);
-            v[i][w] = odd2 ? other : v[i][w];
-            v[i + 2][w] = odd2 ? v[i + 2][w] : other;
-        }
-    const int col = col0 + (lane & 3) * 8;  // v[i] is now the lane's quarter of row i of its four lanes'
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = (lane & ~3) + i;
-        if (row >= rows || col >= n) continue;
-        uint16_t *dst = static_cast<uint16_t *>(out) + (row0 + row) * stride0 + col;
-        if (col + 8 <= n) {
-            *reinterpret_cast<uint4 *>(dst) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 7; ++j)
-                if (col + j < n) dst[j] = static_cast<uint16_t>(v[i][j / 2] >> (16 * (j & 1)));
-        }
-    }
-}
-
-// How many 32-row boxes hold the `valid` rows that a CTA has of a tile.  Rows that no box brings keep what the stage held;
-// they only reach parts of the accumulator that are never stored.
-__device__ __forceinline__ int a_boxes(int valid) {
-    return valid <= 0 ? 0 : min(BM / A_CHUNK_ROWS, (valid + A_CHUNK_ROWS - 1) / A_CHUNK_ROWS);
 }
 
 // Producers run their loops as whole warps, so that addresses and coordinates stay in uniform registers, which is where
@@ -452,16 +352,17 @@ struct TurnedWalk {
         if constexpr (FEW) {  // all rows against one matrix
             const int n = tile % p.n_tiles, first = range_begin + tile / p.n_tiles * NT;
             return {first, min(NT, range_end - first), n * Turned<CG, NT>::TILE_N, 0};
+        } else {
+            while (run + 1 < runs && table[run + 1].tiles_before * p.n_tiles <= tile) ++run;
+            const Run r = table[run];
+            const int length = r.end - r.begin, tiles = (length + NT - 1) / NT;
+            constexpr int STEP = 16 * CG;
+            const int even = tiles == 1 ? length : (length + tiles - 1) / tiles;
+            const int share = (even + STEP - 1) / STEP * STEP;  // rows of a tile, in whole steps
+            int m, n;
+            raster(tile - r.tiles_before * p.n_tiles, tiles, p.n_tiles, p.group_m, m, n);
+            return {r.begin + m * share, min(share, length - m * share), n * Turned<CG, NT>::TILE_N, r.matrix};
         }
-        while (run + 1 < runs && table[run + 1].tiles_before * p.n_tiles <= tile) ++run;
-        const Run r = table[run];
-        const int length = r.end - r.begin, tiles = (length + NT - 1) / NT;
-        constexpr int STEP = 16 * CG;
-        const int even = tiles == 1 ? length : (length + tiles - 1) / tiles;
-        const int share = (even + STEP - 1) / STEP * STEP;  // rows of a tile, in whole steps
-        int m, n;
-        raster(tile - r.tiles_before * p.n_tiles, tiles, p.n_tiles, p.group_m, m, n);
-        return {r.begin + m * share, min(share, length - m * share), n * Turned<CG, NT>::TILE_N, r.matrix};
     }
 };
 
@@ -738,8 +639,9 @@ __global__ void __launch_bounds__(LOW_WARPS * 32) low_kernel(const __grid_consta
 // 32 rows of a turned accumulator: lane l holds column n of all of them and the warp's 32 columns are neighbours.  Three
 // exchanges with the lanes 1, 2 and 4 away leave every lane with eight neighbouring columns of every eighth row, which
 // are 16-byte stores.  (One 2-byte store a row and lane took 80 cycles a row: more than the products of 2048 terms.)
-__device__ __forceinline__ void store_turned(const uint32_t (&acc)[32], void *out, int64_t stride0, int64_t row0, int rows, int n,
-                                             int n_end, bool bf16) {
+// The first sixteen columns of the accumulator are rows from row0 on, `rows0` of them, the others from row1 on.
+__device__ __forceinline__ void store_turned(const uint32_t (&acc)[32], void *out, int64_t stride0, int64_t row0, int rows0,
+                                             int64_t row1, int rows1, int n, int n_end, bool bf16) {
     const int lane = threadIdx.x & 31;
     const bool odd1 = lane & 1, odd2 = lane & 2, odd4 = lane & 4;
     uint32_t pair[16];  // two columns of row 2i + (lane & 1)
@@ -765,9 +667,9 @@ __device__ __forceinline__ void store_turned(const uint32_t (&acc)[32], void *ou
         v.y = odd4 ? other1 : four[2 * i][1];
         v.z = odd4 ? four[2 * i + 1][0] : other0;
         v.w = odd4 ? four[2 * i + 1][1] : other1;
-        const int row = 8 * i + (lane & 7);
-        if (row < rows && col < n_end) {
-            uint16_t *dst = static_cast<uint16_t *>(out) + (row0 + row) * stride0 + col;
+        const int row = 8 * (i & 1) + (lane & 7);
+        if (row < (i < 2 ? rows0 : rows1) && col < n_end) {
+            uint16_t *dst = static_cast<uint16_t *>(out) + ((i < 2 ? row0 : row1) + row) * stride0 + col;
             if (col + 8 <= n_end) {
                 *reinterpret_cast<uint4 *>(dst) = v;
             } else {
@@ -832,7 +734,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tmem_relinquish<CG>();
     }
     if constexpr (FEW) build_range(p, ctl);
-    else build_table(p, table, ctl, NT);
+    else build_table<false>(p, table, ctl, NT);
     tcgen05_fence_before_sync();
     __syncthreads();
     if constexpr (CG == 2) cluster_sync();
@@ -855,7 +757,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             const int row0 = at.row0 + (CG == 1 ? 0 : static_cast<int>(cta_rank) * width_cta);
             const int n0 = at.col0 + (CG == 1 ? 0 : static_cast<int>(cta_rank) * BM);
             const int boxes = (width_cta + A_CHUNK_ROWS - 1) / A_CHUNK_ROWS;
-            const int bytes = CG * (S::W_BYTES + S::SUB * boxes * (A_CHUNK_ROWS * BK * 2));
+            // (64-column boxes wholly behind the matrix, as half of the tile is where down has few ranks, are not copied)
+            const int w_boxes = W_MN ? min(BM / 64, max(0, (p.n - n0 + 63) / 64)) : BM / 64;
+            const int w_boxes_other = CG == 1 ? 0 : W_MN ? min(BM / 64, max(0, (p.n - n0 - BM + 63) / 64)) : BM / 64;
+            const int bytes = (w_boxes + w_boxes_other) * (S::W_BYTES / (BM / 64)) + CG * S::SUB * boxes * (A_CHUNK_ROWS * BK * 2);
             for (int kb = kb_first; kb < kb_last; ++kb) {
                 mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x100 | s);
                 uint8_t *w_dst = smem + s * S::STAGE_BYTES;
@@ -870,7 +775,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                     if constexpr (W_MN) {
 #pragma unroll
                         for (int j = 0; j < BM / 64; ++j)
-                            load_3d<CG>(w_dst + j * (S::DEPTH * 128), &map_w, &ctl->full[s], n0 + j * 64, kb * S::DEPTH, at.matrix);
+                            if (j < w_boxes)
+                                load_3d<CG>(w_dst + j * (S::DEPTH * 128), &map_w, &ctl->full[s], n0 + j * 64, kb * S::DEPTH, at.matrix);
                     } else {
 #pragma unroll
                         for (int sub = 0; sub < S::SUB; ++sub)
@@ -1006,11 +912,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                             low_part[j] = __float_as_uint(isfinite(high) ? v - high : 0.f);
                         }
                         uint16_t *block = static_cast<uint16_t *>(p.out) + n / 32 * 32;
-                        store_turned(acc, block, p.out_stride0, at.row0 + t0, at.rows - t0, n, n_end, bf16);
-                        store_turned(low_part, block + 32, p.out_stride0, at.row0 + t0, at.rows - t0, n, n_end, bf16);
+                        store_turned(acc, block, p.out_stride0, at.row0 + t0, at.rows - t0, at.row0 + t0 + 16, at.rows - t0 - 16, n, n_end, bf16);
+                        store_turned(low_part, block + 32, p.out_stride0, at.row0 + t0, at.rows - t0, at.row0 + t0 + 16, at.rows - t0 - 16, n, n_end, bf16);
                     }
                 } else if (p.out_vec) {
-                    store_turned(acc, p.out, p.out_stride0, at.row0 + t0, at.rows - t0, n, p.n, bf16);
+                    store_turned(acc, p.out, p.out_stride0, at.row0 + t0, at.rows - t0, at.row0 + t0 + 16, at.rows - t0 - 16, n, p.n, bf16);
                 } else if (n < p.n) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
@@ -1086,18 +992,41 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 }
 
 // ---------------------------------------------------------------------------
-// The shared projection with adapters beside it, for many rows: tiles of the projection (rows of lhs are the accumulator's
-// rows), then for every request in the tile the second product of its adapter, 32 ranks a stage, into that request's
-// accumulator rows only.  (scales lhs . down comes in two 16-bit parts from the launch before.)
-// B_MN: rhs has unit stride along its columns; otherwise along its rows (a transposed view).
+// The shared projection with adapters beside it, for many rows, with the operands exchanged as in turned_kernel.  The rows
+// stand in a padded space of accumulator columns in which every request starts at a multiple of 16; a tile is NT columns of
+// it, whatever requests they belong to, against 128 (256) columns of rhs.  Then, for every request with an adapter that has
+// columns in the tile, its second product is an ordinary product into just these columns, 32 ranks a stage: nothing of one
+// request's adapter, infinities and NaN included, meets another's columns.  (scales lhs . down comes in two 16-bit parts from
+// the launch before.)
 // ---------------------------------------------------------------------------
-template <int CG, int BN, bool B_MN>
+// The columns [from, to) of the padded space that a run of the table (tiles_before: its first column) has in [low, high).
+struct Piece {
+    int from, to;
+    __device__ Piece(const Run &run, int low, int high)
+        : from(max(run.tiles_before, low)), to(min(run.tiles_before + (run.end - run.begin + 15) / 16 * 16, high)) {}
+    __device__ int row(const Run &run) const { return run.begin + from - run.tiles_before; }
+};
+
+// The run that holds a column.
+__device__ __forceinline__ int run_at(const Run *table, int runs, int column) {
+    int low = 0, high = runs - 1;
+    while (low < high) {
+        const int mid = (low + high + 1) >> 1;
+        if (table[mid].tiles_before <= column) low = mid;
+        else high = mid - 1;
+    }
+    return low;
+}
+
+template <int CG, int NT, bool W_MN>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-    lora_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_chunk,
-                const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_low,
-                const __grid_constant__ CUtensorMap map_up, const __grid_constant__ Params p) {
-    using S = Shape<CG, BN>;
+    lora_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                const __grid_constant__ CUtensorMap map_x32, const __grid_constant__ CUtensorMap map_x16,
+                const __grid_constant__ CUtensorMap map_low, const __grid_constant__ CUtensorMap map_up,
+                const __grid_constant__ Params p) {
+    using S = Turned<CG, NT>;
     constexpr int STAGES = S::STAGES;
+    constexpr int ROW_BYTES = BK * 2;  // of one row in a 64-deep block
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Control *ctl = reinterpret_cast<Control *>(smem + STAGES * S::STAGE_BYTES);
@@ -1108,8 +1037,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const WaitCtx wait_ctx{&ctl->abort_flag, p.status, KID_GROUPED};
     const uint32_t cta_rank = CG == 1 ? 0u : cluster_cta_rank();
     const bool leader = cta_rank == 0;
-    const int worker = blockIdx.x / CG;
-    const int workers = gridDim.x / CG;
+    const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -1122,23 +1050,81 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         ctl->abort_flag = 0;
         mbar_fence_init();
-        tma_prefetch_desc(&map_a);
-        tma_prefetch_desc(&map_b);
+        tma_prefetch_desc(&map_w);
+        tma_prefetch_desc(&map_x);
+        tma_prefetch_desc(&map_low);
+        tma_prefetch_desc(&map_up);
     }
     if (warp == 1) {
         tmem_alloc<CG>(&ctl->tmem_base, TMEM_COLS);
         tmem_relinquish<CG>();
     }
-    build_table(p, table, ctl, S::TILE_M);
+    build_table<true>(p, table, ctl, 16);
     tcgen05_fence_before_sync();
     __syncthreads();
     if constexpr (CG == 2) cluster_sync();
     tcgen05_fence_after_sync();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
-    const int begin = ctl->row_begin, end = ctl->row_end, runs = ctl->runs;
-    const int m_tiles = (end - begin + S::TILE_M - 1) / S::TILE_M, total = m_tiles * p.n_tiles;
+    const int runs = ctl->runs, columns = ctl->tiles_m * 16;  // of the padded space
+    const int m_tiles = (columns + NT - 1) / NT, total = m_tiles * p.n_tiles;
+    constexpr int STEP = 16 * CG;
 
     if (warp == 0) {
+        // ------------------- TMA producer of the matrices, rhs and up -------------------
+        const bool issuer = elect_one();
+        uint32_t s = 0, phase = 1;
+        const auto next = [&] {
+            if (++s == STAGES) {
+                s = 0;
+                phase ^= 1;
+            }
+        };
+        const int up_bytes = p.up_mn ? BM * RANK_BLOCK * 2 : A_STAGE_BYTES;
+        for (int tile = worker; tile < total; tile += workers) {
+            int m, n;
+            raster(tile, m_tiles, p.n_tiles, p.group_m, m, n);
+            const int first = m * NT, last = min(first + NT, columns);
+            const int n0 = n * S::TILE_N + static_cast<int>(cta_rank) * BM;
+            // (the even CTA's barriers count the bytes of both)
+            const int bytes = CG * S::W_BYTES + S::SUB * (last - first) * ROW_BYTES;
+            for (int kb = 0; kb < p.k_blocks; ++kb) {
+                mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x100 | s);
+                uint8_t *dst = smem + s * S::STAGE_BYTES;
+                if (issuer) {
+                    if (leader) mbar_expect_tx(&ctl->full[s], bytes);
+                    if constexpr (W_MN) {
+#pragma unroll
+                        for (int j = 0; j < BM / 64; ++j)
+                            load_3d<CG>(dst + j * (S::DEPTH * 128), &map_w, &ctl->full[s], n0 + j * 64, kb * S::DEPTH, 0);
+                    } else {
+#pragma unroll
+                        for (int sub = 0; sub < S::SUB; ++sub)
+                            load_3d<CG>(dst + sub * A_STAGE_BYTES, &map_w, &ctl->full[s], kb * S::DEPTH + sub * BK, n0, 0);
+                    }
+                }
+                next();
+            }
+            for (int r = run_at(table, runs, first); r < runs && table[r].tiles_before < last; ++r) {
+                const int matrix = table[r].matrix;
+                if (matrix < 0) continue;
+                for (int rb = 0; rb < p.rank_blocks; ++rb) {
+                    mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x110 | s);
+                    uint8_t *dst = smem + s * S::STAGE_BYTES;
+                    if (issuer) {
+                        if (leader) mbar_expect_tx(&ctl->full[s], CG * (up_bytes + S::X_BYTES));
+                        if (p.up_mn) {
+#pragma unroll
+                            for (int j = 0; j < BM / 64; ++j)
+                                load_3d<CG>(dst + j * (RANK_BLOCK * 128), &map_up, &ctl->full[s], n0 + j * 64, rb * RANK_BLOCK, matrix);
+                        } else {
+                            load_3d<CG>(dst, &map_up, &ctl->full[s], rb * RANK_BLOCK, n0, matrix);
+                        }
+                    }
+                    next();
+                }
+            }
+        }
+    } else if (warp == ROW_WARP) {
         // --------------- TMA producer of the rows, of lhs and of (scales lhs . down) ---------------
         const bool issuer = elect_one();
         uint32_t s = 0, phase = 1;
@@ -1151,170 +1137,123 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         for (int tile = worker; tile < total; tile += workers) {
             int m, n;
             raster(tile, m_tiles, p.n_tiles, p.group_m, m, n);
-            const int row0 = begin + m * S::TILE_M, tile_end = min(end, row0 + S::TILE_M);
-            const int m0 = row0 + static_cast<int>(cta_rank) * BM;
-            const int boxes = a_boxes(tile_end - m0);
-            // the even CTA's barrier counts the bytes of both
-            int bytes = boxes * (A_CHUNK_ROWS * BK * 2) + S::B_STAGE_BYTES;
-            if constexpr (CG == 2) bytes += a_boxes(tile_end - m0 - BM) * (A_CHUNK_ROWS * BK * 2) + S::B_STAGE_BYTES;
-            for (int kb = 0; kb < p.k_blocks; ++kb) {
-                mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x100 | s);
-                uint8_t *dst = smem + s * S::STAGE_BYTES;
-                if (issuer) {
-                    if (leader) mbar_expect_tx(&ctl->full[s], bytes);
-                    if (boxes == BM / A_CHUNK_ROWS) {
-                        load_2d<CG>(dst, &map_a, &ctl->full[s], kb * BK, m0);
-                    } else {
-                        for (int c = 0; c < boxes; ++c)
-                            load_2d<CG>(dst + c * (A_CHUNK_ROWS * BK * 2), &map_a_chunk, &ctl->full[s], kb * BK, m0 + c * A_CHUNK_ROWS);
-                    }
-                }
-                next();
-            }
-            const int b_bytes = p.up_mn ? S::BN_CTA * RANK_BLOCK * 2 : S::B_STAGE_BYTES;
-            for (int r = first_run_behind(table, runs, row0); r < runs && table[r].begin < tile_end; ++r) {
-                // 32-row boxes of a CTA's rows that hold rows of the run
-                const int run_begin = table[r].begin, run_end = min(table[r].end, tile_end);
-                const auto box_range = [&](int base, int &first, int &last) {
-                    first = max(run_begin - base, 0) / A_CHUNK_ROWS;
-                    last = run_end <= base ? 0 : min((run_end - base + A_CHUNK_ROWS - 1) / A_CHUNK_ROWS, BM / A_CHUNK_ROWS);
-                    last = max(first, last);
-                };
-                int first, last, first_other = 0, last_other = 0;
-                box_range(m0, first, last);
-                if constexpr (CG == 2) box_range(row0 + BM, first_other, last_other);
-                int ext_bytes = (last - first) * (A_CHUNK_ROWS * BK * 2) + b_bytes;
-                if constexpr (CG == 2) ext_bytes += (last_other - first_other) * (A_CHUNK_ROWS * BK * 2) + b_bytes;
-                for (int rb = 0; rb < p.rank_blocks; ++rb) {
-                    mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x110 | s);
-                    uint8_t *dst = smem + s * S::STAGE_BYTES;
-                    if (issuer) {
-                        if (leader) mbar_expect_tx(&ctl->full[s], ext_bytes);
-                        for (int c = first; c < last; ++c)
-                            load_2d<CG>(dst + c * (A_CHUNK_ROWS * BK * 2), &map_low, &ctl->full[s], rb * BK, m0 + c * A_CHUNK_ROWS);
-                    }
-                    next();
-                }
-            }
-        }
-    } else if (warp == ROW_WARP) {
-        // -------------------- TMA producer of the matrices, rhs and up --------------------
-        const bool issuer = elect_one();
-        uint32_t s = 0, phase = 1;
-        const auto next = [&] {
-            if (++s == STAGES) {
-                s = 0;
-                phase ^= 1;
-            }
-        };
-        for (int tile = worker; tile < total; tile += workers) {
-            int m, n;
-            raster(tile, m_tiles, p.n_tiles, p.group_m, m, n);
-            const int row0 = begin + m * S::TILE_M, tile_end = min(end, row0 + S::TILE_M);
-            const int n0 = n * BN + static_cast<int>(cta_rank) * S::BN_CTA;
+            const int first = m * NT, last = min(first + NT, columns);
+            // this CTA's columns: half of the tile's for one of a pair
+            const int width_cta = (last - first + STEP - 1) / STEP * 16;
+            const int mine = first + static_cast<int>(cta_rank) * width_cta, mine_end = min(mine + width_cta, last);
+            const int run_first = run_at(table, runs, first), run_mine = run_at(table, runs, mine);
             for (int kb = 0; kb < p.k_blocks; ++kb) {
                 mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x120 | s);
-                uint8_t *dst = smem + s * S::STAGE_BYTES + A_STAGE_BYTES;
-                if (issuer) {
-                    if constexpr (B_MN) {
+                uint8_t *dst = smem + s * S::STAGE_BYTES + S::W_BYTES;
+                for (int r = run_mine; r < runs && table[r].tiles_before < mine_end; ++r) {
+                    const Piece piece(table[r], mine, mine_end);
+                    const int row = piece.row(table[r]), count = piece.to - piece.from;
+                    if (issuer) {
 #pragma unroll
-                        for (int j = 0; j < S::BN_CTA / 64; ++j)
-                            load_3d<CG>(dst + j * (BK * 128), &map_b, &ctl->full[s], n0 + j * 64, kb * BK, 0);
-                    } else {
-                        load_3d<CG>(dst, &map_b, &ctl->full[s], kb * BK, n0, 0);
+                        for (int sub = 0; sub < S::SUB; ++sub) {
+                            uint8_t *at = dst + sub * S::X_BYTES + (piece.from - mine) * ROW_BYTES;
+                            const int k0 = kb * S::DEPTH + sub * BK;
+                            if (count == S::ROWS_CTA) {
+                                load_2d<CG>(at, &map_x, &ctl->full[s], k0, row);
+                            } else {
+                                int c = 0;
+                                for (; c + 32 <= count; c += 32)
+                                    load_2d<CG>(at + c * ROW_BYTES, &map_x32, &ctl->full[s], k0, row + c);
+                                if (c < count) load_2d<CG>(at + c * ROW_BYTES, &map_x16, &ctl->full[s], k0, row + c);
+                            }
+                        }
                     }
+                    __syncwarp();
                 }
                 next();
             }
-            for (int r = first_run_behind(table, runs, row0); r < runs && table[r].begin < tile_end; ++r) {
-                const int matrix = table[r].matrix;
+            for (int r = run_first; r < runs && table[r].tiles_before < last; ++r) {
+                if (table[r].matrix < 0) continue;
+                const Piece piece(table[r], first, last);
+                // a pair's CTAs bring half of the piece each (and what follows it, unused)
+                const int row = piece.row(table[r]) + static_cast<int>(cta_rank) * ((piece.to - piece.from) / CG);
                 for (int rb = 0; rb < p.rank_blocks; ++rb) {
                     mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x130 | s);
-                    uint8_t *dst = smem + s * S::STAGE_BYTES + A_STAGE_BYTES;
-                    if (issuer) {
-                        if (p.up_mn) {
-#pragma unroll
-                            for (int j = 0; j < S::BN_CTA / 64; ++j)
-                                load_3d<CG>(dst + j * (RANK_BLOCK * 128), &map_up, &ctl->full[s], n0 + j * 64, rb * RANK_BLOCK, matrix);
-                        } else {
-                            load_3d<CG>(dst, &map_up, &ctl->full[s], rb * RANK_BLOCK, n0, matrix);
-                        }
-                    }
+                    uint8_t *dst = smem + s * S::STAGE_BYTES + S::W_BYTES;
+                    if (issuer) load_2d<CG>(dst, &map_low, &ctl->full[s], rb * BK, row);
                     next();
                 }
             }
         }
     } else if (warp == 1) {
         // ------------------------------- MMA issuer -------------------------------
-        // The warp runs the loop as one (the instruction takes uniform registers); an elected lane issues.
         if (leader) {
-            const uint32_t idesc = umma_instr_desc(BM * CG, BN, p.bf16 != 0, false, B_MN);
-            const uint32_t idesc_up = umma_instr_desc(BM * CG, BN, p.bf16 != 0, false, p.up_mn != 0);
-            const uint32_t up_step = p.up_mn ? UMMA_K * 128 : UMMA_K * 2, up_lbo = p.up_mn ? RANK_BLOCK * 128 : 16;
             const bool issuer = elect_one();
             const uint32_t smem_base = smem_u32(smem);
+            const uint32_t up_step = p.up_mn ? UMMA_K * 128 : UMMA_K * 2, up_lbo = p.up_mn ? RANK_BLOCK * 128 : 16;
             uint32_t s = 0, phase = 0, acc_it = 0;
             bool ready = false;
             for (int tile = worker; tile < total; tile += workers, ++acc_it) {
                 int m, n;
                 raster(tile, m_tiles, p.n_tiles, p.group_m, m, n);
-                const int row0 = begin + m * S::TILE_M, tile_end = min(end, row0 + S::TILE_M);
+                const int first = m * NT, last = min(first + NT, columns);
+                const uint32_t idesc = umma_instr_desc(BM * CG, (last - first + STEP - 1) / STEP * STEP, p.bf16 != 0, W_MN, false);
                 const uint32_t buf = acc_it & 1;
                 mbar_wait_warp(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
                 tcgen05_fence_after_sync();
-                const uint32_t tmem_acc = tmem_base + buf * BN;
+                const uint32_t tmem_acc = tmem_base + buf * NT;
                 for (int kb = 0; kb < p.k_blocks; ++kb) {
                     if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x300 | s);
                     tcgen05_fence_after_sync();
-                    const uint32_t a_addr = smem_base + s * S::STAGE_BYTES;
-                    const uint32_t b_addr = a_addr + A_STAGE_BYTES;
+                    const uint32_t w_addr = smem_base + s * S::STAGE_BYTES;
+                    const uint32_t x_addr = w_addr + S::W_BYTES;
                     const uint32_t s_next = s + 1 == STAGES ? 0 : s + 1;
                     const uint32_t phase_next = s_next == 0 ? phase ^ 1 : phase;
 #pragma unroll
-                    for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-                        const uint64_t desc_a = umma_smem_desc(a_addr + kk * (UMMA_K * 2), 16, 1024);
-                        const uint64_t desc_b =
-                            umma_smem_desc(b_addr + kk * (B_MN ? UMMA_K * 128 : UMMA_K * 2), B_MN ? BK * 128 : 16, 1024);
-                        if (issuer) umma_ss<CG>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
-                        if (kk == BK / UMMA_K / 2 - 1)  // (a probe between MMAs costs nothing, a wait after them does)
+                    for (int kk = 0; kk < S::DEPTH / UMMA_K; ++kk) {
+                        const int sub = kk / (BK / UMMA_K), step = kk % (BK / UMMA_K);
+                        const uint64_t desc_w =
+                            W_MN ? umma_smem_desc(w_addr + kk * (UMMA_K * 128), S::DEPTH * 128, 1024)
+                                 : umma_smem_desc(w_addr + sub * A_STAGE_BYTES + step * (UMMA_K * 2), 16, 1024);
+                        const uint64_t desc_x = umma_smem_desc(x_addr + sub * S::X_BYTES + step * (UMMA_K * 2), 16, 1024);
+                        if (issuer) umma_ss<CG>(tmem_acc, desc_w, desc_x, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
+                        if (kk == S::DEPTH / UMMA_K / 2 - 1)
                             ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
                     }
                     if (issuer) {
                         if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
                         else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
                     }
+                    __syncwarp();
                     s = s_next;
                     phase = phase_next;
                 }
-                for (int r = first_run_behind(table, runs, row0); r < runs && table[r].begin < tile_end; ++r) {
-                    // Only the accumulator rows of this run take part: what another run's adapter holds, infinities and
-                    // NaN included, cannot reach them.
-                    const int low = table[r].begin - row0, high = min(table[r].end, tile_end) - row0;
-                    uint32_t off[8];
-#pragma unroll
-                    for (int w = 0; w < 8; ++w) off[w] = ~(low_bits(high - 32 * w) & ~low_bits(low - 32 * w));
+                for (int r = run_at(table, runs, first); r < runs && table[r].tiles_before < last; ++r) {
+                    if (table[r].matrix < 0) continue;
+                    const Piece piece(table[r], first, last);
+                    const uint32_t idesc_up = umma_instr_desc(BM * CG, piece.to - piece.from, p.bf16 != 0, p.up_mn != 0, false);
+                    const uint32_t tmem_piece = tmem_acc + (piece.from - first);
                     for (int rb = 0; rb < p.rank_blocks; ++rb) {
                         if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x310 | s);
-                        ready = false;
                         tcgen05_fence_after_sync();
-                        const uint32_t a_addr = smem_base + s * S::STAGE_BYTES;
-                        const uint32_t b_addr = a_addr + A_STAGE_BYTES;
-                        const int steps = (min(RANK_BLOCK, p.rank - rb * RANK_BLOCK) + UMMA_K - 1) / UMMA_K;
-                        for (int kk = 0; kk < steps; ++kk) {
-                            const uint64_t desc_b = umma_smem_desc(b_addr + kk * up_step, up_lbo, 1024);
+                        const uint32_t up_addr = smem_base + s * S::STAGE_BYTES;
+                        const uint32_t low_addr = up_addr + S::W_BYTES;
+                        const uint32_t s_next = s + 1 == STAGES ? 0 : s + 1;
+                        const uint32_t phase_next = s_next == 0 ? phase ^ 1 : phase;
+                        const bool two = p.rank - rb * RANK_BLOCK > UMMA_K;  // steps of 16 ranks
+#pragma unroll
+                        for (int kk = 0; kk < RANK_BLOCK / UMMA_K; ++kk) {
+                            const uint64_t desc_up = umma_smem_desc(up_addr + kk * up_step, up_lbo, 1024);
 #pragma unroll
                             for (int part = 0; part < 2; ++part) {
-                                const uint64_t desc_a =
-                                    umma_smem_desc(a_addr + part * (RANK_BLOCK * 2) + kk * (UMMA_K * 2), 16, 1024);
-                                if (issuer) umma_ss_lanes<CG>(tmem_acc, desc_a, desc_b, idesc_up, off);
+                                const uint64_t desc_low =
+                                    umma_smem_desc(low_addr + part * (RANK_BLOCK * 2) + kk * (UMMA_K * 2), 16, 1024);
+                                if (issuer && (kk == 0 || two)) umma_ss<CG>(tmem_piece, desc_up, desc_low, idesc_up, 1u);
                             }
                         }
+                        ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
                         if (issuer) {
                             if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
                             else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
                         }
-                        s = s + 1 == STAGES ? 0 : s + 1;
-                        if (s == 0) phase ^= 1;
+                        __syncwarp();
+                        s = s_next;
+                        phase = phase_next;
                     }
                 }
                 if (issuer) {
@@ -1330,26 +1269,37 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const bool bf16 = p.bf16 != 0;
         uint32_t acc_it = 0;
         for (int tile = worker; tile < total; tile += workers, ++acc_it) {
-            int m, n;
-            raster(tile, m_tiles, p.n_tiles, p.group_m, m, n);
-            const int row0 = begin + m * S::TILE_M + static_cast<int>(cta_rank) * BM + quadrant * 32, n0 = n * BN;
+            int m, n_tile;
+            raster(tile, m_tiles, p.n_tiles, p.group_m, m, n_tile);
+            const int first = m * NT, last = min(first + NT, columns);
+            const int n = n_tile * S::TILE_N + static_cast<int>(cta_rank) * BM + quadrant * 32 + lane;
             const uint32_t buf = acc_it & 1;
+            int r = run_at(table, runs, first + 32 * half);
             mbar_wait(&ctl->tmem_full[buf], (acc_it >> 1) & 1, wait_ctx, 0x400 | buf);
             tcgen05_fence_after_sync();
-            const uint32_t taddr = tmem_base + buf * BN + (static_cast<uint32_t>(quadrant * 32) << 16);
+            const uint32_t taddr = tmem_base + buf * NT + (static_cast<uint32_t>(quadrant * 32) << 16);
 #pragma unroll 1
-            for (int col = 32 * half; col < BN && n0 + col < p.n && row0 < end; col += 64) {
+            for (int c0 = first + 32 * half; c0 < last; c0 += 64) {
                 uint32_t acc[32];
                 __syncwarp();
-                tmem_ld_32x32(taddr + col, acc);
+                tmem_ld_32x32(taddr + (c0 - first), acc);
                 tmem_wait_ld();
+                // two times sixteen columns, each of one request: their first rows, and how many are rows
+                int row[2], rows[2];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const int c = c0 + 16 * g;
+                    while (r + 1 < runs && table[r + 1].tiles_before <= c) ++r;
+                    row[g] = table[r].begin + c - table[r].tiles_before;
+                    rows[g] = c < last ? min(16, table[r].end - row[g]) : 0;
+                }
                 if (p.out_vec) {
-                    store_rows(acc, p.out, p.out_stride0, row0, end - row0, n0 + col, p.n, bf16);
-                } else if (row0 + lane < end) {
+                    store_turned(acc, p.out, p.out_stride0, row[0], rows[0], row[1], rows[1], n, p.n, bf16);
+                } else if (n < p.n) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
-                        if (n0 + col + j < p.n)
-                            store16(p.out, (row0 + lane) * p.out_stride0 + (n0 + col + j) * p.out_stride1, __uint_as_float(acc[j]), bf16);
+                        if (j % 16 < rows[j / 16])
+                            store16(p.out, (row[j / 16] + j % 16) * p.out_stride0 + n * p.out_stride1, __uint_as_float(acc[j]), bf16);
                 }
             }
             tcgen05_fence_before_sync();
@@ -1827,15 +1777,14 @@ int active_pairs(Kernel kernel, const DeviceState &dev, int threads) {
     return clusters;
 }
 
-struct Maps {
-    CUtensorMap a, a_chunk, b, low, up;
+struct LoraMaps {
+    CUtensorMap w, x, x32, x16, low, up;
 };
 
-template <int CG, int BN, bool B_MN>
-int launch_lora_kernel(cudaStream_t stream, const DeviceState &dev, const Maps &maps, const Params &p, int64_t tiles) {
-    auto kernel = lora_kernel<CG, BN, B_MN>;
-    static_assert(1024 + Shape<CG, BN>::STAGES * Shape<CG, BN>::STAGE_BYTES + CONTROL_BYTES + table_bytes(MAX_RUNS) <= MAX_SMEM,
-                  "shared memory per CTA");
+template <int CG, int NT, bool W_MN>
+int launch_lora_kernel(cudaStream_t stream, const DeviceState &dev, const LoraMaps &maps, const Params &p, int64_t most_tiles) {
+    auto kernel = lora_kernel<CG, NT, W_MN>;
+    static_assert(turned_smem<CG, NT, false, false>(MAX_RUNS) <= MAX_SMEM, "shared memory per CTA");
     static thread_local int configured_device = -1;
     static thread_local int pairs = 0;
     if (configured_device != dev.device) {
@@ -1846,9 +1795,9 @@ int launch_lora_kernel(cudaStream_t stream, const DeviceState &dev, const Maps &
     const int workers = CG == 2 ? pairs : dev.sm_count;
     if (workers <= 0) return fail(NINETOOTHED_B200_ERR_DEVICE, "lora_matmul: no CTA pair fits this device");
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, workers) * CG));
+    config.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(most_tiles, workers) * CG));
     config.blockDim = dim3(NUM_THREADS);
-    config.dynamicSmemBytes = smem_bytes<CG, BN>(p.offsets.runs);
+    config.dynamicSmemBytes = turned_smem<CG, NT, false, false>(p.offsets.runs);
     config.stream = stream;
     cudaLaunchAttribute attr[1];
     if (CG == 2) {
@@ -1857,31 +1806,35 @@ int launch_lora_kernel(cudaStream_t stream, const DeviceState &dev, const Maps &
         config.attrs = attr;
         config.numAttrs = 1;
     }
-    NT_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, maps.a, maps.a_chunk, maps.b, maps.low, maps.up, p));
+    NT_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, maps.w, maps.x, maps.x32, maps.x16, maps.low, maps.up, p));
     return 0;
 }
 
-// Tensor maps, then the launch.  up: null where there are no adapters.
-template <int CG, int BN>
-int launch_lora(cudaStream_t stream, const DeviceState &dev, int dtype, Maps &maps, Params &p, const void *lhs, int64_t lhs_stride0,
-                const Matrices &rhs, const Matrices *up) {
-    using S = Shape<CG, BN>;
-    p.n_tiles = static_cast<int>((static_cast<int64_t>(p.n) + BN - 1) / BN);
-    p.k_blocks = (p.k + BK - 1) / BK;
-    p.group_m = GROUP_ROWS / CG;
+// Tensor maps, then the launch.  up and low: null where there are no adapters.
+template <int CG, int NT>
+int launch_lora(cudaStream_t stream, const DeviceState &dev, int dtype, Params &p, const void *lhs, int64_t lhs_stride0,
+                const Matrices &rhs, const Matrices *up, const void *low) {
+    using S = Turned<CG, NT>;
+    p.n_tiles = static_cast<int>((static_cast<int64_t>(p.n) + S::TILE_N - 1) / S::TILE_N);
+    p.k_blocks = (p.k + S::DEPTH - 1) / S::DEPTH;
+    p.group_m = std::max(1, 2048 / NT);
     const bool mn = rhs.use_mn();
-    if (int rc = map_rows(dev, &maps.a, dtype, lhs, p.rows, p.k, lhs_stride0, BK, BM)) return rc;
-    if (int rc = map_rows(dev, &maps.a_chunk, dtype, lhs, p.rows, p.k, lhs_stride0, BK, A_CHUNK_ROWS)) return rc;
-    if (int rc = map_matrices(dev, &maps.b, dtype, rhs, mn, 64, mn ? BK : S::BN_CTA)) return rc;
+    LoraMaps maps;
+    if (int rc = map_matrices(dev, &maps.w, dtype, rhs, mn, 64, mn ? S::DEPTH : BM)) return rc;
+    if (int rc = map_rows(dev, &maps.x, dtype, lhs, p.rows, p.k, lhs_stride0, BK, S::ROWS_CTA)) return rc;
+    if (int rc = map_rows(dev, &maps.x32, dtype, lhs, p.rows, p.k, lhs_stride0, BK, 32)) return rc;
+    if (int rc = map_rows(dev, &maps.x16, dtype, lhs, p.rows, p.k, lhs_stride0, BK, 16)) return rc;
+    maps.up = maps.low = maps.x;
     if (up != nullptr) {
         p.up_mn = up->use_mn();
-        if (int rc = map_matrices(dev, &maps.up, dtype, *up, p.up_mn, 64, p.up_mn ? RANK_BLOCK : S::BN_CTA)) return rc;
-    } else {
-        maps.up = maps.low = maps.a;
+        const int64_t pitch = p.rank_blocks * (2 * RANK_BLOCK);
+        if (int rc = map_matrices(dev, &maps.up, dtype, *up, p.up_mn, 64, p.up_mn ? RANK_BLOCK : BM)) return rc;
+        if (int rc = map_rows(dev, &maps.low, dtype, low, p.rows, pitch, pitch, BK, S::ROWS_CTA)) return rc;
     }
-    const int64_t tiles = (static_cast<int64_t>(p.rows) + S::TILE_M - 1) / S::TILE_M * p.n_tiles;
-    if (tiles > INT_MAX / 2) return fail(NINETOOTHED_B200_ERR_SHAPE, "lora_matmul: too many tiles");
-    return mn ? launch_lora_kernel<CG, BN, true>(stream, dev, maps, p, tiles) : launch_lora_kernel<CG, BN, false>(stream, dev, maps, p, tiles);
+    const int64_t columns = p.rows + 15 * static_cast<int64_t>(std::min(p.offsets.runs, p.rows));
+    const int64_t most = (columns + NT - 1) / NT * p.n_tiles;
+    if (most > INT_MAX / 16) return fail(NINETOOTHED_B200_ERR_SHAPE, "lora_matmul: too many tiles");
+    return mn ? launch_lora_kernel<CG, NT, true>(stream, dev, maps, p, most) : launch_lora_kernel<CG, NT, false>(stream, dev, maps, p, most);
 }
 
 template <int CG, int NT, bool W_MN, bool SPLIT, Job JOB>
@@ -2007,7 +1960,7 @@ int launch_few(cudaStream_t stream, const DeviceState &dev, int dtype, Params &p
 
 bool has_arrays(const NineToothedTensor &t) { return t.shape != nullptr && t.strides != nullptr; }
 
-constexpr int64_t MAX_DIM = INT_MAX - 4096;  // coordinates of a tile that overhangs stay 32-bit
+constexpr int64_t MAX_DIM = INT_MAX - 65536;  // coordinates of a tile that overhangs, and padded rows, stay 32-bit
 
 int check_offsets(const char *what, const NineToothedTensor &offsets, int64_t runs, int offsets_dtype, Offsets *out) {
     if (offsets_dtype != NINETOOTHED_INT32 && offsets_dtype != NINETOOTHED_INT64)
@@ -2172,7 +2125,6 @@ int run_grouped_grad(cudaStream_t stream, const NineToothedTensor &lhs, const Ni
 // Many rows under adapters: first scales (lhs . down), then the projection with the second products.
 int launch_many(cudaStream_t stream, const DeviceState &dev, int dtype, Params &p, const void *lhs, int64_t lhs_stride0,
                 const Matrices &rhs, const Matrices &down, const Matrices &up, void *workspace) {
-    Maps maps;
     const bool any = p.matrices > 0;
     if (any) {
         Params parts = p;
@@ -2189,16 +2141,15 @@ int launch_many(cudaStream_t stream, const DeviceState &dev, int dtype, Params &
         else if (narrow <= 2 * dev.sm_count) rc = launch_turned<1, 64, false, JOB_PARTS>(stream, dev, dtype, parts, lhs, lhs_stride0, down, live);
         else rc = launch_turned<1, 128, false, JOB_PARTS>(stream, dev, dtype, parts, lhs, lhs_stride0, down, live);
         if (rc != 0) return rc;
-        if ((rc = map_rows(dev, &maps.low, dtype, workspace, p.rows, parts.out_stride0, parts.out_stride0, BK, A_CHUNK_ROWS)) != 0) return rc;
     }
-    // Tiles of 256 x 256 on CTA pairs, or 128 x 128 on single CTAs where that takes fewer waves' time (a 128 x 128 tile takes
-    // about half the pair's time for its 64-deep block: it is bound by L2).
-    const auto waves = [&](int64_t rows, int64_t columns, int64_t workers) {
-        return ((p.rows + rows - 1) / rows * ((p.n + columns - 1) / columns) + workers - 1) / workers;
+    // Tiles of 256 x 256 on CTA pairs, or 128 x 128 on single CTAs where that takes fewer waves' time (as in launch_grouped).
+    const int64_t columns = p.rows + 8 * static_cast<int64_t>(std::min(p.offsets.runs, p.rows));
+    const auto waves = [&](int64_t rows, int64_t workers) {
+        return ((columns + rows - 1) / rows * ((p.n + rows - 1) / rows) + workers - 1) / workers;
     };
-    if (7 * waves(256, 256, dev.sm_count / 2) <= 5 * waves(128, 128, dev.sm_count))
-        return launch_lora<2, 256>(stream, dev, dtype, maps, p, lhs, lhs_stride0, rhs, any ? &up : nullptr);
-    return launch_lora<1, 128>(stream, dev, dtype, maps, p, lhs, lhs_stride0, rhs, any ? &up : nullptr);
+    if (1540 * waves(256, dev.sm_count / 2) <= 1080 * waves(128, dev.sm_count))
+        return launch_lora<2, 256>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, any ? &up : nullptr, workspace);
+    return launch_lora<1, 128>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, any ? &up : nullptr, workspace);
 }
 
 int run_lora(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothedTensor &rhs, const NineToothedTensor &down,
