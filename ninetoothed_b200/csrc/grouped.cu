@@ -273,9 +273,8 @@ __device__ __forceinline__ float load16(const void *in, int64_t at, bool bf16) {
                 : __half2float(static_cast<const __half *>(in)[at]);
 }
 
-// Producers run their loops as whole warps, so that addresses and coordinates stay in uniform registers, which is where
-// the copy instructions read them; an elected lane issues.  (A lone lane took 130 cycles a copy: the moves between the
-// register files made issuing, not memory, the limit.)
+// A copy costs a lone lane about 130 cycles to issue, so the operands have a producer each and stages are 128 deep where they
+// can be: a stage's copies take less than its products.
 template <int CG>
 __device__ __forceinline__ void load_2d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y) {
     if constexpr (CG == 1) tma_load_2d(dst, map, bar, x, y);
@@ -748,8 +747,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
     if (warp == 0 || warp == ROW_WARP) {
         // ------------- TMA producers: warp 0 the matrices, the last warp the rows -------------
-        const bool issuer = elect_one();
+        // (Copies, products and their commits leave from lone lanes, in branches that no other lane of the warp enters.  These
+        // loops go by values from shared memory, so that a warp that walked them together with one elected lane issuing would
+        // not be known to have come together again: such an issuer was seen to commit a tile twice after a loop of its own
+        // lane's, which turned the accumulators' barriers a phase too far.)
         uint32_t s = 0, phase = 1, tile_it = 0;
+        if (lane == 0)
         for (W walk(p, table, ctl, worker, workers); walk.more(); walk.advance(), ++tile_it) {
             const TurnedPlace at = walk.place(p);
             constexpr int STEP = 16 * CG;
@@ -762,10 +765,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             const int w_boxes_other = CG == 1 ? 0 : W_MN ? min(BM / 64, max(0, (p.n - n0 - BM + 63) / 64)) : BM / 64;
             const int bytes = (w_boxes + w_boxes_other) * (S::W_BYTES / (BM / 64)) + CG * S::SUB * boxes * (A_CHUNK_ROWS * BK * 2);
             for (int kb = kb_first; kb < kb_last; ++kb) {
-                mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x100 | s);
+                mbar_wait(&ctl->empty[s], phase, wait_ctx, 0x100 | s);
                 uint8_t *w_dst = smem + s * S::STAGE_BYTES;
                 uint8_t *x_dst = w_dst + S::W_BYTES;
-                if (issuer && warp == 0) {
+                if (warp == 0) {
                     if (leader) {
                         // (the issuer of the products learns the tile's rows here: placing a tile takes a few hundred
                         // cycles, which the producer is ahead and the tensor core would idle)
@@ -782,7 +785,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                         for (int sub = 0; sub < S::SUB; ++sub)
                             load_3d<CG>(w_dst + sub * A_STAGE_BYTES, &map_w, &ctl->full[s], kb * S::DEPTH + sub * BK, n0, at.matrix);
                     }
-                } else if (issuer) {
+                } else {
 #pragma unroll
                     for (int sub = 0; sub < S::SUB; ++sub) {
                         const int k0 = kb * S::DEPTH + sub * BK;
@@ -803,8 +806,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
     } else if (warp == 1) {
         // ------------------------------- MMA issuer -------------------------------
-        if (leader) {
-            const bool issuer = elect_one();
+        if (leader && lane == 0) {
             const uint32_t smem_base = smem_u32(smem);
             uint32_t s = 0, phase = 0, acc_it = 0;
             bool ready = false;
@@ -813,14 +815,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 constexpr int STEP = 16 * CG;
                 uint32_t idesc = 0;
                 const uint32_t buf = acc_it & 1;
-                mbar_wait_warp(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+                mbar_wait(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
                 tcgen05_fence_after_sync();
                 const uint32_t tmem_acc = tmem_base + buf * NT;
                 for (int kb = kb_first; kb < kb_last; ++kb) {
-                    if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x300 | s);
+                    if (!ready) mbar_wait(&ctl->full[s], phase, wait_ctx, 0x300 | s);
                     tcgen05_fence_after_sync();
                     if (kb == kb_first) {
-                        const int rows = __shfl_sync(0xffffffffu, ctl->tile_rows[acc_it % MAX_STAGES], 0);
+                        const int rows = ctl->tile_rows[acc_it % MAX_STAGES];
                         idesc = umma_instr_desc(BM * CG, (rows + STEP - 1) / STEP * STEP, p.bf16 != 0, W_MN, false);
                     }
                     const uint32_t w_addr = smem_base + s * S::STAGE_BYTES;
@@ -834,22 +836,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                             W_MN ? umma_smem_desc(w_addr + kk * (UMMA_K * 128), S::DEPTH * 128, 1024)
                                  : umma_smem_desc(w_addr + sub * A_STAGE_BYTES + step * (UMMA_K * 2), 16, 1024);
                         const uint64_t desc_x = umma_smem_desc(x_addr + sub * S::X_BYTES + step * (UMMA_K * 2), 16, 1024);
-                        if (issuer) umma_ss<CG>(tmem_acc, desc_w, desc_x, idesc, (kb != kb_first || kk != 0) ? 1u : 0u);
+                        umma_ss<CG>(tmem_acc, desc_w, desc_x, idesc, (kb != kb_first || kk != 0) ? 1u : 0u);
                         if (kk == S::DEPTH / UMMA_K / 2 - 1)
-                            ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
+                            ready = mbar_test_wait(&ctl->full[s_next], phase_next);
                     }
-                    if (issuer) {
-                        if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
-                        else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
-                    }
+                    if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
+                    else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
                     s = s_next;
                     phase = phase_next;
                 }
-                if (issuer) {
-                    if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
-                    else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
-                }
-                __syncwarp();
+                if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
+                else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
             }
         }
     } else {
@@ -993,17 +990,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
 // ---------------------------------------------------------------------------
 // The shared projection with adapters beside it, for many rows, with the operands exchanged as in turned_kernel.  The rows
-// stand in a padded space of accumulator columns in which every request starts at a multiple of 16; a tile is NT columns of
+// stand in a padded space of accumulator columns in which every request starts at a multiple of 16 (32); a tile is NT columns of
 // it, whatever requests they belong to, against 128 (256) columns of rhs.  Then, for every request with an adapter that has
 // columns in the tile, its second product is an ordinary product into just these columns, 32 ranks a stage: nothing of one
 // request's adapter, infinities and NaN included, meets another's columns.  (scales lhs . down comes in two 16-bit parts from
 // the launch before.)
 // ---------------------------------------------------------------------------
 // The columns [from, to) of the padded space that a run of the table (tiles_before: its first column) has in [low, high).
+template <int STEP>
 struct Piece {
     int from, to;
     __device__ Piece(const Run &run, int low, int high)
-        : from(max(run.tiles_before, low)), to(min(run.tiles_before + (run.end - run.begin + 15) / 16 * 16, high)) {}
+        : from(max(run.tiles_before, low)), to(min(run.tiles_before + (run.end - run.begin + STEP - 1) / STEP * STEP, high)) {}
     __device__ int row(const Run &run) const { return run.begin + from - run.tiles_before; }
 };
 
@@ -1059,19 +1057,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tmem_alloc<CG>(&ctl->tmem_base, TMEM_COLS);
         tmem_relinquish<CG>();
     }
-    build_table<true>(p, table, ctl, 16);
+    constexpr int STEP = 16 * CG;  // columns of a request start at multiples of it (a product of a pair takes steps of 32)
+    build_table<true>(p, table, ctl, STEP);
     tcgen05_fence_before_sync();
     __syncthreads();
     if constexpr (CG == 2) cluster_sync();
     tcgen05_fence_after_sync();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
-    const int runs = ctl->runs, columns = ctl->tiles_m * 16;  // of the padded space
+    const int runs = __shfl_sync(0xffffffffu, ctl->runs, 0);
+    const int columns = __shfl_sync(0xffffffffu, ctl->tiles_m, 0) * STEP;  // of the padded space
     const int m_tiles = (columns + NT - 1) / NT, total = m_tiles * p.n_tiles;
-    constexpr int STEP = 16 * CG;
 
-    if (warp == 0) {
+    // (lone lanes, as in turned_kernel)
+    if (warp == 0 && lane == 0) {
         // ------------------- TMA producer of the matrices, rhs and up -------------------
-        const bool issuer = elect_one();
         uint32_t s = 0, phase = 1;
         const auto next = [&] {
             if (++s == STAGES) {
@@ -1088,19 +1087,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             // (the even CTA's barriers count the bytes of both)
             const int bytes = CG * S::W_BYTES + S::SUB * (last - first) * ROW_BYTES;
             for (int kb = 0; kb < p.k_blocks; ++kb) {
-                mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x100 | s);
+                mbar_wait(&ctl->empty[s], phase, wait_ctx, 0x100 | s);
                 uint8_t *dst = smem + s * S::STAGE_BYTES;
-                if (issuer) {
-                    if (leader) mbar_expect_tx(&ctl->full[s], bytes);
-                    if constexpr (W_MN) {
+                if (leader) mbar_expect_tx(&ctl->full[s], bytes);
+                if constexpr (W_MN) {
 #pragma unroll
-                        for (int j = 0; j < BM / 64; ++j)
-                            load_3d<CG>(dst + j * (S::DEPTH * 128), &map_w, &ctl->full[s], n0 + j * 64, kb * S::DEPTH, 0);
-                    } else {
+                    for (int j = 0; j < BM / 64; ++j)
+                        load_3d<CG>(dst + j * (S::DEPTH * 128), &map_w, &ctl->full[s], n0 + j * 64, kb * S::DEPTH, 0);
+                } else {
 #pragma unroll
-                        for (int sub = 0; sub < S::SUB; ++sub)
-                            load_3d<CG>(dst + sub * A_STAGE_BYTES, &map_w, &ctl->full[s], kb * S::DEPTH + sub * BK, n0, 0);
-                    }
+                    for (int sub = 0; sub < S::SUB; ++sub)
+                        load_3d<CG>(dst + sub * A_STAGE_BYTES, &map_w, &ctl->full[s], kb * S::DEPTH + sub * BK, n0, 0);
                 }
                 next();
             }
@@ -1108,25 +1105,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 const int matrix = table[r].matrix;
                 if (matrix < 0) continue;
                 for (int rb = 0; rb < p.rank_blocks; ++rb) {
-                    mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x110 | s);
+                    mbar_wait(&ctl->empty[s], phase, wait_ctx, 0x110 | s);
                     uint8_t *dst = smem + s * S::STAGE_BYTES;
-                    if (issuer) {
-                        if (leader) mbar_expect_tx(&ctl->full[s], CG * (up_bytes + S::X_BYTES));
-                        if (p.up_mn) {
+                    if (leader) mbar_expect_tx(&ctl->full[s], CG * (up_bytes + S::X_BYTES));
+                    if (p.up_mn) {
 #pragma unroll
-                            for (int j = 0; j < BM / 64; ++j)
-                                load_3d<CG>(dst + j * (RANK_BLOCK * 128), &map_up, &ctl->full[s], n0 + j * 64, rb * RANK_BLOCK, matrix);
-                        } else {
-                            load_3d<CG>(dst, &map_up, &ctl->full[s], rb * RANK_BLOCK, n0, matrix);
-                        }
+                        for (int j = 0; j < BM / 64; ++j)
+                            load_3d<CG>(dst + j * (RANK_BLOCK * 128), &map_up, &ctl->full[s], n0 + j * 64, rb * RANK_BLOCK, matrix);
+                    } else {
+                        load_3d<CG>(dst, &map_up, &ctl->full[s], rb * RANK_BLOCK, n0, matrix);
                     }
                     next();
                 }
             }
         }
-    } else if (warp == ROW_WARP) {
+    } else if (warp == ROW_WARP && lane == 0) {
         // --------------- TMA producer of the rows, of lhs and of (scales lhs . down) ---------------
-        const bool issuer = elect_one();
         uint32_t s = 0, phase = 1;
         const auto next = [&] {
             if (++s == STAGES) {
@@ -1143,47 +1137,43 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             const int mine = first + static_cast<int>(cta_rank) * width_cta, mine_end = min(mine + width_cta, last);
             const int run_first = run_at(table, runs, first), run_mine = run_at(table, runs, mine);
             for (int kb = 0; kb < p.k_blocks; ++kb) {
-                mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x120 | s);
+                mbar_wait(&ctl->empty[s], phase, wait_ctx, 0x120 | s);
                 uint8_t *dst = smem + s * S::STAGE_BYTES + S::W_BYTES;
                 for (int r = run_mine; r < runs && table[r].tiles_before < mine_end; ++r) {
-                    const Piece piece(table[r], mine, mine_end);
+                    const Piece<STEP> piece(table[r], mine, mine_end);
                     const int row = piece.row(table[r]), count = piece.to - piece.from;
-                    if (issuer) {
 #pragma unroll
-                        for (int sub = 0; sub < S::SUB; ++sub) {
-                            uint8_t *at = dst + sub * S::X_BYTES + (piece.from - mine) * ROW_BYTES;
-                            const int k0 = kb * S::DEPTH + sub * BK;
-                            if (count == S::ROWS_CTA) {
-                                load_2d<CG>(at, &map_x, &ctl->full[s], k0, row);
-                            } else {
-                                int c = 0;
-                                for (; c + 32 <= count; c += 32)
-                                    load_2d<CG>(at + c * ROW_BYTES, &map_x32, &ctl->full[s], k0, row + c);
-                                if (c < count) load_2d<CG>(at + c * ROW_BYTES, &map_x16, &ctl->full[s], k0, row + c);
-                            }
+                    for (int sub = 0; sub < S::SUB; ++sub) {
+                        uint8_t *at = dst + sub * S::X_BYTES + (piece.from - mine) * ROW_BYTES;
+                        const int k0 = kb * S::DEPTH + sub * BK;
+                        if (count == S::ROWS_CTA) {
+                            load_2d<CG>(at, &map_x, &ctl->full[s], k0, row);
+                        } else {
+                            int c = 0;
+                            for (; c + 32 <= count; c += 32)
+                                load_2d<CG>(at + c * ROW_BYTES, &map_x32, &ctl->full[s], k0, row + c);
+                            if (c < count) load_2d<CG>(at + c * ROW_BYTES, &map_x16, &ctl->full[s], k0, row + c);
                         }
                     }
-                    __syncwarp();
                 }
                 next();
             }
             for (int r = run_first; r < runs && table[r].tiles_before < last; ++r) {
                 if (table[r].matrix < 0) continue;
-                const Piece piece(table[r], first, last);
+                const Piece<STEP> piece(table[r], first, last);
                 // a pair's CTAs bring half of the piece each (and what follows it, unused)
                 const int row = piece.row(table[r]) + static_cast<int>(cta_rank) * ((piece.to - piece.from) / CG);
                 for (int rb = 0; rb < p.rank_blocks; ++rb) {
-                    mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x130 | s);
+                    mbar_wait(&ctl->empty[s], phase, wait_ctx, 0x130 | s);
                     uint8_t *dst = smem + s * S::STAGE_BYTES + S::W_BYTES;
-                    if (issuer) load_2d<CG>(dst, &map_low, &ctl->full[s], rb * BK, row);
+                    load_2d<CG>(dst, &map_low, &ctl->full[s], rb * BK, row);
                     next();
                 }
             }
         }
     } else if (warp == 1) {
         // ------------------------------- MMA issuer -------------------------------
-        if (leader) {
-            const bool issuer = elect_one();
+        if (leader && lane == 0) {
             const uint32_t smem_base = smem_u32(smem);
             const uint32_t up_step = p.up_mn ? UMMA_K * 128 : UMMA_K * 2, up_lbo = p.up_mn ? RANK_BLOCK * 128 : 16;
             uint32_t s = 0, phase = 0, acc_it = 0;
@@ -1194,11 +1184,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 const int first = m * NT, last = min(first + NT, columns);
                 const uint32_t idesc = umma_instr_desc(BM * CG, (last - first + STEP - 1) / STEP * STEP, p.bf16 != 0, W_MN, false);
                 const uint32_t buf = acc_it & 1;
-                mbar_wait_warp(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+                mbar_wait(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
                 tcgen05_fence_after_sync();
                 const uint32_t tmem_acc = tmem_base + buf * NT;
                 for (int kb = 0; kb < p.k_blocks; ++kb) {
-                    if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x300 | s);
+                    if (!ready) mbar_wait(&ctl->full[s], phase, wait_ctx, 0x300 | s);
                     tcgen05_fence_after_sync();
                     const uint32_t w_addr = smem_base + s * S::STAGE_BYTES;
                     const uint32_t x_addr = w_addr + S::W_BYTES;
@@ -1211,59 +1201,47 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                             W_MN ? umma_smem_desc(w_addr + kk * (UMMA_K * 128), S::DEPTH * 128, 1024)
                                  : umma_smem_desc(w_addr + sub * A_STAGE_BYTES + step * (UMMA_K * 2), 16, 1024);
                         const uint64_t desc_x = umma_smem_desc(x_addr + sub * S::X_BYTES + step * (UMMA_K * 2), 16, 1024);
-                        if (issuer) umma_ss<CG>(tmem_acc, desc_w, desc_x, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
+                        umma_ss<CG>(tmem_acc, desc_w, desc_x, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
                         if (kk == S::DEPTH / UMMA_K / 2 - 1)
-                            ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
+                            ready = mbar_test_wait(&ctl->full[s_next], phase_next);
                     }
-                    if (issuer) {
-                        if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
-                        else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
-                    }
-                    __syncwarp();
+                    if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
+                    else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
                     s = s_next;
                     phase = phase_next;
                 }
                 for (int r = run_at(table, runs, first); r < runs && table[r].tiles_before < last; ++r) {
                     if (table[r].matrix < 0) continue;
-                    const Piece piece(table[r], first, last);
+                    const Piece<STEP> piece(table[r], first, last);
                     const uint32_t idesc_up = umma_instr_desc(BM * CG, piece.to - piece.from, p.bf16 != 0, p.up_mn != 0, false);
                     const uint32_t tmem_piece = tmem_acc + (piece.from - first);
                     for (int rb = 0; rb < p.rank_blocks; ++rb) {
-                        if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x310 | s);
+                        mbar_wait(&ctl->full[s], phase, wait_ctx, 0x310 | s);
                         tcgen05_fence_after_sync();
                         const uint32_t up_addr = smem_base + s * S::STAGE_BYTES;
                         const uint32_t low_addr = up_addr + S::W_BYTES;
-                        const uint32_t s_next = s + 1 == STAGES ? 0 : s + 1;
-                        const uint32_t phase_next = s_next == 0 ? phase ^ 1 : phase;
-                        const bool two = p.rank - rb * RANK_BLOCK > UMMA_K;  // steps of 16 ranks
-#pragma unroll
-                        for (int kk = 0; kk < RANK_BLOCK / UMMA_K; ++kk) {
+                        const int steps = (min(RANK_BLOCK, p.rank - rb * RANK_BLOCK) + UMMA_K - 1) / UMMA_K;
+                        for (int kk = 0; kk < steps; ++kk) {
                             const uint64_t desc_up = umma_smem_desc(up_addr + kk * up_step, up_lbo, 1024);
 #pragma unroll
-                            for (int part = 0; part < 2; ++part) {
-                                const uint64_t desc_low =
-                                    umma_smem_desc(low_addr + part * (RANK_BLOCK * 2) + kk * (UMMA_K * 2), 16, 1024);
-                                if (issuer && (kk == 0 || two)) umma_ss<CG>(tmem_piece, desc_up, desc_low, idesc_up, 1u);
-                            }
+                            for (int part = 0; part < 2; ++part)
+                                umma_ss<CG>(tmem_piece, desc_up,
+                                            umma_smem_desc(low_addr + part * (RANK_BLOCK * 2) + kk * (UMMA_K * 2), 16, 1024), idesc_up, 1u);
                         }
-                        ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
-                        if (issuer) {
-                            if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
-                            else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
+                        if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
+                        else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
+                        if (++s == STAGES) {
+                            s = 0;
+                            phase ^= 1;
                         }
-                        __syncwarp();
-                        s = s_next;
-                        phase = phase_next;
                     }
                 }
-                if (issuer) {
-                    if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
-                    else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
-                }
-                __syncwarp();
+                ready = false;
+                if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
+                else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
             }
         }
-    } else {
+    } else if (warp >= 2 && warp < ROW_WARP) {
         // -------------------------------- epilogue --------------------------------
         const int quadrant = warp & 3, half = (warp - 2) / 4;
         const bool bf16 = p.bf16 != 0;
@@ -1447,30 +1425,28 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
     const auto produce = [&](const CUtensorMap &map, auto cols, auto of_lhs) {
         constexpr int COLS = decltype(cols)::value;
         constexpr bool LHS = decltype(of_lhs)::value;
-        const bool issuer = elect_one();
         uint32_t s = 0, phase = 1;
+        if (lane != 0) return;  // (a lone lane, as in turned_kernel)
         for (int tile = worker; tile < total; tile += workers) {
             const GradTile at = grad_tile(p, starts, tile, S::TILE_M, BN);
             const int col0 = (LHS ? at.m0 : at.n0) + static_cast<int>(cta_rank) * COLS;
             for (int k0 = 0; k0 < at.length; k0 += BK) {
-                mbar_wait_warp(&ctl->empty[s], phase, wait_ctx, 0x100 | s);
+                mbar_wait(&ctl->empty[s], phase, wait_ctx, 0x100 | s);
                 uint8_t *dst = smem + s * S::STAGE_BYTES + (LHS ? 0 : A_STAGE_BYTES);
                 const bool ragged = at.length - k0 < BK && (at.length & (UMMA_K - 1)) != 0;
-                if (issuer) {
-                    if (ragged) {
-                        if (LHS) {
-                            mbar_expect_tx(&ctl->ragged[s], S::STAGE_BYTES);
-                            if (leader) mbar_arrive(&ctl->full[s]);  // (keeps its phases in step; the issuer waits for `clean` too)
-                        }
-#pragma unroll
-                        for (int j = 0; j < COLS / 64; ++j)
-                            tma_load_2d(dst + j * S::BOX_BYTES, &map, &ctl->ragged[s], col0 + j * 64, at.begin + k0);
-                    } else {
-                        if (LHS && leader) mbar_expect_tx(&ctl->full[s], S::STAGE_BYTES * CG);
-#pragma unroll
-                        for (int j = 0; j < COLS / 64; ++j)
-                            load_2d<CG>(dst + j * S::BOX_BYTES, &map, &ctl->full[s], col0 + j * 64, at.begin + k0);
+                if (ragged) {
+                    if (LHS) {
+                        mbar_expect_tx(&ctl->ragged[s], S::STAGE_BYTES);
+                        if (leader) mbar_arrive(&ctl->full[s]);  // (keeps its phases in step; the issuer waits for `clean` too)
                     }
+#pragma unroll
+                    for (int j = 0; j < COLS / 64; ++j)
+                        tma_load_2d(dst + j * S::BOX_BYTES, &map, &ctl->ragged[s], col0 + j * 64, at.begin + k0);
+                } else {
+                    if (LHS && leader) mbar_expect_tx(&ctl->full[s], S::STAGE_BYTES * CG);
+#pragma unroll
+                    for (int j = 0; j < COLS / 64; ++j)
+                        load_2d<CG>(dst + j * S::BOX_BYTES, &map, &ctl->full[s], col0 + j * 64, at.begin + k0);
                 }
                 if (++s == STAGES) {
                     s = 0;
@@ -1487,25 +1463,23 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
     } else if (warp == 1) {
         // ------------------------------- MMA issuer -------------------------------
         const uint32_t idesc = umma_instr_desc(BM * CG, BN, p.bf16 != 0, true, true);
-        const bool issuer = elect_one();
         const uint32_t smem_base = smem_u32(smem);
         uint32_t s = 0, phase = 0, acc_it = 0, clean_phases = 0;  // (a bit a stage: not every use of a stage is ragged)
         bool ready = false;
-        for (int tile = leader ? worker : total; tile < total; tile += workers) {
+        for (int tile = leader && lane == 0 ? worker : total; tile < total; tile += workers) {
             const int length = grad_tile(p, starts, tile, S::TILE_M, BN).length;
             if (length == 0) continue;  // (the epilogue stores zeros by itself)
             const int blocks = (length + BK - 1) / BK;
             const uint32_t buf = acc_it & 1;
-            mbar_wait_warp(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+            mbar_wait(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
             ++acc_it;
             tcgen05_fence_after_sync();
             const uint32_t tmem_acc = tmem_base + buf * BN;
             for (int kb = 0; kb < blocks; ++kb) {
-                if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x300 | s);
+                if (!ready) mbar_wait(&ctl->full[s], phase, wait_ctx, 0x300 | s);
                 const int left = length - kb * BK;
                 if (left < BK && (left & (UMMA_K - 1)) != 0) {
-                    if (lane == 0) mbar_wait_cluster(&ctl->clean[s], (clean_phases >> s) & 1, wait_ctx, 0x700 | s);
-                    __syncwarp();
+                    mbar_wait_cluster(&ctl->clean[s], (clean_phases >> s) & 1, wait_ctx, 0x700 | s);
                     clean_phases ^= 1u << s;
                 }
                 tcgen05_fence_after_sync();
@@ -1518,22 +1492,17 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
                 for (int kk = 0; kk < BK / UMMA_K; ++kk) {
                     const uint64_t desc_a = umma_smem_desc(a_addr + kk * (UMMA_K * 128), S::BOX_BYTES, 1024);
                     const uint64_t desc_b = umma_smem_desc(b_addr + kk * (UMMA_K * 128), S::BOX_BYTES, 1024);
-                    if (issuer && kk < steps) umma_ss<CG>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
+                    if (kk < steps) umma_ss<CG>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
                     if (kk == BK / UMMA_K / 2 - 1)
-                        ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
+                        ready = mbar_test_wait(&ctl->full[s_next], phase_next);
                 }
-                if (issuer) {
-                    if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
-                    else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
-                }
+                if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
+                else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
                 s = s_next;
                 phase = phase_next;
             }
-            if (issuer) {
-                if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
-                else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
-            }
-            __syncwarp();
+            if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
+            else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
         }
     } else if (warp == ROW_WARP + 1) {
         // --------------- the rows behind a run in its last block ---------------
@@ -1831,7 +1800,7 @@ int launch_lora(cudaStream_t stream, const DeviceState &dev, int dtype, Params &
         if (int rc = map_matrices(dev, &maps.up, dtype, *up, p.up_mn, 64, p.up_mn ? RANK_BLOCK : BM)) return rc;
         if (int rc = map_rows(dev, &maps.low, dtype, low, p.rows, pitch, pitch, BK, S::ROWS_CTA)) return rc;
     }
-    const int64_t columns = p.rows + 15 * static_cast<int64_t>(std::min(p.offsets.runs, p.rows));
+    const int64_t columns = p.rows + (16 * CG - 1) * static_cast<int64_t>(std::min(p.offsets.runs, p.rows));
     const int64_t most = (columns + NT - 1) / NT * p.n_tiles;
     if (most > INT_MAX / 16) return fail(NINETOOTHED_B200_ERR_SHAPE, "lora_matmul: too many tiles");
     return mn ? launch_lora_kernel<CG, NT, true>(stream, dev, maps, p, most) : launch_lora_kernel<CG, NT, false>(stream, dev, maps, p, most);

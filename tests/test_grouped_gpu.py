@@ -322,6 +322,35 @@ def test_lora_matmul_many_requests_and_wide_indices():
     run_lora(*args[:5], args[5].long(), args[6].long())
 
 
+# Grids that take every worker through five or more tiles, so that accumulators, stages and their barriers come round:
+# wide tiles (long runs) and narrow ones (short runs), both layouts of the matrices.
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("lengths, k, n", [([2048, 2500, 1536, 2100], 136, 4096), ([70, 0, 128, 101] * 100, 72, 520),
+                                           ([33, 64, 50] * 300, 64, 264)], ids=["wide", "middle", "narrow"])
+def test_grouped_matmul_many_tiles_a_worker(lengths, k, n, transposed):
+    lhs = normal(60, sum(lengths), k)
+    rhs = normal(61, len(lengths), n, k).transpose(1, 2) if transposed else normal(61, len(lengths), k, n)
+    run_grouped(lhs, rhs, bounds_of(lengths))
+
+
+# (256 x 256 tiles on pairs; 128 x 128 ones take less than half a wave by their rule)
+@pytest.mark.parametrize("lengths", [[64, 100, 1, 0, 129, 31, 512, 7], [128] * 8], ids=str)
+def test_rhs_grad_many_tiles_a_worker(lengths):
+    check_rhs_grad(normal(62, sum(lengths), 2048), normal(63, sum(lengths), 2056), bounds_of(lengths))
+
+
+@pytest.mark.parametrize("turned", [(False, False, False), (True, True, True)], ids=["as they lie", "transposed"])
+@pytest.mark.parametrize("lengths, k, n, rank", [([1500, 0, 300, 4000, 77, 2001], 136, 4096, 40), ([9, 31, 16, 70] * 40, 72, 2056, 16),
+                                                 ([5, 100, 17, 33] * 20, 128, 72, 8)], ids=["wide", "ragged", "few columns"])
+def test_lora_matmul_many_tiles_a_worker(lengths, k, n, rank, turned):
+    which = [(i * 5) % 9 - 1 for i in range(len(lengths))]
+    args = list(lora_inputs(lengths, which, k, n, rank, 8, KINDS[len(lengths) % 2]))
+    for i, turn in zip((1, 2, 3), turned):
+        if turn:
+            args[i] = args[i].transpose(-1, -2).contiguous().transpose(-1, -2)
+    run_lora(*args)
+
+
 def test_lora_matmul_on_sizes_no_tensor_map_addresses_and_without_adapters():
     with warnings.catch_warnings():
         warnings.simplefilter("ignore")
