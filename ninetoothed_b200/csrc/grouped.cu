@@ -44,6 +44,7 @@ constexpr size_t MAX_SMEM = 227 * 1024;
 constexpr int EPILOGUE_WARPS = 8;
 constexpr int ROW_WARP = 2 + EPILOGUE_WARPS;
 constexpr int NUM_THREADS = (ROW_WARP + 1) * 32;
+constexpr int LORA_THREADS = NUM_THREADS + 3 * 32;  // and three more producers of rows
 constexpr int GRAD_THREADS = NUM_THREADS + 32;  // and a warp that clears what a run's last block holds of the next run
 
 enum Job { JOB_PRODUCT, JOB_PARTS, JOB_FEW };  // of turned_kernel
@@ -747,10 +748,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
     if (warp == 0 || warp == ROW_WARP) {
         // ------------- TMA producers: warp 0 the matrices, the last warp the rows -------------
-        // (Copies, products and their commits leave from lone lanes, in branches that no other lane of the warp enters.  These
-        // loops go by values from shared memory, so that a warp that walked them together with one elected lane issuing would
-        // not be known to have come together again: such an issuer was seen to commit a tile twice after a loop of its own
-        // lane's, which turned the accumulators' barriers a phase too far.)
+        // (Lone lanes, in branches that no other lane of the warp enters: these loops go by values from shared memory, and in a
+        // warp that walked them together with one elected lane issuing, nothing would tell the compiler that it stays together.
+        // The issuer below can be an elected lane, 3 to 10% faster than a lone one, as its loops go by values known to be the
+        // warp's and it has no branch of that lane alone that holds more than one instruction.  In lora_kernel, whose issuer
+        // has such a loop, a commit behind it by an elected lane was seen to be issued twice.)
         uint32_t s = 0, phase = 1, tile_it = 0;
         if (lane == 0)
         for (W walk(p, table, ctl, worker, workers); walk.more(); walk.advance(), ++tile_it) {
@@ -806,23 +808,24 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
     } else if (warp == 1) {
         // ------------------------------- MMA issuer -------------------------------
-        if (leader && lane == 0) {
+        if (leader) {
+            const bool issuer = elect_one();
             const uint32_t smem_base = smem_u32(smem);
             uint32_t s = 0, phase = 0, acc_it = 0;
             bool ready = false;
-            const int total = ctl->tiles_m * p.n_tiles;
+            const int total = __shfl_sync(0xffffffffu, ctl->tiles_m, 0) * p.n_tiles;  // (known to be the warp's)
             for (int tile = worker; tile < total; tile += workers, ++acc_it) {
                 constexpr int STEP = 16 * CG;
                 uint32_t idesc = 0;
                 const uint32_t buf = acc_it & 1;
-                mbar_wait(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+                mbar_wait_warp(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
                 tcgen05_fence_after_sync();
                 const uint32_t tmem_acc = tmem_base + buf * NT;
                 for (int kb = kb_first; kb < kb_last; ++kb) {
-                    if (!ready) mbar_wait(&ctl->full[s], phase, wait_ctx, 0x300 | s);
+                    if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x300 | s);
                     tcgen05_fence_after_sync();
                     if (kb == kb_first) {
-                        const int rows = ctl->tile_rows[acc_it % MAX_STAGES];
+                        const int rows = __shfl_sync(0xffffffffu, ctl->tile_rows[acc_it % MAX_STAGES], 0);
                         idesc = umma_instr_desc(BM * CG, (rows + STEP - 1) / STEP * STEP, p.bf16 != 0, W_MN, false);
                     }
                     const uint32_t w_addr = smem_base + s * S::STAGE_BYTES;
@@ -836,17 +839,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                             W_MN ? umma_smem_desc(w_addr + kk * (UMMA_K * 128), S::DEPTH * 128, 1024)
                                  : umma_smem_desc(w_addr + sub * A_STAGE_BYTES + step * (UMMA_K * 2), 16, 1024);
                         const uint64_t desc_x = umma_smem_desc(x_addr + sub * S::X_BYTES + step * (UMMA_K * 2), 16, 1024);
-                        umma_ss<CG>(tmem_acc, desc_w, desc_x, idesc, (kb != kb_first || kk != 0) ? 1u : 0u);
+                        if (issuer) umma_ss<CG>(tmem_acc, desc_w, desc_x, idesc, (kb != kb_first || kk != 0) ? 1u : 0u);
                         if (kk == S::DEPTH / UMMA_K / 2 - 1)
-                            ready = mbar_test_wait(&ctl->full[s_next], phase_next);
+                            ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
                     }
-                    if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
-                    else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
+                    if (issuer) {
+                        if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
+                        else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
+                    }
                     s = s_next;
                     phase = phase_next;
                 }
-                if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
-                else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
+                if (issuer) {
+                    if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
+                    else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
+                }
+                __syncwarp();
             }
         }
     } else {
@@ -1017,7 +1025,7 @@ __device__ __forceinline__ int run_at(const Run *table, int runs, int column) {
 }
 
 template <int CG, int NT, bool W_MN>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(LORA_THREADS, 1)
     lora_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                 const __grid_constant__ CUtensorMap map_x32, const __grid_constant__ CUtensorMap map_x16,
                 const __grid_constant__ CUtensorMap map_low, const __grid_constant__ CUtensorMap map_up,
@@ -1119,8 +1127,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 }
             }
         }
-    } else if (warp == ROW_WARP && lane == 0) {
-        // --------------- TMA producer of the rows, of lhs and of (scales lhs . down) ---------------
+    } else if (warp >= ROW_WARP && lane == 0) {
+        // -------------- TMA producers of the rows, of lhs and of (scales lhs . down) --------------
+        // Where requests meet in a tile its rows are many small boxes: one lane's copies of them took 2300 cycles a stage, over
+        // twice the products' time.  Four lanes share them: the halves of a stage, and every other box.
+        const int sub = (warp - ROW_WARP) & 1, turn = (warp - ROW_WARP) >> 1;
         uint32_t s = 0, phase = 1;
         const auto next = [&] {
             if (++s == STAGES) {
@@ -1139,20 +1150,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             for (int kb = 0; kb < p.k_blocks; ++kb) {
                 mbar_wait(&ctl->empty[s], phase, wait_ctx, 0x120 | s);
                 uint8_t *dst = smem + s * S::STAGE_BYTES + S::W_BYTES;
+                const int k0 = kb * S::DEPTH + sub * BK;
+                int box = turn;  // boxes until this lane's next
                 for (int r = run_mine; r < runs && table[r].tiles_before < mine_end; ++r) {
                     const Piece<STEP> piece(table[r], mine, mine_end);
                     const int row = piece.row(table[r]), count = piece.to - piece.from;
-#pragma unroll
-                    for (int sub = 0; sub < S::SUB; ++sub) {
-                        uint8_t *at = dst + sub * S::X_BYTES + (piece.from - mine) * ROW_BYTES;
-                        const int k0 = kb * S::DEPTH + sub * BK;
-                        if (count == S::ROWS_CTA) {
-                            load_2d<CG>(at, &map_x, &ctl->full[s], k0, row);
-                        } else {
-                            int c = 0;
-                            for (; c + 32 <= count; c += 32)
-                                load_2d<CG>(at + c * ROW_BYTES, &map_x32, &ctl->full[s], k0, row + c);
-                            if (c < count) load_2d<CG>(at + c * ROW_BYTES, &map_x16, &ctl->full[s], k0, row + c);
+                    uint8_t *at = dst + sub * S::X_BYTES + (piece.from - mine) * ROW_BYTES;
+                    if (count == S::ROWS_CTA) {
+                        if (box == 0) load_2d<CG>(at, &map_x, &ctl->full[s], k0, row);
+                        box ^= 1;
+                    } else {
+                        int c = 0;
+                        for (; c + 32 <= count; c += 32, box ^= 1)
+                            if (box == 0) load_2d<CG>(at + c * ROW_BYTES, &map_x32, &ctl->full[s], k0, row + c);
+                        if (c < count) {
+                            if (box == 0) load_2d<CG>(at + c * ROW_BYTES, &map_x16, &ctl->full[s], k0, row + c);
+                            box ^= 1;
                         }
                     }
                 }
@@ -1166,7 +1179,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 for (int rb = 0; rb < p.rank_blocks; ++rb) {
                     mbar_wait(&ctl->empty[s], phase, wait_ctx, 0x130 | s);
                     uint8_t *dst = smem + s * S::STAGE_BYTES + S::W_BYTES;
-                    load_2d<CG>(dst, &map_low, &ctl->full[s], rb * BK, row);
+                    if (warp == ROW_WARP) load_2d<CG>(dst, &map_low, &ctl->full[s], rb * BK, row);
                     next();
                 }
             }
@@ -1463,23 +1476,25 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
     } else if (warp == 1) {
         // ------------------------------- MMA issuer -------------------------------
         const uint32_t idesc = umma_instr_desc(BM * CG, BN, p.bf16 != 0, true, true);
+        const bool issuer = elect_one();
         const uint32_t smem_base = smem_u32(smem);
         uint32_t s = 0, phase = 0, acc_it = 0, clean_phases = 0;  // (a bit a stage: not every use of a stage is ragged)
         bool ready = false;
-        for (int tile = leader && lane == 0 ? worker : total; tile < total; tile += workers) {
-            const int length = grad_tile(p, starts, tile, S::TILE_M, BN).length;
+        for (int tile = leader ? worker : total; tile < total; tile += workers) {
+            const int length = __shfl_sync(0xffffffffu, grad_tile(p, starts, tile, S::TILE_M, BN).length, 0);
             if (length == 0) continue;  // (the epilogue stores zeros by itself)
             const int blocks = (length + BK - 1) / BK;
             const uint32_t buf = acc_it & 1;
-            mbar_wait(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+            mbar_wait_warp(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
             ++acc_it;
             tcgen05_fence_after_sync();
             const uint32_t tmem_acc = tmem_base + buf * BN;
             for (int kb = 0; kb < blocks; ++kb) {
-                if (!ready) mbar_wait(&ctl->full[s], phase, wait_ctx, 0x300 | s);
+                if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x300 | s);
                 const int left = length - kb * BK;
                 if (left < BK && (left & (UMMA_K - 1)) != 0) {
-                    mbar_wait_cluster(&ctl->clean[s], (clean_phases >> s) & 1, wait_ctx, 0x700 | s);
+                    if (lane == 0) mbar_wait_cluster(&ctl->clean[s], (clean_phases >> s) & 1, wait_ctx, 0x700 | s);
+                    __syncwarp();
                     clean_phases ^= 1u << s;
                 }
                 tcgen05_fence_after_sync();
@@ -1492,17 +1507,22 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
                 for (int kk = 0; kk < BK / UMMA_K; ++kk) {
                     const uint64_t desc_a = umma_smem_desc(a_addr + kk * (UMMA_K * 128), S::BOX_BYTES, 1024);
                     const uint64_t desc_b = umma_smem_desc(b_addr + kk * (UMMA_K * 128), S::BOX_BYTES, 1024);
-                    if (kk < steps) umma_ss<CG>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
+                    if (issuer && kk < steps) umma_ss<CG>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
                     if (kk == BK / UMMA_K / 2 - 1)
-                        ready = mbar_test_wait(&ctl->full[s_next], phase_next);
+                        ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
                 }
-                if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
-                else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
+                if (issuer) {
+                    if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
+                    else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
+                }
                 s = s_next;
                 phase = phase_next;
             }
-            if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
-            else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
+            if (issuer) {
+                if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
+                else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
+            }
+            __syncwarp();
         }
     } else if (warp == ROW_WARP + 1) {
         // --------------- the rows behind a run in its last block ---------------
@@ -1758,14 +1778,14 @@ int launch_lora_kernel(cudaStream_t stream, const DeviceState &dev, const LoraMa
     static thread_local int pairs = 0;
     if (configured_device != dev.device) {
         NT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SMEM)));
-        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, NUM_THREADS);
+        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, LORA_THREADS);
         configured_device = dev.device;
     }
     const int workers = CG == 2 ? pairs : dev.sm_count;
     if (workers <= 0) return fail(NINETOOTHED_B200_ERR_DEVICE, "lora_matmul: no CTA pair fits this device");
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(most_tiles, workers) * CG));
-    config.blockDim = dim3(NUM_THREADS);
+    config.blockDim = dim3(LORA_THREADS);
     config.dynamicSmemBytes = turned_smem<CG, NT, false, false>(p.offsets.runs);
     config.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -2112,11 +2132,12 @@ int launch_many(cudaStream_t stream, const DeviceState &dev, int dtype, Params &
         if (rc != 0) return rc;
     }
     // Tiles of 256 x 256 on CTA pairs, or 128 x 128 on single CTAs where that takes fewer waves' time (as in launch_grouped).
-    const int64_t columns = p.rows + 8 * static_cast<int64_t>(std::min(p.offsets.runs, p.rows));
-    const auto waves = [&](int64_t rows, int64_t workers) {
-        return ((columns + rows - 1) / rows * ((p.n + rows - 1) / rows) + workers - 1) / workers;
+    // A request's columns are padded to steps of 16, of 32 on a pair: by half a step, taken over all.
+    const auto waves = [&](int64_t width, int64_t step, int64_t workers) {
+        const int64_t columns = p.rows + step / 2 * static_cast<int64_t>(std::min(p.offsets.runs, p.rows));
+        return ((columns + width - 1) / width * ((p.n + width - 1) / width) + workers - 1) / workers;
     };
-    if (1540 * waves(256, dev.sm_count / 2) <= 1080 * waves(128, dev.sm_count))
+    if (1540 * waves(256, 32, dev.sm_count / 2) <= 1080 * waves(128, 16, dev.sm_count))
         return launch_lora<2, 256>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, any ? &up : nullptr, workspace);
     return launch_lora<1, 128>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, any ? &up : nullptr, workspace);
 }
