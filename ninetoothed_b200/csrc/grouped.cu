@@ -399,6 +399,7 @@ __device__ __forceinline__ void mbar_wait_cluster(uint64_t *bar, uint32_t parity
 
 __device__ __forceinline__ void griddepcontrol_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddepcontrol_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
 __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(EPILOGUE_WARPS * 32) : "memory"); }
 
@@ -741,6 +742,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     if constexpr (SPLIT) cluster_arrive();  // (awaited before the first access to another CTA's memory)
     tcgen05_fence_after_sync();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+    if constexpr (PARTS) griddepcontrol_launch_dependents();  // (the projection waits for this kernel before it reads the parts)
     using W = TurnedWalk<CG, NT, FEW>;
     // this CTA's share of the reduction (a share may be empty)
     const int kb_first = SPLIT ? p.k_blocks * static_cast<int>(cta_rank) / split : 0;
@@ -1132,6 +1134,12 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
         // Where requests meet in a tile its rows are many small boxes: one lane's copies of them took 2300 cycles a stage, over
         // twice the products' time.  Four lanes share them: the halves of a stage, and every other box.
         const int sub = (warp - ROW_WARP) & 1, turn = (warp - ROW_WARP) >> 1;
+        bool waited = false;
+        const auto wait_parts = [&] {  // for the kernel before this one, under which this one starts
+            griddepcontrol_wait();
+            fence_proxy_async();  // (it wrote, copies read)
+            waited = true;
+        };
         uint32_t s = 0, phase = 1;
         const auto next = [&] {
             if (++s == STAGES) {
@@ -1179,11 +1187,15 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
                 for (int rb = 0; rb < p.rank_blocks; ++rb) {
                     mbar_wait(&ctl->empty[s], phase, wait_ctx, 0x130 | s);
                     uint8_t *dst = smem + s * S::STAGE_BYTES + S::W_BYTES;
-                    if (warp == ROW_WARP) load_2d<CG>(dst, &map_low, &ctl->full[s], rb * BK, row);
+                    if (warp == ROW_WARP) {
+                        if (!waited) wait_parts();
+                        load_2d<CG>(dst, &map_low, &ctl->full[s], rb * BK, row);
+                    }
                     next();
                 }
             }
         }
+        if (warp == ROW_WARP && !waited) wait_parts();  // (what follows this launch may rely on the one before)
     } else if (warp == 1) {
         // ------------------------------- MMA issuer -------------------------------
         if (leader && lane == 0) {
@@ -1788,12 +1800,16 @@ int launch_lora_kernel(cudaStream_t stream, const DeviceState &dev, const LoraMa
     config.blockDim = dim3(LORA_THREADS);
     config.dynamicSmemBytes = turned_smem<CG, NT, false, false>(p.offsets.runs);
     config.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    config.attrs = attr;
+    config.numAttrs = 0;
     if (CG == 2) {
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim = {2, 1, 1};
-        config.attrs = attr;
-        config.numAttrs = 1;
+        attr[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[config.numAttrs++].val.clusterDim = {2, 1, 1};
+    }
+    if (p.matrices > 0) {  // starts under the kernel that computes scales (lhs . down)
+        attr[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
     NT_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, maps.w, maps.x, maps.x32, maps.x16, maps.low, maps.up, p));
     return 0;
