@@ -1899,9 +1899,10 @@ int launch_turned(cudaStream_t stream, const DeviceState &dev, int dtype, Params
 // hold rows, and a run of r rows makes about r / NT + 1/2 tiles.
 //   - Fewer tiles than half the SMs: clusters of 2 to 8 CTAs share each tile's reduction (one row against two 4096 x 2048
 //     matrices: 16.0 us without, 11.2 with four CTAs a tile).
-//   - Otherwise the width with the least modelled time, waves x blocks x cycles per 128-deep block (measured: 830 for 64
-//     rows, 1080 for 128, 1540 for 256 on a pair).  Runs of 96, 192 and 384 rows against eight 4096 x 1024 matrices take
-//     19.7, 30.5, 42.5 us with 64 rows a tile, 23.3, 24.3, 39.4 with 128, 24.2, 30.3, 31.4 with 256.
+//   - Otherwise the width with the least modelled time, waves x blocks x cycles per 128-deep block (830 for 64 rows, 1080
+//     for 128, 1400 for 256 on a pair: between the 1540 measured where all SMs wait for memory and the 1100 of the products).
+//     Runs of 96, 192 and 384 rows against eight 4096 x 1024 matrices take 19.7, 30.5, 42.5 us with 64 rows a tile, 23.3,
+//     24.3, 39.4 with 128, 24.2, 30.3, 31.4 with 256; 29 runs of 172 rows on average against 1544 x 1160 ones 58, 45, 39.
 int launch_grouped(cudaStream_t stream, const DeviceState &dev, int dtype, Params &p, const void *lhs, int64_t lhs_stride0,
                    const Matrices &rhs, int64_t live) {
     const int64_t n_tiles = (static_cast<int64_t>(p.n) + BM - 1) / BM;
@@ -1915,7 +1916,7 @@ int launch_grouped(cudaStream_t stream, const DeviceState &dev, int dtype, Param
         return (tiles + workers - 1) / workers * cycles;
     };
     const int64_t narrow = cost(64, 128, dev.sm_count, 830), middle = cost(128, 128, dev.sm_count, 1080),
-                  wide = cost(256, 256, dev.sm_count / 2, 1540);
+                  wide = cost(256, 256, dev.sm_count / 2, 1400);
     if (narrow <= middle && narrow <= wide)
         return launch_turned<1, 64, false, JOB_PRODUCT>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
     if (middle <= wide) return launch_turned<1, 128, false, JOB_PRODUCT>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, live);
@@ -2153,7 +2154,7 @@ int launch_many(cudaStream_t stream, const DeviceState &dev, int dtype, Params &
         const int64_t columns = p.rows + step / 2 * static_cast<int64_t>(std::min(p.offsets.runs, p.rows));
         return ((columns + width - 1) / width * ((p.n + width - 1) / width) + workers - 1) / workers;
     };
-    if (1540 * waves(256, 32, dev.sm_count / 2) <= 1080 * waves(128, 16, dev.sm_count))
+    if (1400 * waves(256, 32, dev.sm_count / 2) <= 1080 * waves(128, 16, dev.sm_count))
         return launch_lora<2, 256>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, any ? &up : nullptr, workspace);
     return launch_lora<1, 128>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, any ? &up : nullptr, workspace);
 }
