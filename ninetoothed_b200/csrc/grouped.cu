@@ -756,8 +756,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         // warp's and it has no branch of that lane alone that holds more than one instruction.  In lora_kernel, whose issuer
         // has such a loop, a commit behind it by an elected lane was seen to be issued twice.)
         uint32_t s = 0, phase = 1, tile_it = 0;
-        if (lane == 0)
-        for (W walk(p, table, ctl, worker, workers); walk.more(); walk.advance(), ++tile_it) {
+        for (W walk(p, table, ctl, worker, workers); lane == 0 && walk.more(); walk.advance(), ++tile_it) {
             const TurnedPlace at = walk.place(p);
             constexpr int STEP = 16 * CG;
             const int width_cta = (at.rows + STEP - 1) / STEP * 16;
