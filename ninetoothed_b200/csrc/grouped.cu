@@ -1133,6 +1133,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
         // Where requests meet in a tile its rows are many small boxes: one lane's copies of them took 2300 cycles a stage, over
         // twice the products' time.  Four lanes share them: the halves of a stage, and every other box.
         const int sub = (warp - ROW_WARP) & 1, turn = (warp - ROW_WARP) >> 1;
+        constexpr int BOXES = S::ROWS_CTA / 16 / 2;  // most of one lane
         bool waited = false;
         const auto wait_parts = [&] {  // for the kernel before this one, under which this one starts
             griddepcontrol_wait();
@@ -1154,28 +1155,39 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
             const int width_cta = (last - first + STEP - 1) / STEP * 16;
             const int mine = first + static_cast<int>(cta_rank) * width_cta, mine_end = min(mine + width_cta, last);
             const int run_first = run_at(table, runs, first), run_mine = run_at(table, runs, mine);
+            // this lane's boxes, found once a tile (the walk of the requests costs as much as the copies): where each begins in
+            // lhs and in a stage, and, in the offset's last bits, how many rows it has
+            int box_row[BOXES], box_at[BOXES], boxes = 0, box = 0;
+            for (int r = run_mine; r < runs && table[r].tiles_before < mine_end; ++r) {
+                const Piece<STEP> piece(table[r], mine, mine_end);
+                const int row = piece.row(table[r]), count = piece.to - piece.from;
+                for (int c = 0; c < count; ++box) {
+                    const int size = count == S::ROWS_CTA ? S::ROWS_CTA : count - c >= 32 ? 32 : 16;
+                    if ((box & 1) == turn) {
+#pragma unroll
+                        for (int i = 0; i < BOXES; ++i)
+                            if (i == boxes) {
+                                box_row[i] = row + c;
+                                box_at[i] = (piece.from - mine + c) * ROW_BYTES + size;
+                            }
+                        ++boxes;
+                    }
+                    c += size;
+                }
+            }
             for (int kb = 0; kb < p.k_blocks; ++kb) {
                 mbar_wait(&ctl->empty[s], phase, wait_ctx, 0x120 | s);
-                uint8_t *dst = smem + s * S::STAGE_BYTES + S::W_BYTES;
+                uint8_t *dst = smem + s * S::STAGE_BYTES + S::W_BYTES + sub * S::X_BYTES;
                 const int k0 = kb * S::DEPTH + sub * BK;
-                int box = turn;  // boxes until this lane's next
-                for (int r = run_mine; r < runs && table[r].tiles_before < mine_end; ++r) {
-                    const Piece<STEP> piece(table[r], mine, mine_end);
-                    const int row = piece.row(table[r]), count = piece.to - piece.from;
-                    uint8_t *at = dst + sub * S::X_BYTES + (piece.from - mine) * ROW_BYTES;
-                    if (count == S::ROWS_CTA) {
-                        if (box == 0) load_2d<CG>(at, &map_x, &ctl->full[s], k0, row);
-                        box ^= 1;
-                    } else {
-                        int c = 0;
-                        for (; c + 32 <= count; c += 32, box ^= 1)
-                            if (box == 0) load_2d<CG>(at + c * ROW_BYTES, &map_x32, &ctl->full[s], k0, row + c);
-                        if (c < count) {
-                            if (box == 0) load_2d<CG>(at + c * ROW_BYTES, &map_x16, &ctl->full[s], k0, row + c);
-                            box ^= 1;
-                        }
+#pragma unroll
+                for (int i = 0; i < BOXES; ++i)
+                    if (i < boxes) {
+                        const int size = box_at[i] & (ROW_BYTES * 2 - 1);
+                        uint8_t *at = dst + (box_at[i] - size);
+                        if (size == 16) load_2d<CG>(at, &map_x16, &ctl->full[s], k0, box_row[i]);
+                        else if (size == 32) load_2d<CG>(at, &map_x32, &ctl->full[s], k0, box_row[i]);
+                        else load_2d<CG>(at, &map_x, &ctl->full[s], k0, box_row[i]);
                     }
-                }
                 next();
             }
             for (int r = run_first; r < runs && table[r].tiles_before < last; ++r) {
