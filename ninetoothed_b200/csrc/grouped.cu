@@ -1937,18 +1937,19 @@ int launch_grouped(cudaStream_t stream, const DeviceState &dev, int dtype, Param
 int64_t low_chunks(int64_t k) { return (k + LOW_CHUNK - 1) / LOW_CHUNK; }
 
 // Few rows, or requests of few rows each: the adapters' part costs no tile of its own and runs under the streaming of rhs, a
-// row at a time (0.05 to 0.15 us a row).  Otherwise every request of a tile costs the tensor cores' issuer about half a
-// microsecond, whatever its length, and every 32 ranks more of it as much again or less.  4096 x 4096, rank 16, this way
-// against the other: 64 rows in 64 requests 19 against 46 us, in 4 requests 19 / 29; 256 rows in 256 requests 48 / 95, in 16
-// requests 45 / 33; 512 rows in 512 requests 97 / 125, in 128 requests 91 / 62.
-bool few_rows(int64_t rows, int64_t rank, int64_t requests) {
-    const int64_t blocks = (rank + RANK_BLOCK - 1) / RANK_BLOCK;
-    return rank <= FEW_RANK && (rows <= 64 || (rows <= FEW_ROWS && rows - 64 < requests * (1 + blocks)));
+// row at a time: 0.05 to 0.35 us a row, by the rank.  Otherwise a request takes at least 16 columns of a tile, whatever its
+// rows, and its second product half a microsecond of that tile.  What is hidden under the streaming of rhs, short for a small
+// k, is why the rank is weighed against k.  us this way / the other (rows in requests):
+//   4096 x 4096, rank 16: 16 in 1 15 / 24, 64 in 64 19 / 63, 256 in 64 48 / 64, in 16 47 / 32, 512 in 128 97 / 115, in 64 96 / 64
+//   4096 x 4096, rank 64: 1 in 1 16 / 25, 16 in 4 20 / 29, 64 in 64 37 / 74, 64 in 4 36 / 29
+//   1024 x 2048, rank 64: 1 in 1 21 / 12, 64 in 64 31 / 28, 128 in 128 30 / 42, in 32 29 / 25, 512 in 256 84 / 84
+bool few_rows(int64_t rows, int64_t k, int64_t rank, int64_t requests) {
+    return rank <= FEW_RANK && rows <= FEW_ROWS && rows * rank < requests * (rank + 48) + (k >= 32 * rank ? 2048 : -64 * 48);
 }
 
 size_t lora_workspace(int64_t rows, int64_t k, int64_t rank) {
     const size_t parts = static_cast<size_t>(rows) * ((rank + RANK_BLOCK - 1) / RANK_BLOCK) * RANK_BLOCK * 4;
-    const size_t sums = few_rows(rows, rank, rows) ? static_cast<size_t>(low_chunks(k)) * rows * rank * 4 : 0;
+    const size_t sums = few_rows(rows, k, rank, rows) ? static_cast<size_t>(low_chunks(k)) * rows * rank * 4 : 0;
     return std::max(parts, sums);
 }
 
@@ -2231,7 +2232,7 @@ int run_lora(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothe
         p.out_stride0 = output.strides[0];
         p.out_stride1 = output.strides[1];
         p.out_vec = output_vec(output);
-        if (few_rows(rows, rank, runs))
+        if (any ? few_rows(rows, k, rank, std::min(runs, rows)) : rows <= SPLIT_NT)
             return launch_few(stream, *dev, dtype, p, lhs.data, lhs.strides[0], shared, first, second, static_cast<float *>(workspace));
         return launch_many(stream, *dev, dtype, p, lhs.data, lhs.strides[0], shared, first, second, workspace);
     }

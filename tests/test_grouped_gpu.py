@@ -296,7 +296,7 @@ def test_lora_matmul_transposed_views(turned):
 
 
 @pytest.mark.parametrize("turned", [(False, False), (False, True), (True, False), (True, True)])
-@pytest.mark.parametrize("k, n, rank", [(2056, 136, 24), (4104, 130, 20), (72, 264, 128), (264, 8, 8)])
+@pytest.mark.parametrize("k, n, rank", [(2056, 136, 24), (4104, 130, 20), (72, 264, 128), (264, 8, 8), (4104, 136, 128)])
 def test_lora_matmul_few_rows(k, n, rank, turned):
     """Single rows under adapters, whose matrices lie either way round, in wider tensors, ragged in every size."""
     lengths, adapters = [1] * 30 + [0, 5, 3], [i % 6 - 1 for i in range(33)]
