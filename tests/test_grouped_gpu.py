@@ -380,6 +380,22 @@ def test_a_broken_adapter_stays_with_its_requests():
         broken[1] = kept
 
 
+@pytest.mark.parametrize("rank", [24, 40])
+@pytest.mark.parametrize("lengths", [[3, 5], [200, 70]], ids=str)
+def test_an_infinite_row_stays_infinite(lengths, rank):
+    """Positive matrices: a row that holds an infinity is infinite in every column, none of it NaN, and no other row is."""
+    lhs, rhs, down, up, scales, offsets, which = lora_inputs(lengths, [1, 0], 136, 264, rank, 2, torch.float16)
+    lhs, rhs, down, up = lhs.abs(), rhs.abs(), down.abs(), up.abs()
+    lhs[1, 17] = float("inf")
+    from ninetoothed_b200.torch_ops import ops
+
+    output = torch.zeros(lhs.shape[0], 264, dtype=torch.float16, device="cuda")
+    ops.lora_matmul(lhs, rhs, down, up, scales, offsets, which, output)
+    assert (output[1] == float("inf")).all()
+    output[1] = 0
+    assert output.isfinite().all()
+
+
 def test_lora_matmul_workspace_of_the_caller():
     from ninetoothed_b200 import _capi
 
