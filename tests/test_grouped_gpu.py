@@ -510,6 +510,48 @@ def test_an_expert_layer_forward_and_backward():
     assert (eager["y"][:held].double() - y).norm() <= 2 * 2.0 ** -8 * y.norm()
 
 
+@pytest.mark.parametrize("lengths", [[1, 0, 3, 2], [130, 0, 260, 31], [900, 700, 45]], ids=str)
+def test_calls_in_a_row_share_a_workspace(lengths):
+    """A call on the output of the one before, with and without adapters in between, all through one workspace, captured and
+    replayed on other bounds: what the same calls give with the device idle between them, bit for bit."""
+    from ninetoothed_b200 import _capi
+
+    x, w, down, up, scales, offsets, which = lora_inputs(lengths, [i % 3 - (i == 1) for i in range(len(lengths))], 264, 264, 40, 3,
+                                                         torch.bfloat16)
+    bare = torch.full_like(which, -1)
+    size = _capi.lora_matmul_workspace_size(x, down)
+
+    def chain(workspace, outputs, idle):
+        at = x
+        for i, output in enumerate(outputs):
+            _capi.lora_matmul(at, w, down, up, scales, offsets, bare if i == 2 else which, output, workspace=workspace)
+            at = output
+            if idle:
+                torch.cuda.synchronize()
+
+    def outputs():
+        return [torch.zeros_like(x) for _ in range(6)]
+
+    captured, workspace = outputs(), torch.zeros(size, dtype=torch.uint8, device="cuda")
+    chain(workspace, captured, idle=True)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+        chain(workspace, captured, idle=False)
+    torch.cuda.current_stream().wait_stream(stream)
+    for shift in (0, 1, 2):
+        offsets.copy_(bounds_of(lengths, first=shift))
+        expected = outputs()
+        chain(torch.zeros(size, dtype=torch.uint8, device="cuda"), expected, idle=True)
+        workspace.fill_(255)  # (NaN, were it read before it is written)
+        for output in captured:
+            output.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for i, (got, want) in enumerate(zip(captured, expected)):
+            assert torch.equal(got, want), i
+
+
 def test_two_streams_at_once():
     """Calls in flight on two streams, the adapters' workspaces among them, give what each gives alone."""
     args = [lora_inputs([400, 300, 1], [i, 1 - i, i], 520, 1032, 40, 2, torch.bfloat16) for i in range(2)]
