@@ -50,8 +50,7 @@ constexpr int GRAD_THREADS = NUM_THREADS + 32;  // and a warp that clears what a
 enum Job { JOB_PRODUCT, JOB_PARTS, JOB_FEW };  // of turned_kernel
 
 constexpr int SPLIT_NT = 64;   // rows of a tile whose reduction a cluster shares
-constexpr int FEW_ROWS = 1024;  // rows of a call whose adapters' part may be computed a row at a time (see few_rows)
-constexpr int FEW_RANK = 128;  // largest rank there
+constexpr int FEW_RANK = 128;  // largest rank whose adapters' part may be computed a row at a time (see few_rows)
 constexpr int LOW_WARPS = 8;
 constexpr int LOW_CHUNK = LOW_WARPS * 256;  // terms of a partial sum of (lhs . down) there
 constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product elsewhere: 32 high parts, 32 low parts
@@ -1015,7 +1014,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 //
 // What bounds it: for long requests the products of the projection and the board's power, as in turned_kernel: 8192 rows of 6
 // requests, 4096 x 4096, rank 32, take 238 us back to back (1.17 PFLOP/s), some 15 of them the launch before, which reads lhs
-// once more.  For short ones the padding: 2048 rows of 256 requests take 208 us, of 64 94.  Small calls are latency: of the 33 us of
+// once more.  For short ones the padding (rank 16): 2048 rows of 256 requests take 208 us, of 64 94.  Small calls are latency: of the 33 us of
 // 1533 rows of 40 requests (1000 x 2056, rank 24) 10 are the launch before, 5 this one's table and first copies.
 // ---------------------------------------------------------------------------
 // The columns [from, to) of the padded space that a run of the table (tiles_before: its first column) has in [low, high).
@@ -1954,19 +1953,21 @@ int launch_grouped(cudaStream_t stream, const DeviceState &dev, int dtype, Param
 int64_t low_chunks(int64_t k) { return (k + LOW_CHUNK - 1) / LOW_CHUNK; }
 
 // Few rows, or requests of few rows each: the adapters' part costs no tile of its own and runs under the streaming of rhs, a
-// row at a time: 0.05 to 0.35 us a row, by the rank.  Otherwise a request takes at least 16 columns of a tile, whatever its
+// row at a time: 0.05 to 0.4 us a row, by the rank.  Otherwise a request takes at least 16 columns of a tile, whatever its
 // rows, and its second product half a microsecond of that tile.  What is hidden under the streaming of rhs, short for a small
 // k, is why the rank is weighed against k.  us this way / the other (rows in requests):
-//   4096 x 4096, rank 16: 16 in 1 15 / 24, 64 in 64 19 / 63, 256 in 64 48 / 64, in 16 47 / 32, 512 in 128 97 / 115, in 64 96 / 64
+//   4096 x 4096, rank 16: 16 in 1 15 / 24, 64 in 64 19 / 63, 256 in 64 48 / 64, in 16 47 / 32, 512 in 128 97 / 115, in 64 96 / 64,
+//   2048 in 2048 492 / 1616, 4096 in 2048 969 / 1632, 8192 in 2048 1912 / 1638
+//   4096 x 1024, rank 8: 2048 in 2048 170 / 669, 8192 in 2048 584 / 679
 //   4096 x 4096, rank 64: 1 in 1 16 / 25, 16 in 4 20 / 29, 64 in 64 37 / 74, 64 in 4 36 / 29
 //   1024 x 2048, rank 64: 1 in 1 21 / 12, 64 in 64 31 / 28, 128 in 128 30 / 42, in 32 29 / 25, 512 in 256 84 / 84
 bool few_rows(int64_t rows, int64_t k, int64_t rank, int64_t requests) {
-    return rank <= FEW_RANK && rows <= FEW_ROWS && rows * rank < requests * (rank + 48) + (k >= 32 * rank ? 2048 : -64 * 48);
+    return rank <= FEW_RANK && rows * rank < requests * (rank + 48) + (k >= 32 * rank ? 2048 : -64 * 48);
 }
 
 size_t lora_workspace(int64_t rows, int64_t k, int64_t rank) {
     const size_t parts = static_cast<size_t>(rows) * ((rank + RANK_BLOCK - 1) / RANK_BLOCK) * RANK_BLOCK * 4;
-    const size_t sums = few_rows(rows, k, rank, rows) ? static_cast<size_t>(low_chunks(k)) * rows * rank * 4 : 0;
+    const size_t sums = few_rows(rows, k, rank, std::min<int64_t>(rows, MAX_RUNS)) ? static_cast<size_t>(low_chunks(k)) * rows * rank * 4 : 0;
     return std::max(parts, sums);
 }
 

@@ -320,6 +320,11 @@ def test_lora_matmul_many_requests_and_wide_indices():
     lengths = [i % 3 for i in range(2048)]
     args = lora_inputs(lengths, [(i * 7) % 40 - 2 for i in range(2048)], 128, 136, 16, 36, torch.float16)
     run_lora(*args[:5], args[5].long(), args[6].long())
+    # of a rank that goes a tile at a time whatever the requests, and more rows in as many requests
+    args = lora_inputs(lengths, [(i * 7) % 40 - 2 for i in range(2048)], 128, 136, 136, 36, torch.bfloat16)
+    run_lora(*args[:5], args[5].long(), args[6].long())
+    lengths = [i % 5 for i in range(2048)]
+    run_lora(*lora_inputs(lengths, [(i * 7) % 40 - 2 for i in range(2048)], 520, 136, 16, 36, torch.bfloat16))
 
 
 # Grids that take every worker through five or more tiles, so that accumulators, stages and their barriers come round:
