@@ -8,9 +8,9 @@
 // Nothing is read back to the host: every CTA turns the offsets into a table of runs in shared memory (bounds are
 // clamped by a running maximum, so no offsets can lead out of the tensors) and walks the tiles that follow from it.
 //
-// The kernels share a skeleton: persistent CTAs (or CTA pairs) of eleven warps, two that copy an operand each with TMA, one
-// that issues tcgen05.mma, eight that drain the accumulator; a ring of shared-memory stages; two accumulator buffers in
-// tensor memory, so that a tile's epilogue runs under the next tile's products.
+// The kernels share a skeleton: persistent CTAs (or CTA pairs) of eleven warps or a few more, at least two that copy an operand
+// each with TMA, one that issues tcgen05.mma, eight that drain the accumulator; a ring of shared-memory stages; two accumulator
+// buffers in tensor memory, so that a tile's epilogue runs under the next tile's products.
 //   turned_kernel   the grouped product (matrix columns are the accumulator's rows), the adapters' first product, and the
 //                   whole of lora_matmul for few rows (with low_kernel before it)
 //   lora_kernel     lora_matmul for many rows
