@@ -2237,8 +2237,9 @@ int run_lora(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothe
     p.bf16 = dtype == NINETOOTHED_BFLOAT16;
     p.scales = static_cast<const float *>(scales.data);
     p.scales_stride = scales.strides[0];
-    p.rank = static_cast<int>(rank);
-    p.rank_blocks = static_cast<int>((rank + RANK_BLOCK - 1) / RANK_BLOCK);
+    // (without adapters the shapes' rank says nothing: no kernel may size or fill anything by it)
+    p.rank = any ? static_cast<int>(rank) : 0;
+    p.rank_blocks = (p.rank + RANK_BLOCK - 1) / RANK_BLOCK;
     p.status = dev->status;
     const Matrices shared{rhs.data, 1, k, n, 0, rhs.strides[0], rhs.strides[1]};
     const Matrices first{down.data, count, k, rank, down.strides[0], down.strides[1], down.strides[2]};

@@ -368,6 +368,14 @@ def test_lora_matmul_on_sizes_no_tensor_map_addresses_and_without_adapters():
     run_lora(args[0], args[1], args[2][:0], args[3][:0], args[4][:0], *args[5:])
 
 
+@pytest.mark.parametrize("rows", [64, 65])
+@pytest.mark.parametrize("k, n", [(64, 72), (264, 9608)])
+def test_lora_matmul_an_empty_pool_of_a_large_rank(k, n, rows):
+    """No adapters at all, but shapes that give them a rank beyond what the few-row kernel holds a row's values of."""
+    args = lora_inputs([rows - 24, 24], [1, 0], k, n, 256, 2, torch.bfloat16, padding=0)
+    run_lora(args[0], args[1], args[2][:0], args[3][:0], args[4][:0], *args[5:])
+
+
 def test_a_broken_adapter_stays_with_its_requests():
     lhs, rhs, down, up, scales, offsets, which = lora_inputs([5, 20, 1, 40, 3], [0, 1, 2, 1, 0], 128, 136, 16, 3, torch.bfloat16)
     clean = run_lora(lhs, rhs, down, up, scales, offsets, which)
