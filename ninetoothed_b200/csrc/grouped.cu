@@ -44,7 +44,8 @@ constexpr size_t MAX_SMEM = 227 * 1024;
 constexpr int EPILOGUE_WARPS = 8;
 constexpr int ROW_WARP = 2 + EPILOGUE_WARPS;
 constexpr int NUM_THREADS = (ROW_WARP + 1) * 32;
-constexpr int LORA_THREADS = NUM_THREADS + 3 * 32;  // and three more producers of rows
+constexpr int ROW_PRODUCERS = 4;  // of lora_kernel
+constexpr int LORA_THREADS = NUM_THREADS + (ROW_PRODUCERS - 1) * 32;
 constexpr int GRAD_THREADS = NUM_THREADS + 32;  // and a warp that clears what a run's last block holds of the next run
 
 enum Job { JOB_PRODUCT, JOB_PARTS, JOB_FEW };  // of turned_kernel
@@ -55,6 +56,8 @@ constexpr int LOW_WARPS = 8;
 constexpr int LOW_CHUNK = LOW_WARPS * 256;  // terms of a partial sum of (lhs . down) there
 constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product elsewhere: 32 high parts, 32 low parts
 
+// A wait on a barrier tells a phase from the next one only, so no lane that goes through the ring of stages may fall a whole
+// round behind: every producer has a part in `full`, by bytes that it copies into the stage or by arriving.
 struct Control {
     uint64_t full[MAX_STAGES];
     uint64_t empty[MAX_STAGES];
@@ -1060,7 +1063,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&ctl->full[s], 1);
+            mbar_init(&ctl->full[s], 1 + ROW_PRODUCERS * CG);
             mbar_init(&ctl->empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -1153,7 +1156,9 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
             waited = true;
         };
         uint32_t s = 0, phase = 1;
-        const auto next = [&] {
+        const auto next = [&] {  // (a stage that a lane copies nothing of may not be filled and emptied without it: see Control)
+            if (leader) mbar_arrive(&ctl->full[s]);
+            else mbar_arrive_cluster(&ctl->full[s], 0);
             if (++s == STAGES) {
                 s = 0;
                 phase ^= 1;

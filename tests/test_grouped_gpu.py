@@ -356,6 +356,14 @@ def test_lora_matmul_many_tiles_a_worker(lengths, k, n, rank, turned):
     run_lora(*args)
 
 
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+def test_lora_matmul_many_ranks_a_tile(kind):
+    """Tiles of one stage of the projection and twenty of an adapter's ranks, which most of the lanes that bring rows have no
+    part in: none may be left behind."""
+    lengths, which = [3000, 2500, 70, 1100], [1, 0, -1, 2]
+    run_lora(*lora_inputs(lengths, which, 72, 2056, 640, 3, kind))
+
+
 def test_lora_matmul_on_sizes_no_tensor_map_addresses_and_without_adapters():
     with warnings.catch_warnings():
         warnings.simplefilter("ignore")
