@@ -773,9 +773,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             const int row0 = at.row0 + (CG == 1 ? 0 : static_cast<int>(cta_rank) * width_cta);
             const int n0 = at.col0 + (CG == 1 ? 0 : static_cast<int>(cta_rank) * BM);
             const int boxes = (width_cta + A_CHUNK_ROWS - 1) / A_CHUNK_ROWS;
-            // (64-column boxes wholly behind the matrix, as half of the tile is where down has few ranks, are not copied)
-            const int w_boxes = W_MN ? min(BM / 64, max(0, (p.n - n0 + 63) / 64)) : BM / 64;
-            const int w_boxes_other = CG == 1 ? 0 : W_MN ? min(BM / 64, max(0, (p.n - n0 - BM + 63) / 64)) : BM / 64;
+            // (64-column boxes wholly behind the matrix, as half of the tile is where down has few ranks, are not copied; but one
+            // is, so that this lane has a part in every stage)
+            const int w_boxes = W_MN ? min(BM / 64, max(1, (p.n - n0 + 63) / 64)) : BM / 64;
+            const int w_boxes_other = CG == 1 ? 0 : W_MN ? min(BM / 64, max(1, (p.n - n0 - BM + 63) / 64)) : BM / 64;
             const int bytes = (w_boxes + w_boxes_other) * (S::W_BYTES / (BM / 64)) + CG * S::SUB * boxes * (A_CHUNK_ROWS * BK * 2);
             for (int kb = kb_first; kb < kb_last; ++kb) {
                 mbar_wait(&ctl->empty[s], phase, wait_ctx, 0x100 | s);

@@ -338,6 +338,13 @@ def test_grouped_matmul_many_tiles_a_worker(lengths, k, n, transposed):
     run_grouped(lhs, rhs, bounds_of(lengths))
 
 
+@pytest.mark.parametrize("lengths, k", [([2048, 2500, 1536, 2100], 136), ([1500] * 8, 1032)], ids=["short", "long"])
+@pytest.mark.parametrize("n", [4104, 520, 264])
+def test_grouped_matmul_columns_end_in_a_pairs_first_half(lengths, k, n):
+    """The other half of the pair, which has no column of the last tile, keeps step with the ring of stages."""
+    run_grouped(normal(64, sum(lengths), k), normal(65, len(lengths), k, n), bounds_of(lengths))
+
+
 # (256 x 256 tiles on pairs; 128 x 128 ones take less than half a wave by their rule)
 @pytest.mark.parametrize("lengths", [[64, 100, 1, 0, 129, 31, 512, 7], [128] * 8], ids=str)
 def test_rhs_grad_many_tiles_a_worker(lengths):
