@@ -406,6 +406,32 @@ __device__ __forceinline__ void mbar_wait_cluster(uint64_t *bar, uint32_t parity
     }
 }
 
+// Bounded wait of a warp that issues products, by all of it together: one lane probes, the warp's vote says whether to go on.
+// (32 lanes probing one barrier are served one after the other.)
+template <bool CLUSTER = false>
+__device__ __forceinline__ void mbar_wait_together(uint64_t *bar, uint32_t parity, const WaitCtx &ctx, uint32_t code) {
+    const bool prober = (threadIdx.x & 31) == 0;
+    uint64_t start = 0;
+    for (uint32_t i = 0;; ++i) {
+        bool over = true;
+        if (prober) over = CLUSTER ? mbar_test_wait_cluster(bar, parity) : mbar_try_wait(bar, parity);
+        if (__all_sync(0xffffffffu, over)) break;
+        if (i < 64 || i % 32 != 0) continue;
+        if (prober) {
+            const uint64_t now = global_timer_ns();
+            if (start == 0) start = now;
+            const bool failed_before = *ctx.abort_flag != 0;
+            over = now - start > (failed_before ? WAIT_LIMIT_AFTER_FAILURE_NS : WAIT_LIMIT_NS);
+            if (over && !failed_before) {
+                *ctx.abort_flag = 1;
+                atomicCAS(ctx.status, 0u, STATUS_WAIT_TIMEOUT | (ctx.kernel_id << 16) | code);
+            }
+        }
+        if (__all_sync(0xffffffffu, over)) break;
+    }
+    __syncwarp();
+}
+
 __device__ __forceinline__ void griddepcontrol_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddepcontrol_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
@@ -761,10 +787,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     if (warp == 0 || warp == ROW_WARP) {
         // ------------- TMA producers: warp 0 the matrices, the last warp the rows -------------
         // (Lone lanes, in branches that no other lane of the warp enters: these loops go by values from shared memory, and in a
-        // warp that walked them together with one elected lane issuing, nothing would tell the compiler that it stays together.
-        // The issuer below can be an elected lane, 3 to 10% faster than a lone one, as its loops go by values known to be the
-        // warp's and it has no branch of that lane alone that holds more than one instruction.  In lora_kernel, whose issuer
-        // has such a loop, a commit behind it by an elected lane was seen to be issued twice.)
+        // warp that walked them together with one elected lane issuing, nothing would tell the compiler that it stays together.)
         uint32_t s = 0, phase = 1, tile_it = 0;
         for (W walk(p, table, ctl, worker, workers); lane == 0 && walk.more(); walk.advance(), ++tile_it) {
             const TurnedPlace at = walk.place(p);
@@ -820,8 +843,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
     } else if (warp == 1) {
         // ------------------------------- MMA issuer -------------------------------
+        // (The warp goes through the loop together: its branches are its votes and values known to be the warp's.  What one lane
+        // does alone is a single probe of a barrier, followed by a vote, or a stage's products and their commit, behind an
+        // election of their own and before a __syncwarp.  An earlier lora_kernel, whose issuer held one election through loops that
+        // the elected lane went through by itself, was seen to issue a commit twice.  Its issuer is a lone lane throughout.)
         if (leader) {
-            const bool issuer = elect_one();
             const uint32_t smem_base = smem_u32(smem);
             uint32_t s = 0, phase = 0, acc_it = 0;
             bool ready = false;
@@ -830,11 +856,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 constexpr int STEP = 16 * CG;
                 uint32_t idesc = 0;
                 const uint32_t buf = acc_it & 1;
-                mbar_wait_warp(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+                mbar_wait_together(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
                 tcgen05_fence_after_sync();
                 const uint32_t tmem_acc = tmem_base + buf * NT;
                 for (int kb = kb_first; kb < kb_last; ++kb) {
-                    if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x300 | s);
+                    if (!ready) mbar_wait_together(&ctl->full[s], phase, wait_ctx, 0x300 | s);
                     tcgen05_fence_after_sync();
                     if (kb == kb_first) {
                         const int rows = __shfl_sync(0xffffffffu, ctl->tile_rows[acc_it % MAX_STAGES], 0);
@@ -844,25 +870,25 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                     const uint32_t x_addr = w_addr + S::W_BYTES;
                     const uint32_t s_next = s + 1 == STAGES ? 0 : s + 1;
                     const uint32_t phase_next = s_next == 0 ? phase ^ 1 : phase;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < S::DEPTH / UMMA_K; ++kk) {
-                        const int sub = kk / (BK / UMMA_K), step = kk % (BK / UMMA_K);
-                        const uint64_t desc_w =
-                            W_MN ? umma_smem_desc(w_addr + kk * (UMMA_K * 128), S::DEPTH * 128, 1024)
-                                 : umma_smem_desc(w_addr + sub * A_STAGE_BYTES + step * (UMMA_K * 2), 16, 1024);
-                        const uint64_t desc_x = umma_smem_desc(x_addr + sub * S::X_BYTES + step * (UMMA_K * 2), 16, 1024);
-                        if (issuer) umma_ss<CG>(tmem_acc, desc_w, desc_x, idesc, (kb != kb_first || kk != 0) ? 1u : 0u);
-                        if (kk == S::DEPTH / UMMA_K / 2 - 1)
-                            ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
-                    }
-                    if (issuer) {
+                        for (int kk = 0; kk < S::DEPTH / UMMA_K; ++kk) {
+                            const int sub = kk / (BK / UMMA_K), step = kk % (BK / UMMA_K);
+                            const uint64_t desc_w =
+                                W_MN ? umma_smem_desc(w_addr + kk * (UMMA_K * 128), S::DEPTH * 128, 1024)
+                                     : umma_smem_desc(w_addr + sub * A_STAGE_BYTES + step * (UMMA_K * 2), 16, 1024);
+                            const uint64_t desc_x = umma_smem_desc(x_addr + sub * S::X_BYTES + step * (UMMA_K * 2), 16, 1024);
+                            umma_ss<CG>(tmem_acc, desc_w, desc_x, idesc, (kb != kb_first || kk != 0) ? 1u : 0u);
+                        }
                         if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
                         else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
                     }
+                    __syncwarp();
+                    ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
                     s = s_next;
                     phase = phase_next;
                 }
-                if (issuer) {
+                if (elect_one()) {
                     if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
                     else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
                 }
@@ -1521,7 +1547,6 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
     } else if (warp == 1) {
         // ------------------------------- MMA issuer -------------------------------
         const uint32_t idesc = umma_instr_desc(BM * CG, BN, p.bf16 != 0, true, true);
-        const bool issuer = elect_one();
         const uint32_t smem_base = smem_u32(smem);
         uint32_t s = 0, phase = 0, acc_it = 0, clean_phases = 0;  // (a bit a stage: not every use of a stage is ragged)
         bool ready = false;
@@ -1530,16 +1555,15 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
             if (length == 0) continue;  // (the epilogue stores zeros by itself)
             const int blocks = (length + BK - 1) / BK;
             const uint32_t buf = acc_it & 1;
-            mbar_wait_warp(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
+            mbar_wait_together(&ctl->tmem_empty[buf], ((acc_it >> 1) & 1) ^ 1, wait_ctx, 0x200 | buf);
             ++acc_it;
             tcgen05_fence_after_sync();
             const uint32_t tmem_acc = tmem_base + buf * BN;
             for (int kb = 0; kb < blocks; ++kb) {
-                if (!ready) mbar_wait_warp(&ctl->full[s], phase, wait_ctx, 0x300 | s);
+                if (!ready) mbar_wait_together(&ctl->full[s], phase, wait_ctx, 0x300 | s);
                 const int left = length - kb * BK;
                 if (left < BK && (left & (UMMA_K - 1)) != 0) {
-                    if (lane == 0) mbar_wait_cluster(&ctl->clean[s], (clean_phases >> s) & 1, wait_ctx, 0x700 | s);
-                    __syncwarp();
+                    mbar_wait_together<true>(&ctl->clean[s], (clean_phases >> s) & 1, wait_ctx, 0x700 | s);
                     clean_phases ^= 1u << s;
                 }
                 tcgen05_fence_after_sync();
@@ -1548,22 +1572,22 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
                 const uint32_t b_addr = a_addr + A_STAGE_BYTES;
                 const uint32_t s_next = s + 1 == STAGES ? 0 : s + 1;
                 const uint32_t phase_next = s_next == 0 ? phase ^ 1 : phase;
+                if (elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-                    const uint64_t desc_a = umma_smem_desc(a_addr + kk * (UMMA_K * 128), S::BOX_BYTES, 1024);
-                    const uint64_t desc_b = umma_smem_desc(b_addr + kk * (UMMA_K * 128), S::BOX_BYTES, 1024);
-                    if (issuer && kk < steps) umma_ss<CG>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
-                    if (kk == BK / UMMA_K / 2 - 1)
-                        ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
-                }
-                if (issuer) {
+                    for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                        const uint64_t desc_a = umma_smem_desc(a_addr + kk * (UMMA_K * 128), S::BOX_BYTES, 1024);
+                        const uint64_t desc_b = umma_smem_desc(b_addr + kk * (UMMA_K * 128), S::BOX_BYTES, 1024);
+                        if (kk < steps) umma_ss<CG>(tmem_acc, desc_a, desc_b, idesc, (kb != 0 || kk != 0) ? 1u : 0u);
+                    }
                     if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
                     else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
                 }
+                __syncwarp();
+                ready = __all_sync(0xffffffffu, mbar_test_wait(&ctl->full[s_next], phase_next));
                 s = s_next;
                 phase = phase_next;
             }
-            if (issuer) {
+            if (elect_one()) {
                 if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
                 else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
             }

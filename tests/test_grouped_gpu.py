@@ -580,6 +580,29 @@ def test_calls_in_a_row_share_a_workspace(lengths):
             assert torch.equal(got, want), i
 
 
+def test_calls_repeat_themselves():
+    """Every call of the same inputs gives the same bits, also where every worker has many ragged tiles."""
+    from ninetoothed_b200.torch_ops import ops
+
+    lengths = [(i * 37) % 150 for i in range(64)]
+    rows, offsets = sum(lengths), bounds_of(lengths)
+    lhs, rhs, grad = normal(101, rows, 520), normal(102, 64, 520, 1032), normal(103, rows, 1032)
+    down, up = normal(104, 4, 520, 40), normal(105, 4, 40, 1032)
+    scales, which = torch.ones(4, device="cuda"), torch.arange(64, device="cuda") % 5 - 1
+    product, rhs_grad, beside = torch.zeros_like(grad), torch.empty_like(rhs), torch.zeros_like(grad)
+    first = None
+    for _ in range(30):
+        for t in (product, rhs_grad, beside):
+            t.fill_(float("nan"))
+        ops.grouped_matmul(lhs, rhs, offsets, product)
+        ops.grouped_matmul_rhs_grad(lhs, grad, offsets, rhs_grad)
+        ops.lora_matmul(lhs, rhs[0], down, up, scales, offsets, which, beside)
+        if first is None:
+            first = [t.clone() for t in (product, rhs_grad, beside)]
+        for got, want in zip((product, rhs_grad, beside), first):
+            assert torch.equal(got, want)
+
+
 def test_two_streams_at_once():
     """Calls in flight on two streams, the adapters' workspaces among them, give what each gives alone."""
     args = [lora_inputs([400, 300, 1], [i, 1 - i, i], 520, 1032, 40, 2, torch.bfloat16) for i in range(2)]
