@@ -432,6 +432,11 @@ __device__ __forceinline__ void mbar_wait_together(uint64_t *bar, uint32_t parit
     __syncwarp();
 }
 
+// An arrival at the even CTA's barrier that tells of no writes.  (As a release it would have this lane wait for its copies' issue.)
+__device__ __forceinline__ void arrive_leader(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_address(bar, 0)) : "memory");
+}
+
 __device__ __forceinline__ void griddepcontrol_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddepcontrol_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
@@ -1185,7 +1190,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
         uint32_t s = 0, phase = 1;
         const auto next = [&] {  // (a stage that a lane copies nothing of may not be filled and emptied without it: see Control)
             if (leader) mbar_arrive(&ctl->full[s]);
-            else mbar_arrive_cluster(&ctl->full[s], 0);
+            else arrive_leader(&ctl->full[s]);
             if (++s == STAGES) {
                 s = 0;
                 phase ^= 1;
