@@ -1295,8 +1295,18 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
                     s = s_next;
                     phase = phase_next;
                 }
+                // (Products of one shape into the same accumulator follow one another in the order of their issue, products of
+                // different shapes need not: the second products wait until the projection's have ended, which is when its
+                // last stage is empty.)
+                bool ended = false;
+                const uint32_t s_last = s == 0 ? STAGES - 1 : s - 1, phase_last = s == 0 ? phase ^ 1 : phase;
                 for (int r = run_at(table, runs, first); r < runs && table[r].tiles_before < last; ++r) {
                     if (table[r].matrix < 0) continue;
+                    if (!ended) {
+                        mbar_wait(&ctl->empty[s_last], phase_last, wait_ctx, 0x800 | s_last);
+                        tcgen05_fence_after_sync();
+                        ended = true;
+                    }
                     const Piece<STEP> piece(table[r], first, last);
                     const uint32_t idesc_up = umma_instr_desc(BM * CG, piece.to - piece.from, p.bf16 != 0, p.up_mn != 0, false);
                     const uint32_t tmem_piece = tmem_acc + (piece.from - first);
