@@ -214,8 +214,8 @@ NineToothedResult launch_grouped_matmul_rhs_grad(NineToothedStream stream, NineT
  * another request's rows.  The gradient towards lhs is the same call on transposed views, with up and down
  * in each other's place.
  *
- * Sums are fp32.  scales[a] * (lhs[t] . down[a]) is kept between the two products as the sum of two numbers
- * of `dtype` (in fp16 it overflows beyond 65504).  `workspace` is device memory of at least
+ * Sums are fp32.  scales[a] * (lhs[t] . down[a]) keeps the range of fp32 between the two products, to 2^-22 of itself in
+ * fp16 and 2^-16 in bf16 at least, however many rows a call has.  `workspace` is device memory of at least
  * launch_lora_matmul_workspace_size(lhs, down) bytes, 256-byte aligned, free to reuse once the stream has
  * passed this call; calls that may overlap need one each.
  */

@@ -45,7 +45,9 @@ constexpr int EPILOGUE_WARPS = 8;
 constexpr int ROW_WARP = 2 + EPILOGUE_WARPS;
 constexpr int NUM_THREADS = (ROW_WARP + 1) * 32;
 constexpr int ROW_PRODUCERS = 4;  // of lora_kernel
-constexpr int LORA_THREADS = NUM_THREADS + (ROW_PRODUCERS - 1) * 32;
+constexpr int SPLIT_WARP = ROW_WARP + ROW_PRODUCERS;
+constexpr int SPLITTERS = 4;  // warps of lora_kernel that make fp16 adapters' operands from what the copies bring
+constexpr int lora_threads(bool wide) { return (SPLIT_WARP + (wide ? SPLITTERS : 0)) * 32; }
 constexpr int GRAD_THREADS = NUM_THREADS + 32;  // and a warp that clears what a run's last block holds of the next run
 
 enum Job { JOB_PRODUCT, JOB_PARTS, JOB_FEW };  // of turned_kernel
@@ -54,7 +56,8 @@ constexpr int SPLIT_NT = 64;   // rows of a tile whose reduction a cluster share
 constexpr int FEW_RANK = 128;  // largest rank whose adapters' part may be computed a row at a time (see few_rows)
 constexpr int LOW_WARPS = 8;
 constexpr int LOW_CHUNK = LOW_WARPS * 256;  // terms of a partial sum of (lhs . down) there
-constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product elsewhere: 32 high parts, 32 low parts
+constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product elsewhere: one 128-byte swizzle row of
+                               // their values, which are pairs of bf16 (32 high parts, 32 low parts) or 32 bits wide
 
 // A wait on a barrier tells a phase from the next one only, so no lane that goes through the ring of stages may fall a whole
 // round behind: every producer has a part in `full`, by bytes that it copies into the stage or by arriving.
@@ -64,8 +67,8 @@ struct Control {
     uint64_t tmem_full[2];
     uint64_t tmem_empty[2];
     uint64_t partials;
-    uint64_t ragged[MAX_STAGES];
-    uint64_t clean[MAX_STAGES];
+    uint64_t raw[MAX_STAGES];    // copies that warps of the CTA have to work on before products may read them
+    uint64_t clean[MAX_STAGES];  // ... and that they have
     int tile_rows[MAX_STAGES];  // rows of the tiles whose stages are in the ring
     uint32_t tmem_base;
     uint32_t abort_flag;
@@ -262,9 +265,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
     return packed;
 }
 
-__device__ __forceinline__ float round16(float v, bool bf16) {
-    return bf16 ? __bfloat162float(__float2bfloat16_rn(v)) : __half2float(__float2half_rn(v));
-}
+// A value as two numbers of eight bits each.
+struct Bf16Parts {
+    float high, low;
+    __device__ explicit Bf16Parts(float v) : high(__bfloat162float(__float2bfloat16_rn(v))) {
+        // (an infinite or NaN high part says it all; inf - inf must not turn it into NaN)
+        low = isfinite(high) ? v - high : 0.f;
+    }
+};
 
 __device__ __forceinline__ void store16(void *out, int64_t at, float v, bool bf16) {
     if (bf16) static_cast<__nv_bfloat16 *>(out)[at] = __float2bfloat16_rn(v);
@@ -724,9 +732,10 @@ __device__ __forceinline__ void store_turned(const uint32_t (&acc)[32], void *ou
     }
 }
 
-// JOB_PARTS: a run's adapter's down is the matrix, and scales (lhs . down) leaves as two 16-bit parts, in blocks of 32 ranks:
-// 32 high parts, 32 low parts (value = high + low to twice the type's precision, so that the second product runs on the
-// tensor cores without the rounding of one 16-bit operand).  Ranks behind the last are zero (of an infinite row or scale too).
+// JOB_PARTS: a run's adapter's down is the matrix, and scales (lhs . down) leaves in blocks of 32 ranks, 32 bits a rank: of fp16
+// operands as it is, of bf16 ones as 32 high parts and 32 low parts (value = high + low to 2^-16, so that the second product runs
+// on the tensor cores without the rounding of one 16-bit operand; bf16 has the range of fp32, fp16 has not).  Ranks behind the
+// last are zero (of an infinite row or scale too).
 // JOB_FEW: the shared projection and the adapters of a call with few rows.  The epilogue's warps, idle while the tile's
 // products run, compute the adapters' part of the rows that their CTA will store, (lhs . down) . up in fp32, and put it
 // where the CTA's own partial sums are added to it.
@@ -950,18 +959,24 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                         store_remote(remote_address(dst, cta), v);
                     }
                 } else if constexpr (PARTS) {
-                    if (n - lane < n_end) {
+                    if (n - lane < n_end && bf16) {
                         uint32_t low_part[32];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const float v = n < p.n ? scale * __uint_as_float(acc[j]) : 0.f, high = round16(v, bf16);
-                            acc[j] = __float_as_uint(v);
-                            // (an infinite or NaN high part says it all; inf - inf must not turn it into NaN)
-                            low_part[j] = __float_as_uint(isfinite(high) ? v - high : 0.f);
+                            const float v = n < p.n ? scale * __uint_as_float(acc[j]) : 0.f;
+                            const Bf16Parts parts(v);
+                            acc[j] = __float_as_uint(parts.high);
+                            low_part[j] = __float_as_uint(parts.low);
                         }
-                        uint16_t *block = static_cast<uint16_t *>(p.out) + n / 32 * 32;
-                        store_turned(acc, block, p.out_stride0, at.row0 + t0, at.rows - t0, at.row0 + t0 + 16, at.rows - t0 - 16, n, n_end, bf16);
-                        store_turned(low_part, block + 32, p.out_stride0, at.row0 + t0, at.rows - t0, at.row0 + t0 + 16, at.rows - t0 - 16, n, n_end, bf16);
+                        uint16_t *block = static_cast<uint16_t *>(p.out) + n / RANK_BLOCK * RANK_BLOCK;
+                        const int64_t pitch = 2 * p.out_stride0;
+                        store_turned(acc, block, pitch, at.row0 + t0, at.rows - t0, at.row0 + t0 + 16, at.rows - t0 - 16, n, n_end, true);
+                        store_turned(low_part, block + RANK_BLOCK, pitch, at.row0 + t0, at.rows - t0, at.row0 + t0 + 16, at.rows - t0 - 16, n, n_end, true);
+                    } else if (n - lane < n_end) {
+                        float *out = static_cast<float *>(p.out) + (at.row0 + t0) * p.out_stride0 + n;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (t0 + j < at.rows) out[j * p.out_stride0] = n < p.n ? scale * __uint_as_float(acc[j]) : 0.f;
                     }
                 } else if (p.out_vec) {
                     store_turned(acc, p.out, p.out_stride0, at.row0 + t0, at.rows - t0, at.row0 + t0 + 16, at.rows - t0 - 16, n, p.n, bf16);
@@ -997,10 +1012,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                             if (t + j >= last) break;
                             const int64_t row_at = (at.row0 + t + j) * p.out_stride0;
                             if constexpr (PARTS) {
-                                const float v = n < p.n ? scale * sum[j] : 0.f, high = round16(v, bf16);
-                                const int64_t to = row_at + n / RANK_BLOCK * (2 * RANK_BLOCK) + n % RANK_BLOCK;
-                                store16(p.out, to, v, bf16);
-                                store16(p.out, to + RANK_BLOCK, isfinite(high) ? v - high : 0.f, bf16);
+                                const float v = n < p.n ? scale * sum[j] : 0.f;
+                                if (bf16) {
+                                    const int64_t to = 2 * row_at + n / RANK_BLOCK * (2 * RANK_BLOCK) + n % RANK_BLOCK;
+                                    const Bf16Parts parts(v);
+                                    store16(p.out, to, parts.high, true);
+                                    store16(p.out, to + RANK_BLOCK, parts.low, true);
+                                } else {
+                                    static_cast<float *>(p.out)[row_at + n] = v;
+                                }
                             } else {
                                 store16(p.out, row_at + column_at, sum[j], bf16);
                             }
@@ -1044,8 +1064,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 // stand in a padded space of accumulator columns in which every request starts at a multiple of 16 (32); a tile is NT columns of
 // it, whatever requests they belong to, against 128 (256) columns of rhs.  Then, for every request with an adapter that has
 // columns in the tile, its second product is an ordinary product into just these columns, 32 ranks a stage: nothing of one
-// request's adapter, infinities and NaN included, meets another's columns.  (scales lhs . down comes in two 16-bit parts from
-// the launch before, under which this one starts.)
+// request's adapter, infinities and NaN included, meets another's columns.  (scales lhs . down) comes from the launch before, under
+// which this one starts.
+//
+// WIDE (fp16): two fp16 parts would hold neither values above 65504 nor the low parts of small ones, so the value comes in 32
+// bits, and four warps split it into two operands of eleven bits and eight of exponent (kind::tf32), and widen up to a third, once
+// the copies have landed.  Products of such operands take twice as long, and the tile's end waits for the warps: bf16, whose two
+// parts have the range of fp32, would lose 6 % by it at 8192 rows of 6 requests (4096 x 4096, rank 32: 239 and 254 us) and 15 % at
+// 4096 rows towards the input (4096 x 2048, rank 64: 81.5 and 93.8).
 //
 // What bounds it: for long requests the products of the projection and the board's power, as in turned_kernel: 8192 rows of 6
 // requests, 4096 x 4096, rank 32, take 238 us back to back (1.17 PFLOP/s), some 15 of them the launch before, which reads lhs
@@ -1061,6 +1087,59 @@ struct Piece {
     __device__ int row(const Run &run) const { return run.begin + from - run.tiles_before; }
 };
 
+// One operand of a second product, 128 columns of up and 32 ranks, in 32 bits as a K-major tile of 128-byte swizzle rows: exact for
+// either type.  `raw` holds the ranks as rows (MN: two boxes of 64 columns) or the columns (64 ranks each, the first 32 count).
+// Threads go through it in an order in which eight neighbours read and write different banks.
+template <bool MN>
+__device__ __forceinline__ void widen_up(const uint8_t *raw, uint8_t *wide, int thread, bool bf16) {
+    const auto put = [&](int column, int chunk, float a, float b, float c, float d) {  // four ranks of a column
+        *reinterpret_cast<float4 *>(wide + column * 128 + ((chunk ^ (column & 7)) << 4)) = make_float4(a, b, c, d);
+    };
+    if constexpr (MN) {  // four ranks of eight columns
+        static_assert(SPLITTERS * 32 == BM / 8 * RANK_BLOCK / 4, "one task a thread");
+        const int q = thread & 7, c = (thread >> 3) ^ (q >> 1);
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int rank = 4 * q + i;
+            v[i] = *reinterpret_cast<const uint4 *>(raw + (c >> 3) * (RANK_BLOCK * 128) + rank * 128 + (((c & 7) ^ (rank & 7)) << 4));
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const auto at = [&](const uint4 &w) { return half_of(j < 2 ? w.x : j < 4 ? w.y : j < 6 ? w.z : w.w, j & 1, bf16); };
+            put(c * 8 + j, q, at(v[0]), at(v[1]), at(v[2]), at(v[3]));
+        }
+    } else {  // eight ranks of a column
+#pragma unroll
+        for (int task = thread; task < BM * (RANK_BLOCK / 8); task += SPLITTERS * 32) {
+            const int column = task / 32 * 8 + (task & 7), c = (task >> 3) & 3;
+            const uint4 v = *reinterpret_cast<const uint4 *>(raw + column * 128 + ((c ^ (column & 7)) << 4));
+            put(column, 2 * c, half_of(v.x, 0, bf16), half_of(v.x, 1, bf16), half_of(v.y, 0, bf16), half_of(v.y, 1, bf16));
+            put(column, 2 * c + 1, half_of(v.z, 0, bf16), half_of(v.z, 1, bf16), half_of(v.w, 0, bf16), half_of(v.w, 1, bf16));
+        }
+    }
+}
+
+// The other operand, (scales lhs . down) of `rows` rows and 32 ranks, as two numbers of eleven bits each, which is what the
+// products keep of a 32-bit operand: the value's first eleven and the rest, rounded, 2^-22 of the value off at most.  The first
+// take the value's place, the second lie `second` bytes behind.
+__device__ __forceinline__ void split_low(uint8_t *values, int second, int rows, int thread) {
+    for (int i = thread; i < rows * (RANK_BLOCK / 4); i += SPLITTERS * 32) {
+        float4 *at = reinterpret_cast<float4 *>(values) + i;
+        const auto high_of = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xffffe000u); };
+        const auto rest_of = [](float v, float high) {
+            uint32_t rest;
+            asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(rest) : "f"(v - high));
+            return isfinite(v) ? __uint_as_float(rest) : 0.f;  // (an infinite or NaN value's first part says it all)
+        };
+        const float4 v = *at;
+        const float4 high = make_float4(high_of(v.x), high_of(v.y), high_of(v.z), high_of(v.w));
+        *at = high;
+        *reinterpret_cast<float4 *>(values + second + i * 16) =
+            make_float4(rest_of(v.x, high.x), rest_of(v.y, high.y), rest_of(v.z, high.z), rest_of(v.w, high.w));
+    }
+}
+
 // The run that holds a column.
 __device__ __forceinline__ int run_at(const Run *table, int runs, int column) {
     int low = 0, high = runs - 1;
@@ -1072,8 +1151,8 @@ __device__ __forceinline__ int run_at(const Run *table, int runs, int column) {
     return low;
 }
 
-template <int CG, int NT, bool W_MN>
-__global__ void __launch_bounds__(LORA_THREADS, 1)
+template <int CG, int NT, bool W_MN, bool WIDE>
+__global__ void __launch_bounds__(lora_threads(WIDE), 1)
     lora_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                 const __grid_constant__ CUtensorMap map_x32, const __grid_constant__ CUtensorMap map_x16,
                 const __grid_constant__ CUtensorMap map_low, const __grid_constant__ CUtensorMap map_up,
@@ -1081,6 +1160,9 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
     using S = Turned<CG, NT>;
     constexpr int STAGES = S::STAGES;
     constexpr int ROW_BYTES = BK * 2;  // of one row in a 64-deep block
+    constexpr int UP_CG = WIDE ? 1 : CG;  // (what warps of the CTA work on arrives at a barrier of the CTA)
+    constexpr int UP_AT = S::W_BYTES - BM * RANK_BLOCK * 4;  // where a stage holds up in 32 bits, behind what the copies bring
+    static_assert(UP_AT >= A_STAGE_BYTES && UP_AT % 1024 == 0, "a stage of ranks");
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Control *ctl = reinterpret_cast<Control *>(smem + STAGES * S::STAGE_BYTES);
@@ -1097,6 +1179,8 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&ctl->full[s], 1 + ROW_PRODUCERS * CG);
             mbar_init(&ctl->empty[s], 1);
+            mbar_init(&ctl->raw[s], 1);
+            mbar_init(&ctl->clean[s], SPLITTERS * CG);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&ctl->tmem_full[b], 1);
@@ -1163,19 +1247,25 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
                 for (int rb = 0; rb < p.rank_blocks; ++rb) {
                     mbar_wait(&ctl->empty[s], phase, wait_ctx, 0x110 | s);
                     uint8_t *dst = smem + s * S::STAGE_BYTES;
-                    if (leader) mbar_expect_tx(&ctl->full[s], CG * (up_bytes + S::X_BYTES));
+                    if constexpr (WIDE) {
+                        mbar_expect_tx(&ctl->raw[s], up_bytes + S::X_BYTES);
+                        if (leader) mbar_arrive(&ctl->full[s]);  // (keeps its phases in step; the issuer waits for `clean` too)
+                    } else if (leader) {
+                        mbar_expect_tx(&ctl->full[s], CG * (up_bytes + S::X_BYTES));
+                    }
+                    uint64_t *bar = WIDE ? &ctl->raw[s] : &ctl->full[s];
                     if (p.up_mn) {
 #pragma unroll
                         for (int j = 0; j < BM / 64; ++j)
-                            load_3d<CG>(dst + j * (RANK_BLOCK * 128), &map_up, &ctl->full[s], n0 + j * 64, rb * RANK_BLOCK, matrix);
+                            load_3d<UP_CG>(dst + j * (RANK_BLOCK * 128), &map_up, bar, n0 + j * 64, rb * RANK_BLOCK, matrix);
                     } else {
-                        load_3d<CG>(dst, &map_up, &ctl->full[s], rb * RANK_BLOCK, n0, matrix);
+                        load_3d<UP_CG>(dst, &map_up, bar, rb * RANK_BLOCK, n0, matrix);
                     }
                     next();
                 }
             }
         }
-    } else if (warp >= ROW_WARP && lane == 0) {
+    } else if (warp >= ROW_WARP && warp < SPLIT_WARP && lane == 0) {
         // -------------- TMA producers of the rows, of lhs and of (scales lhs . down) --------------
         // Where requests meet in a tile its rows are many small boxes: one lane's copies of them took 2300 cycles a stage, over
         // twice the products' time.  Four lanes share them: the halves of a stage, and every other box.
@@ -1249,7 +1339,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
                     uint8_t *dst = smem + s * S::STAGE_BYTES + S::W_BYTES;
                     if (warp == ROW_WARP) {
                         if (!waited) wait_parts();
-                        load_2d<CG>(dst, &map_low, &ctl->full[s], rb * BK, row);
+                        load_2d<UP_CG>(dst, &map_low, WIDE ? &ctl->raw[s] : &ctl->full[s], rb * (WIDE ? RANK_BLOCK : BK), row);
                     }
                     next();
                 }
@@ -1262,6 +1352,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
             const uint32_t smem_base = smem_u32(smem);
             const uint32_t up_step = p.up_mn ? UMMA_K * 128 : UMMA_K * 2, up_lbo = p.up_mn ? RANK_BLOCK * 128 : 16;
             uint32_t s = 0, phase = 0, acc_it = 0;
+            [[maybe_unused]] uint32_t clean_phases = 0;  // (a bit a stage, as in grad_kernel)
             bool ready = false;
             for (int tile = worker; tile < total; tile += workers, ++acc_it) {
                 int m, n;
@@ -1308,20 +1399,28 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
                         ended = true;
                     }
                     const Piece<STEP> piece(table[r], first, last);
-                    const uint32_t idesc_up = umma_instr_desc(BM * CG, piece.to - piece.from, p.bf16 != 0, p.up_mn != 0, false);
+                    const uint32_t idesc_up = WIDE ? umma_instr_desc_tf32(BM * CG, piece.to - piece.from)
+                                                   : umma_instr_desc(BM * CG, piece.to - piece.from, p.bf16 != 0, p.up_mn != 0, false);
                     const uint32_t tmem_piece = tmem_acc + (piece.from - first);
                     for (int rb = 0; rb < p.rank_blocks; ++rb) {
                         mbar_wait(&ctl->full[s], phase, wait_ctx, 0x310 | s);
+                        if constexpr (WIDE) {
+                            mbar_wait_cluster(&ctl->clean[s], (clean_phases >> s) & 1, wait_ctx, 0x700 | s);
+                            clean_phases ^= 1u << s;
+                        }
                         tcgen05_fence_after_sync();
-                        const uint32_t up_addr = smem_base + s * S::STAGE_BYTES;
-                        const uint32_t low_addr = up_addr + S::W_BYTES;
-                        const int steps = (min(RANK_BLOCK, p.rank - rb * RANK_BLOCK) + UMMA_K - 1) / UMMA_K;
+                        const uint32_t stage = smem_base + s * S::STAGE_BYTES, low_addr = stage + S::W_BYTES;
+                        constexpr int STEP_K = WIDE ? 8 : UMMA_K;
+                        const int steps = (min(RANK_BLOCK, p.rank - rb * RANK_BLOCK) + STEP_K - 1) / STEP_K;
                         for (int kk = 0; kk < steps; ++kk) {
-                            const uint64_t desc_up = umma_smem_desc(up_addr + kk * up_step, up_lbo, 1024);
+                            const uint64_t desc_up = WIDE ? umma_smem_desc(stage + UP_AT + kk * 32, 16, 1024) : umma_smem_desc(stage + kk * up_step, up_lbo, 1024);
 #pragma unroll
-                            for (int part = 0; part < 2; ++part)
-                                umma_ss<CG>(tmem_piece, desc_up,
-                                            umma_smem_desc(low_addr + part * (RANK_BLOCK * 2) + kk * (UMMA_K * 2), 16, 1024), idesc_up, 1u);
+                            for (int part = 0; part < 2; ++part) {
+                                if constexpr (WIDE)
+                                    umma_ss_tf32<CG>(tmem_piece, desc_up, umma_smem_desc(low_addr + part * S::X_BYTES + kk * 32, 16, 1024), idesc_up, 1u);
+                                else
+                                    umma_ss<CG>(tmem_piece, desc_up, umma_smem_desc(low_addr + part * (RANK_BLOCK * 2) + kk * (UMMA_K * 2), 16, 1024), idesc_up, 1u);
+                            }
                         }
                         if constexpr (CG == 1) umma_commit<1>(&ctl->empty[s]);
                         else umma_commit_pair_multicast(&ctl->empty[s], 0x3);
@@ -1334,6 +1433,37 @@ __global__ void __launch_bounds__(LORA_THREADS, 1)
                 ready = false;
                 if constexpr (CG == 1) umma_commit<1>(&ctl->tmem_full[buf]);
                 else umma_commit_pair_multicast(&ctl->tmem_full[buf], 0x3);
+            }
+        }
+    } else if (WIDE && warp >= SPLIT_WARP) {
+        // ------------- the adapters' operands: up in 32 bits, (scales lhs . down) in two parts -------------
+        const int thread = static_cast<int>(threadIdx.x) - SPLIT_WARP * 32;
+        const bool bf16 = p.bf16 != 0;
+        uint32_t it = 0, phases = 0;  // stages so far; a phase bit a stage
+        for (int tile = worker; tile < total; tile += workers) {
+            int m, n;
+            raster(tile, m_tiles, p.n_tiles, p.group_m, m, n);
+            const int first = m * NT, last = min(first + NT, columns);
+            it += p.k_blocks;
+            for (int r = run_at(table, runs, first); r < runs && table[r].tiles_before < last; ++r) {
+                if (table[r].matrix < 0) continue;
+                const Piece<STEP> piece(table[r], first, last);
+                for (int rb = 0; rb < p.rank_blocks; ++rb, ++it) {
+                    const uint32_t s = it % STAGES;
+                    mbar_wait_warp(&ctl->raw[s], (phases >> s) & 1, wait_ctx, 0x600 | s);
+                    phases ^= 1u << s;
+                    uint8_t *stage = smem + s * S::STAGE_BYTES;
+                    if (p.up_mn) widen_up<true>(stage, stage + UP_AT, thread, bf16);
+                    else widen_up<false>(stage, stage + UP_AT, thread, bf16);
+                    split_low(stage + S::W_BYTES, S::X_BYTES, (piece.to - piece.from) / CG, thread);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (leader) mbar_arrive(&ctl->clean[s]);
+                        else mbar_arrive_cluster(&ctl->clean[s], 0);
+                    }
+                    __syncwarp();
+                }
             }
         }
     } else if (warp >= 2 && warp < ROW_WARP) {
@@ -1439,7 +1569,7 @@ __device__ __forceinline__ void build_starts(const Offsets &offsets, int rows, i
 // warp 10 copies output_grad.
 //
 // In a pair the even CTA's barriers count both CTAs' copies, but each CTA has to overwrite its own rows: a ragged block is
-// therefore copied against a barrier of its own in each CTA (`ragged`), whose warp 11 overwrites the rows, ahead of the
+// therefore copied against a barrier of its own in each CTA (`raw`), whose warp 11 overwrites the rows, ahead of the
 // issuer like the copies, and arrives at the barrier that the issuer waits for (`clean`, in the even CTA).
 constexpr int OUT_BOX_BYTES = 32 * 64;  // 32 rows of 32 columns; two an epilogue warp, so that filling one hides the other's store
 
@@ -1494,7 +1624,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&ctl->full[s], 1);
             mbar_init(&ctl->empty[s], 1);
-            mbar_init(&ctl->ragged[s], 1);
+            mbar_init(&ctl->raw[s], 1);
             mbar_init(&ctl->clean[s], CG);
         }
         for (int b = 0; b < 2; ++b) {
@@ -1535,12 +1665,12 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
                 const bool ragged = at.length - k0 < BK && (at.length & (UMMA_K - 1)) != 0;
                 if (ragged) {
                     if (LHS) {
-                        mbar_expect_tx(&ctl->ragged[s], S::STAGE_BYTES);
+                        mbar_expect_tx(&ctl->raw[s], S::STAGE_BYTES);
                         if (leader) mbar_arrive(&ctl->full[s]);  // (keeps its phases in step; the issuer waits for `clean` too)
                     }
 #pragma unroll
                     for (int j = 0; j < COLS / 64; ++j)
-                        tma_load_2d(dst + j * S::BOX_BYTES, &map, &ctl->ragged[s], col0 + j * 64, at.begin + k0);
+                        tma_load_2d(dst + j * S::BOX_BYTES, &map, &ctl->raw[s], col0 + j * 64, at.begin + k0);
                 } else {
                     if (LHS && leader) mbar_expect_tx(&ctl->full[s], S::STAGE_BYTES * CG);
 #pragma unroll
@@ -1617,7 +1747,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
             if ((length & (UMMA_K - 1)) == 0) continue;
             const uint32_t s = (it - 1) % STAGES, phase = (phases >> s) & 1;
             phases ^= 1u << s;
-            mbar_wait_warp(&ctl->ragged[s], phase, wait_ctx, 0x600 | s);
+            mbar_wait_warp(&ctl->raw[s], phase, wait_ctx, 0x600 | s);
             const int first = length & (BK - 1), chunks = (UMMA_K - (length & (UMMA_K - 1))) * 8;  // 16-byte chunks of a box
             uint8_t *rows = smem + s * S::STAGE_BYTES + first * 128;
             for (int i = lane; i < chunks; i += 32)
@@ -1803,6 +1933,14 @@ int map_rows(const DeviceState &dev, CUtensorMap *map, int dtype, const void *da
     return make_tensor_map(dev, map, dtype, 2, data, dims, strides, box, true);
 }
 
+// 32-bit sums, a row's in whole blocks of RANK_BLOCK.
+int map_sums(const DeviceState &dev, CUtensorMap *map, const void *data, int64_t rows, int64_t pitch, uint32_t box_rows) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(pitch), static_cast<uint64_t>(rows)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(pitch) * 4};
+    const uint32_t box[2] = {RANK_BLOCK, box_rows};
+    return make_tensor_map(dev, map, NINETOOTHED_FLOAT32, 2, data, dims, strides, box, true);
+}
+
 // box_inner x box_outer boxes over one matrix at a time
 int map_matrices(const DeviceState &dev, CUtensorMap *map, int dtype, const Matrices &t, bool mn, uint32_t box_inner,
                  uint32_t box_outer) {
@@ -1854,22 +1992,22 @@ struct LoraMaps {
     CUtensorMap w, x, x32, x16, low, up;
 };
 
-template <int CG, int NT, bool W_MN>
+template <int CG, int NT, bool W_MN, bool WIDE>
 int launch_lora_kernel(cudaStream_t stream, const DeviceState &dev, const LoraMaps &maps, const Params &p, int64_t most_tiles) {
-    auto kernel = lora_kernel<CG, NT, W_MN>;
+    auto kernel = lora_kernel<CG, NT, W_MN, WIDE>;
     static_assert(turned_smem<CG, NT, false, false>(MAX_RUNS) <= MAX_SMEM, "shared memory per CTA");
     static thread_local int configured_device = -1;
     static thread_local int pairs = 0;
     if (configured_device != dev.device) {
         NT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SMEM)));
-        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, LORA_THREADS);
+        if constexpr (CG == 2) pairs = active_pairs(kernel, dev, lora_threads(WIDE));
         configured_device = dev.device;
     }
     const int workers = CG == 2 ? pairs : dev.sm_count;
     if (workers <= 0) return fail(NINETOOTHED_B200_ERR_DEVICE, "lora_matmul: no CTA pair fits this device");
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(most_tiles, workers) * CG));
-    config.blockDim = dim3(LORA_THREADS);
+    config.blockDim = dim3(lora_threads(WIDE));
     config.dynamicSmemBytes = turned_smem<CG, NT, false, false>(p.offsets.runs);
     config.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -1888,7 +2026,7 @@ int launch_lora_kernel(cudaStream_t stream, const DeviceState &dev, const LoraMa
 }
 
 // Tensor maps, then the launch.  up and low: null where there are no adapters.
-template <int CG, int NT>
+template <int CG, int NT, bool WIDE>
 int launch_lora(cudaStream_t stream, const DeviceState &dev, int dtype, Params &p, const void *lhs, int64_t lhs_stride0,
                 const Matrices &rhs, const Matrices *up, const void *low) {
     using S = Turned<CG, NT>;
@@ -1904,14 +2042,16 @@ int launch_lora(cudaStream_t stream, const DeviceState &dev, int dtype, Params &
     maps.up = maps.low = maps.x;
     if (up != nullptr) {
         p.up_mn = up->use_mn();
-        const int64_t pitch = p.rank_blocks * (2 * RANK_BLOCK);
+        const int64_t pitch = p.rank_blocks * RANK_BLOCK;
         if (int rc = map_matrices(dev, &maps.up, dtype, *up, p.up_mn, 64, p.up_mn ? RANK_BLOCK : BM)) return rc;
-        if (int rc = map_rows(dev, &maps.low, dtype, low, p.rows, pitch, pitch, BK, S::ROWS_CTA)) return rc;
+        if (int rc = WIDE ? map_sums(dev, &maps.low, low, p.rows, pitch, S::ROWS_CTA)
+                          : map_rows(dev, &maps.low, dtype, low, p.rows, 2 * pitch, 2 * pitch, BK, S::ROWS_CTA))
+            return rc;
     }
     const int64_t columns = p.rows + (16 * CG - 1) * static_cast<int64_t>(std::min(p.offsets.runs, p.rows));
     const int64_t most = (columns + NT - 1) / NT * p.n_tiles;
     if (most > INT_MAX / 16) return fail(NINETOOTHED_B200_ERR_SHAPE, "lora_matmul: too many tiles");
-    return mn ? launch_lora_kernel<CG, NT, true>(stream, dev, maps, p, most) : launch_lora_kernel<CG, NT, false>(stream, dev, maps, p, most);
+    return mn ? launch_lora_kernel<CG, NT, true, WIDE>(stream, dev, maps, p, most) : launch_lora_kernel<CG, NT, false, WIDE>(stream, dev, maps, p, most);
 }
 
 template <int CG, int NT, bool W_MN, bool SPLIT, Job JOB>
@@ -2211,7 +2351,7 @@ int launch_many(cudaStream_t stream, const DeviceState &dev, int dtype, Params &
         Params parts = p;
         parts.n = p.rank;
         parts.out = workspace;
-        parts.out_stride0 = p.rank_blocks * (2 * RANK_BLOCK);
+        parts.out_stride0 = p.rank_blocks * RANK_BLOCK;
         parts.out_stride1 = 1;
         const int64_t live = std::min(p.offsets.runs, p.rows), n_tiles = (p.rank + BM - 1) / BM;
         const int64_t blocks = (static_cast<int64_t>(p.k) + 2 * BK - 1) / (2 * BK), narrow = (live + p.rows / 64) * n_tiles;
@@ -2230,8 +2370,10 @@ int launch_many(cudaStream_t stream, const DeviceState &dev, int dtype, Params &
         return ((columns + width - 1) / width * ((p.n + width - 1) / width) + workers - 1) / workers;
     };
     if (1400 * waves(256, 32, dev.sm_count / 2) <= 1080 * waves(128, 16, dev.sm_count))
-        return launch_lora<2, 256>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, any ? &up : nullptr, workspace);
-    return launch_lora<1, 128>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, any ? &up : nullptr, workspace);
+        return p.bf16 ? launch_lora<2, 256, false>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, any ? &up : nullptr, workspace)
+                      : launch_lora<2, 256, true>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, any ? &up : nullptr, workspace);
+    return p.bf16 ? launch_lora<1, 128, false>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, any ? &up : nullptr, workspace)
+                  : launch_lora<1, 128, true>(stream, dev, dtype, p, lhs, lhs_stride0, rhs, any ? &up : nullptr, workspace);
 }
 
 int run_lora(cudaStream_t stream, const NineToothedTensor &lhs, const NineToothedTensor &rhs, const NineToothedTensor &down,

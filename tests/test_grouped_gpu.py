@@ -2,7 +2,7 @@
 
 Bounds: a sum of K products in fp32 is within K * 2^-23 of its terms' magnitudes (the tensor core may truncate where a
 rounding would take half of that), the one rounding at the store within half a step of the stored type, and the value
-between the adapters' two products, kept as two 16-bit parts, within half a step squared.
+between the adapters' two products within half a step squared (it is kept to 2^-22 of itself, fp16's half step squared).
 """
 
 import warnings
@@ -422,6 +422,27 @@ def test_an_infinite_row_stays_infinite(lengths, rank):
     assert (output[1] == float("inf")).all()
     output[1] = 0
     assert output.isfinite().all()
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("power", [18, -18])
+@pytest.mark.parametrize("lengths", [[3, 5], [200, 300], [1500, 900]], ids=str)
+def test_the_value_between_the_products_keeps_its_range(lengths, power, kind):
+    """scales (lhs . down) far above fp16's largest number, or among its smallest, and up the other way: exact to 2^-22 of that
+    value, however many rows the call has."""
+    lhs, rhs, down, up, scales, offsets, which = lora_inputs(lengths, [1, 0], 136, 520, 40, 2, kind)
+    scales = scales * 2.0 ** power
+    up = (up.float() * 2.0 ** (-power // 2)).to(kind)
+    from ninetoothed_b200.torch_ops import ops
+
+    output = torch.zeros(lhs.shape[0], 520, dtype=kind, device="cuda")
+    ops.lora_matmul(lhs, torch.zeros_like(rhs), down, up, scales, offsets, which, output)
+    k, rank, unit = 136, 40, 2.0 ** -23
+    for (a, b), adapter in zip(spans(offsets), which.tolist()):
+        x, d, u, s = lhs[a:b].double(), down[adapter].double(), up[adapter].double(), scales[adapter].double()
+        low, low_size = s * (x @ d), s * (x.abs() @ d.abs())
+        off = low_size * ((k + 1) * unit) + low.abs() * (2.0 ** -22 + (k + rank) * unit)
+        assert_within(output[a:b], low @ u, off @ u.abs())
 
 
 def test_lora_matmul_workspace_of_the_caller():
