@@ -56,8 +56,8 @@ constexpr int SPLIT_NT = 64;   // rows of a tile whose reduction a cluster share
 constexpr int FEW_RANK = 128;  // largest rank whose adapters' part may be computed a row at a time (see few_rows)
 constexpr int LOW_WARPS = 8;
 constexpr int LOW_CHUNK = LOW_WARPS * 256;  // terms of a partial sum of (lhs . down) there
-constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product elsewhere: one 128-byte swizzle row of
-                               // their values, which are pairs of bf16 (32 high parts, 32 low parts) or 32 bits wide
+constexpr int RANK_BLOCK = 32;  // ranks of one stage of the adapters' second product elsewhere: a 128-byte swizzle row of
+                               // values, which are pairs of bf16 (32 first parts, 32 rests) or 32 bits wide
 
 // A wait on a barrier tells a phase from the next one only, so no lane that goes through the ring of stages may fall a whole
 // round behind: every producer has a part in `full`, by bytes that it copies into the stage or by arriving.
@@ -265,12 +265,17 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
     return packed;
 }
 
-// A value as two numbers of eight bits each.
-struct Bf16Parts {
-    float high, low;
-    __device__ explicit Bf16Parts(float v) : high(__bfloat162float(__float2bfloat16_rn(v))) {
-        // (an infinite or NaN high part says it all; inf - inf must not turn it into NaN)
-        low = isfinite(high) ? v - high : 0.f;
+// A value as the sum of two numbers, its first `bits` bits and the rest (which the caller rounds), for a second product with each.
+// Where an element of up is infinite both products have to be infinite with the value's sign, so neither part is zero or of the
+// other sign: the first bits are cut off, not rounded, and a value that has no others is halved.  (Of values below 2^-100 the
+// second part may still be zero.)  Both parts of an infinity or NaN are the value.
+struct TwoParts {
+    float first, rest;
+    __device__ TwoParts(float v, int bits) {
+        first = __uint_as_float(__float_as_uint(v) & (0xffffffffu << (24 - bits)));
+        rest = v - first;
+        if (rest == 0.f) first = rest = 0.5f * v;
+        if (!isfinite(v)) first = rest = v;
     }
 };
 
@@ -733,7 +738,7 @@ __device__ __forceinline__ void store_turned(const uint32_t (&acc)[32], void *ou
 }
 
 // JOB_PARTS: a run's adapter's down is the matrix, and scales (lhs . down) leaves in blocks of 32 ranks, 32 bits a rank: of fp16
-// operands as it is, of bf16 ones as 32 high parts and 32 low parts (value = high + low to 2^-16, so that the second product runs
+// operands as it is, of bf16 ones as 32 first parts and 32 rests (their sum is the value to 2^-16, so that the second product runs
 // on the tensor cores without the rounding of one 16-bit operand; bf16 has the range of fp32, fp16 has not).  Ranks behind the
 // last are zero (of an infinite row or scale too).
 // JOB_FEW: the shared projection and the adapters of a call with few rows.  The epilogue's warps, idle while the tile's
@@ -960,18 +965,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                     }
                 } else if constexpr (PARTS) {
                     if (n - lane < n_end && bf16) {
-                        uint32_t low_part[32];
+                        uint32_t rest[32];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
                             const float v = n < p.n ? scale * __uint_as_float(acc[j]) : 0.f;
-                            const Bf16Parts parts(v);
-                            acc[j] = __float_as_uint(parts.high);
-                            low_part[j] = __float_as_uint(parts.low);
+                            const TwoParts parts(v, 8);
+                            acc[j] = __float_as_uint(parts.first);
+                            rest[j] = __float_as_uint(parts.rest);
                         }
                         uint16_t *block = static_cast<uint16_t *>(p.out) + n / RANK_BLOCK * RANK_BLOCK;
                         const int64_t pitch = 2 * p.out_stride0;
                         store_turned(acc, block, pitch, at.row0 + t0, at.rows - t0, at.row0 + t0 + 16, at.rows - t0 - 16, n, n_end, true);
-                        store_turned(low_part, block + RANK_BLOCK, pitch, at.row0 + t0, at.rows - t0, at.row0 + t0 + 16, at.rows - t0 - 16, n, n_end, true);
+                        store_turned(rest, block + RANK_BLOCK, pitch, at.row0 + t0, at.rows - t0, at.row0 + t0 + 16, at.rows - t0 - 16, n, n_end, true);
                     } else if (n - lane < n_end) {
                         float *out = static_cast<float *>(p.out) + (at.row0 + t0) * p.out_stride0 + n;
 #pragma unroll
@@ -1015,9 +1020,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                                 const float v = n < p.n ? scale * sum[j] : 0.f;
                                 if (bf16) {
                                     const int64_t to = 2 * row_at + n / RANK_BLOCK * (2 * RANK_BLOCK) + n % RANK_BLOCK;
-                                    const Bf16Parts parts(v);
-                                    store16(p.out, to, parts.high, true);
-                                    store16(p.out, to + RANK_BLOCK, parts.low, true);
+                                    const TwoParts parts(v, 8);
+                                    store16(p.out, to, parts.first, true);
+                                    store16(p.out, to + RANK_BLOCK, parts.rest, true);
                                 } else {
                                     static_cast<float *>(p.out)[row_at + n] = v;
                                 }
@@ -1126,17 +1131,16 @@ __device__ __forceinline__ void widen_up(const uint8_t *raw, uint8_t *wide, int 
 __device__ __forceinline__ void split_low(uint8_t *values, int second, int rows, int thread) {
     for (int i = thread; i < rows * (RANK_BLOCK / 4); i += SPLITTERS * 32) {
         float4 *at = reinterpret_cast<float4 *>(values) + i;
-        const auto high_of = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xffffe000u); };
-        const auto rest_of = [](float v, float high) {
-            uint32_t rest;
-            asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(rest) : "f"(v - high));
-            return isfinite(v) ? __uint_as_float(rest) : 0.f;  // (an infinite or NaN value's first part says it all)
+        const auto rounded = [](float v) {
+            uint32_t bits;
+            asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(bits) : "f"(v));
+            return __uint_as_float(bits);
         };
         const float4 v = *at;
-        const float4 high = make_float4(high_of(v.x), high_of(v.y), high_of(v.z), high_of(v.w));
-        *at = high;
+        const TwoParts x(v.x, 11), y(v.y, 11), z(v.z, 11), w(v.w, 11);
+        *at = make_float4(x.first, y.first, z.first, w.first);
         *reinterpret_cast<float4 *>(values + second + i * 16) =
-            make_float4(rest_of(v.x, high.x), rest_of(v.y, high.y), rest_of(v.z, high.z), rest_of(v.w, high.w));
+            make_float4(rounded(x.rest), rounded(y.rest), rounded(z.rest), rounded(w.rest));
     }
 }
 

@@ -425,19 +425,45 @@ def test_an_infinite_row_stays_infinite(lengths, rank):
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("whole", [False, True], ids=["any", "whole numbers"])
+@pytest.mark.parametrize("lengths, k, n", [([3, 5], 1288, 264), ([3, 5], 136, 264), ([200, 300], 136, 264), ([1500, 900], 136, 2056)],
+                         ids=str)
+def test_infinities_in_up(lengths, k, n, whole, kind):
+    """A value between the products times an infinity is an infinity of its sign (NaN for zero), also where the value is a short
+    number, and no other column changes."""
+    lhs, rhs, down, up, scales, offsets, which = lora_inputs(lengths, [1, 0], k, n, 40, 2, kind)
+    if whole:
+        lhs, down = (t.float().sign().mul(t.abs() > 0.03).to(kind) for t in (lhs, down))
+        scales = torch.ones_like(scales)
+    from ninetoothed_b200.torch_ops import ops
+
+    clean, output = (torch.zeros(lhs.shape[0], n, dtype=kind, device="cuda") for _ in range(2))
+    ops.lora_matmul(lhs, rhs, down, up, scales, offsets, which, clean)
+    for adapter, rank, column, value in ((0, 0, 7, "inf"), (0, 39, 8, "-inf"), (1, 17, n - 1, "inf"), (1, 31, 100, "-inf")):
+        up[adapter, rank, column] = float(value)
+    ops.lora_matmul(lhs, rhs, down, up, scales, offsets, which, output)
+    for (a, b), adapter in zip(spans(offsets), which.tolist()):
+        x = lhs[a:b].double()
+        exact = x @ rhs.double() + scales[adapter].double() * (x @ down[adapter].double()) @ up[adapter].double()
+        sick = up[adapter].isinf().any(0)
+        torch.testing.assert_close(output[a:b, sick].double(), exact[:, sick], rtol=0, atol=0, equal_nan=True)
+        assert torch.equal(output[a:b, ~sick], clean[a:b, ~sick])
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
 @pytest.mark.parametrize("power", [18, -18])
-@pytest.mark.parametrize("lengths", [[3, 5], [200, 300], [1500, 900]], ids=str)
-def test_the_value_between_the_products_keeps_its_range(lengths, power, kind):
+@pytest.mark.parametrize("lengths, k", [([3, 5], 1288), ([3, 5], 136), ([200, 300], 136), ([1500, 900], 136)], ids=str)
+def test_the_value_between_the_products_keeps_its_range(lengths, k, power, kind):
     """scales (lhs . down) far above fp16's largest number, or among its smallest, and up the other way: exact to 2^-22 of that
     value, however many rows the call has."""
-    lhs, rhs, down, up, scales, offsets, which = lora_inputs(lengths, [1, 0], 136, 520, 40, 2, kind)
+    lhs, rhs, down, up, scales, offsets, which = lora_inputs(lengths, [1, 0], k, 520, 40, 2, kind)
     scales = scales * 2.0 ** power
     up = (up.float() * 2.0 ** (-power // 2)).to(kind)
     from ninetoothed_b200.torch_ops import ops
 
     output = torch.zeros(lhs.shape[0], 520, dtype=kind, device="cuda")
     ops.lora_matmul(lhs, torch.zeros_like(rhs), down, up, scales, offsets, which, output)
-    k, rank, unit = 136, 40, 2.0 ** -23
+    rank, unit = 40, 2.0 ** -23
     for (a, b), adapter in zip(spans(offsets), which.tolist()):
         x, d, u, s = lhs[a:b].double(), down[adapter].double(), up[adapter].double(), scales[adapter].double()
         low, low_size = s * (x @ d), s * (x.abs() @ d.abs())
