@@ -12,7 +12,9 @@ There is no fallback: if the library is missing or a call fails, this raises.
 from __future__ import annotations
 
 import ctypes
+import os
 import pathlib
+import sys
 import threading
 import warnings
 
@@ -235,7 +237,19 @@ def warn_of_plain_launches():
     count = lib.ninetoothed_b200_plain_launches(0)
     if count != _plain_launches_seen:
         _plain_launches_seen = count
-        warnings.warn(lib.ninetoothed_b200_last_note().decode("utf-8", "replace"), SlowPathWarning, stacklevel=4)
+        warnings.warn(lib.ninetoothed_b200_last_note().decode("utf-8", "replace"), SlowPathWarning, stacklevel=_callers_level())
+
+
+_OWN_FILES = tuple(str(pathlib.Path(module_file).resolve().parent) + os.sep for module_file in (__file__, torch.__file__))
+
+
+def _callers_level() -> int:
+    """``stacklevel``, for a warning of the calling function, of the nearest frame outside this package and PyTorch: how many
+    frames lie between depends on whether a call came through the operators, in C++ or in Python, or to this module."""
+    level, frame = 1, sys._getframe(1)
+    while frame.f_back is not None and os.path.realpath(frame.f_code.co_filename).startswith(_OWN_FILES):
+        level, frame = level + 1, frame.f_back
+    return level
 
 
 def matmul(lhs, rhs, output):

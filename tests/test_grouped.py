@@ -1,6 +1,8 @@
 """What the products by runs of rows refuse, before anything touches a device."""
 
 import ctypes
+import inspect
+import pathlib
 
 import pytest
 import torch
@@ -44,6 +46,32 @@ def test_every_tensor_is_checked_for_rank_type_and_being_one(function, good):
                 function(**{**good, name: good[name].to(torch.int16)})
             with pytest.raises(RuntimeError, match="CUDA tensors only"):
                 function(**{**good, name: good[name].long()})
+
+
+def test_the_slow_path_warning_names_the_call(monkeypatch):
+    """Whatever frames of this package and of PyTorch lie between the call and the warning."""
+    class Library:
+        launches = 10 ** 9
+
+        def ninetoothed_b200_plain_launches(self, reset):
+            self.launches += 1
+            return self.launches
+
+        def ninetoothed_b200_last_note(self):
+            return b"slow"
+
+    fake = Library()
+    monkeypatch.setattr(_capi, "library", lambda: fake)
+    monkeypatch.setattr(_capi, "_plain_launches_seen", 0)
+    names = {"warn": _capi.warn_of_plain_launches}
+    inner, outer = pathlib.Path(_capi.__file__).with_name("torch_ops.py"), pathlib.Path(torch.__file__).with_name("_ops.py")
+    exec(compile("def through_package(): warn()", str(inner), "exec"), names)
+    exec(compile("def through_torch(): through_package()", str(outer), "exec"), names)
+    for call in (names["warn"], names["through_package"], names["through_torch"]):
+        with pytest.warns(_capi.SlowPathWarning, match="slow") as caught:
+            call()
+        assert caught[0].filename == __file__
+        assert caught[0].lineno == inspect.currentframe().f_lineno - 2
 
 
 def launch(name, tensors, *trailing):

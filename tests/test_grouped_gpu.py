@@ -5,6 +5,7 @@ rounding would take half of that), the one rounding at the store within half a s
 between the adapters' two products within half a step squared (it is kept to 2^-22 of itself, fp16's half step squared).
 """
 
+import inspect
 import warnings
 
 import pytest
@@ -126,6 +127,17 @@ def test_grouped_matmul_views_and_strided_bounds():
         first = output.clone()
         _capi.grouped_matmul(wide, rhs, offsets, output)
         check_grouped(wide, rhs, offsets, output, first)
+
+
+def test_the_slow_path_warning_names_the_operators_call():
+    from ninetoothed_b200 import _capi
+    from ninetoothed_b200.torch_ops import ops
+
+    lhs, rhs, offsets = normal(8, 40, 7), normal(9, 2, 7, 9), bounds_of([10, 30])
+    output = torch.empty(40, 9, dtype=torch.bfloat16, device="cuda")
+    with pytest.warns(_capi.SlowPathWarning) as caught:
+        ops.grouped_matmul(lhs, rhs, offsets, output)
+    assert (caught[0].filename, caught[0].lineno) == (__file__, inspect.currentframe().f_lineno - 1)
 
 
 @pytest.mark.parametrize("k, n", [(0, 8), (7, 9), (33, 70)])
