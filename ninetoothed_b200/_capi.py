@@ -23,6 +23,18 @@ import torch
 LIBRARY_PATH = pathlib.Path(__file__).resolve().parent / "lib" / "libninetoothed_b200.so"
 TORCH_LIBRARY_PATH = LIBRARY_PATH.with_name("libninetoothed_b200_torch.so")
 
+
+def torch_version_record() -> pathlib.Path:
+    """The file beside the operators' C++ library that names the PyTorch it was built with."""
+    return TORCH_LIBRARY_PATH.with_suffix(".torch-version")
+
+
+def torch_library_fits() -> bool:
+    """Whether the operators' C++ library is there and was built with this PyTorch, whose C++ interface it is tied to."""
+    record = torch_version_record()
+    return TORCH_LIBRARY_PATH.exists() and record.exists() and record.read_text().strip() == str(torch.__version__)
+
+
 # enum NineToothedDataType (same order as the reference, src/ninetoothed/aot.py:524-537)
 DTYPE_INDEX = {
     torch.int8: 0, torch.int16: 1, torch.int32: 2, torch.int64: 3,

@@ -88,16 +88,24 @@ def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
     header = INCLUDE_DIR / "ninetoothed_b200.h"
-    if force or not TORCH_LIBRARY.exists() or TORCH_LIBRARY.stat().st_mtime < max(TORCH_SOURCE.stat().st_mtime,
+    if force or not _torch_binding_fits() or TORCH_LIBRARY.stat().st_mtime < max(TORCH_SOURCE.stat().st_mtime,
                                                                                  header.stat().st_mtime):
         _build_torch_binding()
     return LIBRARY
+
+
+def _torch_binding_fits() -> bool:
+    from ninetoothed_b200 import _capi
+
+    return _capi.torch_library_fits()
 
 
 def _build_torch_binding() -> None:
     import sysconfig
 
     import torch
+
+    from ninetoothed_b200 import _capi
 
     torch_dir = pathlib.Path(torch.__file__).resolve().parent
     cuda_include = pathlib.Path(find_nvcc()).resolve().parent.parent / "include"
@@ -110,6 +118,7 @@ def _build_torch_binding() -> None:
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for {TORCH_SOURCE.name}:\n{proc.stdout}\n{proc.stderr}")
+    _capi.torch_version_record().write_text(f"{torch.__version__}\n")
 
 
 if __name__ == "__main__":

@@ -76,11 +76,11 @@ def _max_pool2d(input, output, window_height, window_width, ceil_mode):
 _LIBRARY.impl("matmul", _matmul, "CUDA")
 _LIBRARY.impl("bmm", _bmm, "CUDA")
 _LIBRARY.impl("addmm", _addmm, "CUDA")
-if _capi.TORCH_LIBRARY_PATH.exists():
+if _capi.torch_library_fits():
     # The products by runs of rows are small calls as often as not: their ordinary calls are marshalled in C++, which
-    # hands everything else to the functions above.
+    # hands everything else to the functions of the same names in `_capi`.
     torch.ops.load_library(str(_capi.TORCH_LIBRARY_PATH))
-else:  # (not built: these raise)
+else:  # (not built, or with another PyTorch: the same calls, marshalled in Python)
     _LIBRARY.impl("grouped_matmul", _grouped_matmul, "CUDA")
     _LIBRARY.impl("grouped_matmul_rhs_grad", _grouped_matmul_rhs_grad, "CUDA")
     _LIBRARY.impl("lora_matmul", _lora_matmul, "CUDA")

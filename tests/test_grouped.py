@@ -3,6 +3,8 @@
 import ctypes
 import inspect
 import pathlib
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -72,6 +74,29 @@ def test_the_slow_path_warning_names_the_call(monkeypatch):
             call()
         assert caught[0].filename == __file__
         assert caught[0].lineno == inspect.currentframe().f_lineno - 2
+
+
+def test_the_operators_library_is_tied_to_its_pytorch(monkeypatch, tmp_path):
+    assert _capi.torch_library_fits()  # as built
+    monkeypatch.setattr(_capi, "TORCH_LIBRARY_PATH", tmp_path / "lib.so")
+    assert not _capi.torch_library_fits()
+    _capi.TORCH_LIBRARY_PATH.write_bytes(b"no library")
+    assert not _capi.torch_library_fits()  # nothing says what it was built with
+    _capi.torch_version_record().write_text("0.1\n")
+    assert not _capi.torch_library_fits()
+    _capi.torch_version_record().write_text(f"{torch.__version__}\n")
+    assert _capi.torch_library_fits()
+
+
+def test_the_operators_import_beside_a_library_of_another_pytorch(tmp_path):
+    (tmp_path / "lib.so").write_bytes(b"no library")
+    (tmp_path / "lib.torch-version").write_text("0.1\n")
+    program = (f"import pathlib, torch; from ninetoothed_b200 import _capi\n"
+               f"_capi.TORCH_LIBRARY_PATH = pathlib.Path({str(tmp_path / 'lib.so')!r})\n"
+               "import ninetoothed_b200.torch_ops\n"
+               "for name in ('matmul', 'softmax', 'grouped_matmul', 'grouped_matmul_rhs_grad', 'lora_matmul'):\n"
+               "    assert torch._C._dispatch_has_kernel_for_dispatch_key(f'ninetoothed_b200::{name}', 'CUDA'), name\n")
+    subprocess.run([sys.executable, "-c", program], check=True, cwd=pathlib.Path(_capi.__file__).resolve().parent.parent)
 
 
 def launch(name, tensors, *trailing):
