@@ -2141,17 +2141,20 @@ int launch_grouped(cudaStream_t stream, const DeviceState &dev, int dtype, Param
 
 int64_t low_chunks(int64_t k) { return (k + LOW_CHUNK - 1) / LOW_CHUNK; }
 
-// Few rows, or requests of few rows each: the adapters' part costs no tile of its own and runs under the streaming of rhs, a
-// row at a time: 0.05 to 0.4 us a row, by the rank.  Otherwise a request takes at least 16 columns of a tile, whatever its
-// rows, and its second product half a microsecond of that tile.  What is hidden under the streaming of rhs, short for a small
-// k, is why the rank is weighed against k.  us this way / the other (rows in requests):
-//   4096 x 4096, rank 16: 16 in 1 15 / 24, 64 in 64 19 / 63, 256 in 64 48 / 64, in 16 47 / 32, 512 in 128 97 / 115, in 64 96 / 64,
-//   2048 in 2048 492 / 1616, 4096 in 2048 969 / 1632, 8192 in 2048 1912 / 1638
-//   4096 x 1024, rank 8: 2048 in 2048 170 / 669, 8192 in 2048 584 / 679
-//   4096 x 4096, rank 64: 1 in 1 16 / 25, 16 in 4 20 / 29, 64 in 64 37 / 74, 64 in 4 36 / 29
-//   1024 x 2048, rank 64: 1 in 1 21 / 12, 64 in 64 31 / 28, 128 in 128 30 / 42, in 32 29 / 25, 512 in 256 84 / 84
+// Few rows, or requests of few rows each: the adapters' part costs no tile of its own and runs under the streaming of rhs, a row
+// at a time, which takes about 5.5 ns x (rank + 22) a row.  Otherwise a request takes at least 16 columns of a tile, whatever its
+// rows, which is 0.8 us a request, 145 of those units.  The constant behind them is what the launch before the projection takes
+// more where it goes by tiles, 3600 units, or, where k is short beside the rank, what is missing of a streaming to run under.  All
+// three are fitted to these times in us, this way / the other (rows in requests, bf16):
+//   4096 x 4096, rank 16: 16 in 1 16 / 24, 64 in 64 21 / 63, 64 in 4 20 / 27, 256 in 64 48 / 64, 256 in 16 48 / 32,
+//   512 in 128 96 / 116, 512 in 64 96 / 65, 2048 in 2048 488 / 1623, 6000 in 2048 1394 / 1669, 8192 in 2048 1895 / 1661
+//   4096 x 4096, rank 8: 128 in 4 23 / 29, 256 in 4 43 / 28, 256 in 64 44 / 65
+//   4096 x 1024, rank 8: 2048 in 2048 166 / 654, 8192 in 2048 576 / 681
+//   4096 x 4096, rank 64: 1 in 1 19 / 25, 16 in 4 22 / 29, 64 in 64 39 / 73, 64 in 4 36 / 29, 1024 in 512 466 / 465
+//   1024 x 2048, rank 64: 1 in 1 21 / 12, 64 in 64 34 / 28, 128 in 128 32 / 44, 128 in 32 34 / 26, 512 in 256 88 / 86
+// (fp16 takes as long this way and 2 to 45 % longer the other, most for ranks that are much beside k.)
 bool few_rows(int64_t rows, int64_t k, int64_t rank, int64_t requests) {
-    return rank <= FEW_RANK && rows * rank < requests * (rank + 48) + (k >= 32 * rank ? 2048 : -64 * 48);
+    return rank <= FEW_RANK && rows * (rank + 22) < requests * 145 + (k >= 32 * rank ? 3600 : -4000);
 }
 
 size_t lora_workspace(int64_t rows, int64_t k, int64_t rank) {
