@@ -1920,13 +1920,10 @@ struct Matrices {
     int64_t count, rows, cols, stride0, stride1, stride2;
     bool mn() const { return rows_addressable(data, rows, cols, stride1, stride2); }
     bool k_major() const { return rows_addressable(data, cols, rows, stride2, stride1); }
-    bool batch_ok(bool as_mn) const {  // one matrix behind the other
-        const int64_t span = as_mn ? row_pitch(rows, cols, stride1) * (rows - 1) + cols
-                                   : row_pitch(cols, rows, stride2) * (cols - 1) + rows;
-        return count <= 1 || (stride0 % 8 == 0 && stride0 >= span && stride0 < (1LL << 38));
-    }
-    bool addressable() const { return (mn() && batch_ok(true)) || (k_major() && batch_ok(false)); }
-    bool use_mn() const { return mn() && batch_ok(true); }
+    // (matrices need not lie one behind the other: a weight held as [rows, count, cols] has its matrices between each other's rows)
+    bool batch_ok() const { return count <= 1 || (stride0 % 8 == 0 && stride0 > 0 && stride0 < (1LL << 38)); }
+    bool addressable() const { return (mn() || k_major()) && batch_ok(); }
+    bool use_mn() const { return mn() && batch_ok(); }
 };
 
 int map_rows(const DeviceState &dev, CUtensorMap *map, int dtype, const void *data, int64_t rows, int64_t cols,

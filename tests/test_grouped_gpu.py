@@ -129,6 +129,31 @@ def test_grouped_matmul_views_and_strided_bounds():
         check_grouped(wide, rhs, offsets, output, first)
 
 
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("lengths", [[3, 0, 5, 1], [150, 260, 0, 90], [900, 700, 45, 300]], ids=str)
+def test_matrices_between_each_others_rows(lengths, transposed):
+    """Matrices held with their index in the middle, which is how some checkpoints have them: on the tensor cores, as others."""
+    from ninetoothed_b200 import _capi
+
+    k, n, rank, rows = 264, 520, 24, sum(lengths)
+
+    def middle(t):  # the same matrices in memory as [rows, count, columns], either way round
+        if transposed:
+            return middle_of(t.transpose(1, 2)).transpose(1, 2)
+        return middle_of(t)
+
+    def middle_of(t):
+        return t.transpose(0, 1).contiguous().transpose(0, 1)
+
+    before = _capi.plain_launches()
+    lhs, grad, offsets = normal(110, rows, k), normal(111, rows, n), bounds_of(lengths)
+    run_grouped(lhs, middle(normal(112, 4, k, n)), offsets)
+    check_rhs_grad(lhs, grad, offsets, rhs_grad=middle_of(torch.full((4, k, n), float("nan"), dtype=torch.bfloat16, device="cuda")))
+    lhs, rhs, down, up, scales, offsets, which = lora_inputs(lengths, [1, 0, 2, 3], k, n, rank, 4, torch.bfloat16)
+    run_lora(lhs, rhs, middle(down), middle(up), scales, offsets, which)
+    assert _capi.plain_launches() == before
+
+
 def test_the_slow_path_warning_names_the_operators_call():
     from ninetoothed_b200 import _capi
     from ninetoothed_b200.torch_ops import ops
