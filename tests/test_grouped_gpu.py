@@ -382,6 +382,17 @@ def test_grouped_matmul_columns_end_in_a_pairs_first_half(lengths, k, n):
     run_grouped(normal(64, sum(lengths), k), normal(65, len(lengths), k, n), bounds_of(lengths))
 
 
+# One run with most of the rows among many short ones, which averages do not show.
+@pytest.mark.parametrize("lengths", [[4000] + [40] * 60, [7] * 100 + [3000, 0] + [1] * 40], ids=["ahead", "among"])
+def test_skewed_runs(lengths):
+    rows, groups = sum(lengths), len(lengths)
+    lhs, grad, offsets = normal(66, rows, 264), normal(67, rows, 520), bounds_of(lengths)
+    run_grouped(lhs, normal(68, groups, 264, 520), offsets)
+    check_rhs_grad(lhs, grad, offsets)
+    for kind in KINDS:
+        run_lora(*lora_inputs(lengths, [i % 9 - 1 for i in range(groups)], 264, 520, 24, 8, kind))
+
+
 # (256 x 256 tiles on pairs; 128 x 128 ones take less than half a wave by their rule)
 @pytest.mark.parametrize("lengths", [[64, 100, 1, 0, 129, 31, 512, 7], [128] * 8], ids=str)
 def test_rhs_grad_many_tiles_a_worker(lengths):
@@ -731,6 +742,23 @@ def test_different_products_on_two_streams_at_once():
     torch.cuda.synchronize()
     for got, expected in zip(together, alone):
         assert torch.equal(got, expected)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second device")
+def test_tensors_on_another_device_than_the_current_one():
+    from ninetoothed_b200.torch_ops import ops
+
+    lhs, rhs, down, up, scales, offsets, which = lora_inputs([100, 60, 7], [1, -1, 0], 136, 264, 24, 2, torch.bfloat16)
+    args = lhs, rhs, down, up, scales, offsets, which
+    expected = [torch.zeros(lhs.shape[0], n, dtype=lhs.dtype, device="cuda") for n in (24, 264)]
+    ops.grouped_matmul(lhs, down, offsets[:3], expected[0])
+    ops.lora_matmul(*args, expected[1])
+    far = [t.to("cuda:1") for t in args]
+    outputs = [torch.zeros_like(t, device="cuda:1") for t in expected]
+    ops.grouped_matmul(far[0], far[2], far[5][:3], outputs[0])
+    ops.lora_matmul(*far, outputs[1])
+    for got, want in zip(outputs, expected):
+        assert torch.equal(got.cpu(), want.cpu())
 
 
 def test_far_rows_pass_32_bit_offsets():
