@@ -312,12 +312,13 @@ __device__ __forceinline__ void load_3d(void *dst, const CUtensorMap *map, uint6
 // device has SMs.  Every CTA adds up and stores the tile's rows of one share, reading the others' partial sums, in
 // the order of the CTAs, from its own shared memory, where they have put them.
 //
-// What bounds it: for short runs the matrices, each read once: 64 of 2048 x 1024 for 256 rows take 45.8 us, 5.5 TB/s; the two
+// What bounds it: for short runs the matrices, each read once: 64 of 2048 x 1024 for 256 rows take 45.6 us, 5.5 TB/s; the two
 // 4096 x 2048 matrices of two single rows 11 us, of which 5 are their bytes and the rest a launch, a table and the first
-// copy's latency.  For long runs the products and the board's power: 16384 rows over 16 matrices of 2048 x 4096 take 190 us in a
-// short burst, 250 (1.1 PFLOP/s) back to back; 16 equal dense products of the same size as a library's batch 225.  In between
-// what an SM takes in: 64 bytes a cycle, which a 128 x 128 tile's 64 KB a block fill for twice as long as its products take, a
-// pair's 256 x 256 tile for as long.  64 runs of 256 rows on average against 2048 x 1024 matrices: 97 us, 3.8 TB/s.
+// copy's latency.  For long runs the products and the board's power: 16384 rows over 16 matrices of 2048 x 4096 take 206 us in a
+// short burst, with the tensor pipe at work 79 % of the time, 246 (1.1 PFLOP/s) back to back; 16 equal dense products of the same
+// size as a library's batch 225.  In between nothing is near its limit: 64 runs of 256 rows on average against 2048 x 1024
+// matrices take 98 us, with the tensor pipe at work 42 % of the time, 4 TB/s of DRAM, and 33 bytes a cycle into an SM, which
+// takes in 64; 29 runs of 172 rows against 1544 x 1160 ones 41 us, with 24 %, 2.6 TB/s and 20 bytes.
 // ---------------------------------------------------------------------------
 template <int CG, int NT>
 struct Turned {
@@ -1079,9 +1080,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 // 4096 rows towards the input (4096 x 2048, rank 64: 81.5 and 93.8).
 //
 // What bounds it: for long requests the products of the projection and the board's power, as in turned_kernel: 8192 rows of 6
-// requests, 4096 x 4096, rank 32, take 238 us back to back (1.17 PFLOP/s), some 15 of them the launch before, which reads lhs
-// once more.  For short ones the padding (rank 16): 2048 rows of 256 requests take 208 us, of 64 94.  Small calls are latency: of the 33 us of
-// 1533 rows of 40 requests (1000 x 2056, rank 24) 10 are the launch before, 5 this one's table and first copies.
+// requests, 4096 x 4096, rank 32, take 242 us back to back (1.16 PFLOP/s; fp16 267), some 15 of them the launch before, which
+// reads lhs once more.  For short ones the padding (rank 16): 2048 rows of 256 requests take 209 us, of 64 75.  Small calls are
+// latency: of the 37 us of 1533 rows of 40 requests (1000 x 2056, rank 24, fp16) 10 are the launch before, 5 this one's table and
+// first copies.
 // ---------------------------------------------------------------------------
 // The columns [from, to) of the padded space that a run of the table (tiles_before: its first column) has in [low, high).
 template <int STEP>
@@ -1532,9 +1534,11 @@ __global__ void __launch_bounds__(lora_threads(WIDE), 1)
 // last step is overwritten with zeros in BOTH operands (a zero in one alone would let a NaN or an infinity of the
 // neighbouring run through).
 //
-// What bounds it: for long runs the products and the board's power: 16384 rows in 16 runs, 2048 x 4096, take 229 us in a short
-// burst, 276 (1.0 PFLOP/s) back to back; 16 equal dense products as a library's batch 235.  For short ones the gradient's own
-// bytes, written once: 61 runs of 33 rows, 1024 x 776, take 46 us, 2.3 TB/s (a fill of the same size reaches 3.9).
+// What bounds it: for long runs the products, but not they alone: 16384 rows in 16 runs, 2048 x 4096, take 220 us in a short
+// burst, 14 more than as many products forward, with the tensor pipe at work 67 % of the time against 79 %, and 264 (1.0 PFLOP/s)
+// back to back, under the board's power limit; 16 equal dense products as a library's batch 235.  For short ones: 61 runs of 33
+// rows, 1024 x 776, take 46 us, of which a fill of the gradient takes 26; every tile is one ragged block that goes through copy,
+// clearing, products and stores in turn.
 // ---------------------------------------------------------------------------
 struct GradParams {
     Offsets offsets;
@@ -1811,7 +1815,6 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1)
                         tma_store_commit();
                     }
                 } else if (row < p.m) {
-                    
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
                         if (at.n0 + col + j < p.n)
